@@ -315,6 +315,108 @@ int rolaq_ipc_get_handle(const void* ptr, void* handle);
 int rolaq_ipc_open(const void* handle, void** ptr);
 int rolaq_ipc_close(void* ptr);
 
+/*
+ * The 4-bit latent cache (no counterpart in the reference, whose packed pool holds 2 bits:
+ * deployment/patches/rolaq_sglang.patch:123-133).  Uniform min/max codec of
+ * mla_quant/oscar.py:91-101 with 16 levels, no BF16 window rows.  One layer:
+ *   codes  uint8 [num_slots, D/2]      element 2i in the low half of byte i, 2i + 1 in the high half
+ *   params f32   [num_slots, D/128, 2] (scale, zero) of each 128 elements: value = (code - zero) * scale
+ *   rope   bf16  [num_slots, Dr]       k_pe, unquantized
+ * and, for the page selection (all three NULL where it is not used), one box per page of 64 slots:
+ *   box_center int8 / box_radius uint8 [num_slots/64, D + Dr] in units of 2^box_exps[page][part],
+ *   box_exps   int32 [num_slots/64, 2] (part 0: the latent, part 1: the rotary columns).
+ * D is 256 or 512, Dr 32 or 64, num_slots a multiple of 64; all buffers contiguous, 16-byte aligned.
+ */
+typedef struct rolaq_int4_cache {
+  uint8_t* codes;
+  float* params;
+  uint16_t* rope;
+  int8_t* box_center;
+  uint8_t* box_radius;
+  int32_t* box_exps;
+  int64_t num_slots;
+  int32_t latent_dim;
+  int32_t rope_dim;
+} rolaq_int4_cache;
+
+/*
+ * Quantise rows as they are written: per 128 elements lo / hi = min / max, scale = (hi - lo) / 15
+ * (1 where |hi - lo| <= 1e-8), code = clamp(round_half_even((x - lo) / scale), 0, 15), zero =
+ * -lo / scale, every operation one IEEE FP32 rounding; k_pe is copied.  Row i goes to slots[i]
+ * (outside [0, num_slots): skipped, ROLAQ_DEV_BAD_SLOT).  Rows that share a slot leave any one of them.
+ * A group that holds a NaN or an infinity gets params that read back as NaN.
+ *   c    bf16 or f32 (c_is_f32) [n, D], row stride ld_c;  k_pe bf16 [n, Dr], row stride ld_pe
+ *   (both 16-byte aligned, strides multiples of 8 elements);  slots int32 or int64 [n]
+ */
+int rolaq_int4_write(const void* c, int c_is_f32, int64_t ld_c, const uint16_t* k_pe, int64_t ld_pe,
+                     const void* slots, int slots_are_int64, int64_t n, const rolaq_int4_cache* cache, int32_t* err,
+                     cudaStream_t stream);
+
+/*
+ * Read rows back: out[i] = (code - zero) * scale of slots[i] (one FP32 rounding each, then BF16 unless
+ * out_is_f32), out_pe[i] = rope (NULL: not wanted).  A bad slot reads as zeros, ROLAQ_DEV_BAD_SLOT.
+ * out and out_pe 16-byte aligned, strides multiples of 8 elements.
+ */
+int rolaq_int4_read(const rolaq_int4_cache* cache, const void* slots, int slots_are_int64, int64_t n, void* out,
+                    int out_is_f32, int64_t ld_out, uint16_t* out_pe, int64_t ld_pe, int32_t* err,
+                    cudaStream_t stream);
+
+/*
+ * The boxes of the first counts[i] tokens (1..64) of pages[i], from what the cache holds: per column
+ * lo / hi = min / max of the values, unit = the least power of two (>= 2^-100) with
+ * max(|lo|, |hi|) <= 127 units over the part's columns (1 where all are 0), center =
+ * round_half_even((lo + hi) / 2 / unit), radius = ceil(max(hi / unit - center, center - lo / unit)):
+ * center -+ radius holds every token's value.  A page outside the pool or a count outside 1..64 is
+ * skipped, ROLAQ_DEV_BAD_PAGE.  A NaN value is passed over; a column that holds an infinity has no box.
+ */
+int rolaq_int4_update_boxes(const rolaq_int4_cache* cache, const int32_t* pages, const int32_t* counts, int64_t n,
+                            int32_t* err, cudaStream_t stream);
+
+/* The boxes of pages[i] as values: lo / hi f32 [n, D + Dr], row stride ld (zeros for a page outside
+ * the pool, ROLAQ_DEV_BAD_PAGE). */
+int rolaq_int4_read_boxes(const rolaq_int4_cache* cache, const int32_t* pages, int64_t n, float* lo, float* hi,
+                          int64_t ld, int32_t* err, cudaStream_t stream);
+
+/* Bytes of device scratch that rolaq_int4_decode / rolaq_int4_select_pages need for calls of up to
+ * this size (-1: sizes out of range).  Zeroed once by the caller before its first use; calls that
+ * overlap in time need one each. */
+int64_t rolaq_int4_workspace_bytes(int32_t batch, int32_t q_len, int32_t heads, int32_t latent_dim,
+                                   int32_t max_pages);
+
+/*
+ * Absorbed attention over the 4-bit cache: out = softmax(sm_scale q k^T) v with k = (latent, rope) and
+ * v = latent of each request's tokens, all heads sharing them.  Token t of request b lives in slot
+ * page_table[b][t / 64] * 64 + t % 64.  Query token t of q_len sits at position seq_lens[b] - q_len + t
+ * and attends to the positions up to its own; a row that sees none gets out = 0, lse = -inf.  Tokens of
+ * a page outside the pool take no weight (ROLAQ_DEV_BAD_PAGE); a length above 64 max_pages is cut
+ * (ROLAQ_DEV_BAD_REQ); what a page holds past a request's length is never used.
+ *   q    bf16 [B, q_len, H, D + Dr], strides in elements (multiples of 8), 16-byte aligned
+ *   out  bf16 [B, q_len, H, D], likewise;  lse f32 [B, q_len, H] contiguous (natural log; NULL: not wanted)
+ */
+int rolaq_int4_decode(const uint16_t* q, int64_t q_stride_b, int64_t q_stride_t, int64_t q_stride_h, int32_t batch,
+                      int32_t q_len, int32_t heads, const rolaq_int4_cache* cache, const int32_t* page_table,
+                      int64_t pt_stride, int32_t max_pages, const int32_t* seq_lens, float sm_scale, void* workspace,
+                      int64_t workspace_bytes, uint16_t* out, int64_t out_stride_b, int64_t out_stride_t,
+                      int64_t out_stride_h, float* lse, int32_t* err, cudaStream_t stream);
+
+/*
+ * The pages a single-token query attends to, as a page table that rolaq_int4_decode takes.  With n =
+ * ceil(seq_len / 64): all pages when n <= budget, else the first keep_first, the last keep_last and,
+ * of the others, those of the largest score, as many as the budget leaves (equal scores: the lower
+ * index).  score = max over the heads of the sum over both parts of
+ *   2^(e_q + e_page) (sum q8 center + sum |q8| radius),  q8 = round_half_even(q / 2^e_q) in -127..127,
+ * an upper bound, up to q's rounding, of any token's q k^T; the sums are whole numbers, so the choice
+ * does not depend on their order.  sel_table[b] holds the chosen pages in the request's order, then
+ * -1; sel_lens[b] = (chosen - 1) * 64 + tokens of the last page (0 for an empty request).
+ *   q  bf16 [B, H, D + Dr], strides in elements;  sel_table int32 [B, budget] (row stride sel_stride)
+ *   budget >= keep_first + keep_last, keep_last >= 1
+ */
+int rolaq_int4_select_pages(const uint16_t* q, int64_t q_stride_b, int64_t q_stride_h, int32_t batch, int32_t heads,
+                            const rolaq_int4_cache* cache, const int32_t* page_table, int64_t pt_stride,
+                            int32_t max_pages, const int32_t* seq_lens, int32_t budget, int32_t keep_first,
+                            int32_t keep_last, void* workspace, int64_t workspace_bytes, int32_t* sel_table,
+                            int64_t sel_stride, int32_t* sel_lens, int32_t* err, cudaStream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

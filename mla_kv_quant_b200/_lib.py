@@ -55,6 +55,13 @@ EXPORTS = (
     "rolaq_ipc_get_handle",
     "rolaq_ipc_open",
     "rolaq_ipc_close",
+    "rolaq_int4_write",
+    "rolaq_int4_read",
+    "rolaq_int4_update_boxes",
+    "rolaq_int4_read_boxes",
+    "rolaq_int4_workspace_bytes",
+    "rolaq_int4_decode",
+    "rolaq_int4_select_pages",
 )
 
 
@@ -86,6 +93,22 @@ class Codec(ctypes.Structure):
         ("scale_factor", ctypes.c_float),
         ("zero_const", ctypes.c_float),
         ("family", ctypes.c_int32),
+    ]
+
+
+class Int4Cache(ctypes.Structure):
+    """``rolaq_int4_cache``."""
+
+    _fields_ = [
+        ("codes", ctypes.c_void_p),
+        ("params", ctypes.c_void_p),
+        ("rope", ctypes.c_void_p),
+        ("box_center", ctypes.c_void_p),
+        ("box_radius", ctypes.c_void_p),
+        ("box_exps", ctypes.c_void_p),
+        ("num_slots", ctypes.c_int64),
+        ("latent_dim", ctypes.c_int32),
+        ("rope_dim", ctypes.c_int32),
     ]
 
 
@@ -138,6 +161,19 @@ _SIGS = {
     "rolaq_ipc_get_handle": (INT, [P, P]),
     "rolaq_ipc_open": (INT, [P, ctypes.POINTER(ctypes.c_void_p)]),
     "rolaq_ipc_close": (INT, [P]),
+    "rolaq_int4_write": (INT, [P, INT, I64, P, I64, P, INT, I64, P, P, P]),
+    "rolaq_int4_read": (INT, [P, P, INT, I64, P, INT, I64, P, I64, P, P]),
+    "rolaq_int4_update_boxes": (INT, [P, P, P, I64, P, P]),
+    "rolaq_int4_read_boxes": (INT, [P, P, I64, P, P, I64, P, P]),
+    "rolaq_int4_workspace_bytes": (I64, [I32, I32, I32, I32, I32]),
+    "rolaq_int4_decode": (
+        INT,
+        [P, I64, I64, I64, I32, I32, I32, P, P, I64, I32, P, F32, P, I64, P, I64, I64, I64, P, P, P],
+    ),
+    "rolaq_int4_select_pages": (
+        INT,
+        [P, I64, I64, I32, I32, P, P, I64, I32, P, I32, I32, I32, P, I64, P, I64, P, P, P],
+    ),
 }
 
 

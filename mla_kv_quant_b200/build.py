@@ -21,8 +21,9 @@ ROOT = PKG.parent
 CSRC = PKG / "csrc"
 OUT_DIR = PKG / "_lib"
 LIB = OUT_DIR / "librolaq_b200.so"
-SOURCES = ["abi.cu", "writer.cu", "codec.cu", "decode.cu", "decode_tc.cu", "proj.cu", "window.cu", "peer.cu"]
-HEADERS = ["common.cuh", "kernels.cuh", "merge.cuh"]
+SOURCES = ["abi.cu", "writer.cu", "codec.cu", "decode.cu", "decode_tc.cu", "proj.cu", "window.cu", "peer.cu",
+           "int4_abi.cu", "int4_store.cu", "int4_decode.cu", "int4_select.cu"]
+HEADERS = ["common.cuh", "kernels.cuh", "merge.cuh", "abi.cuh", "int4.cuh"]
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 
 

@@ -6,6 +6,7 @@
 #include <cstring>
 #include <mutex>
 
+#include "abi.cuh"
 #include "kernels.cuh"
 
 namespace rolaq {
@@ -29,13 +30,7 @@ int sm_count() {
   return n > 0 ? n : 148;
 }
 
-}  // namespace rolaq
-
-using namespace rolaq;
-
-namespace {
-
-thread_local char g_msg[512] = "";
+static thread_local char g_msg[512] = "";
 
 int fail(int code, const char* fmt, ...) {
   va_list ap;
@@ -45,7 +40,19 @@ int fail(int code, const char* fmt, ...) {
   return code;
 }
 
-bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
+int cuda_rc(int rc, const char* what) {
+  if (rc == ROLAQ_ECUDA) {
+    cudaError_t e = cudaGetLastError();
+    return fail(ROLAQ_ECUDA, "%s: %s", what, cudaGetErrorString(e));
+  }
+  return rc;
+}
+
+}  // namespace rolaq
+
+using namespace rolaq;
+
+namespace {
 
 int check_cache(const rolaq_layer_cache* c, bool need_window, bool need_rope = true) {
   if (c == nullptr) return fail(ROLAQ_EINVAL, "cache is NULL");
@@ -75,14 +82,6 @@ int codec_ok(const rolaq_codec& k) {
   if (!(k.threshold > 0.f) || !(k.scale_factor > 0.f) || !(k.threshold < 1e30f) || !(k.scale_factor < 1e30f))
     return fail(ROLAQ_EINVAL, "codec threshold and scale_factor must be finite and > 0");
   return ROLAQ_OK;
-}
-
-int cuda_rc(int rc, const char* what) {
-  if (rc == ROLAQ_ECUDA) {
-    cudaError_t e = cudaGetLastError();
-    return fail(ROLAQ_ECUDA, "%s: %s", what, cudaGetErrorString(e));
-  }
-  return rc;
 }
 
 }  // namespace
