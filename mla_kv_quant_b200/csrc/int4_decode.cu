@@ -1,102 +1,681 @@
 // Absorbed attention over the 4-bit latent cache.
 //
-// One CTA per query row (query token and head) and request; its warps take the request's tokens in
-// turn.  A lane holds D/32 latent columns (one group's) and Dr/32 rotary ones; the running maximum
-// and sum of the softmax stay in registers, the warps' results are joined at the end.
+// With value (c - z) s of a 4-bit code c, per 128-element group g of a token t:
+//   q . k_t = sum_g s_gt (q_g . c_gt - z_gt sum q_g) + q_pe . k_pe_t
+//   sum_t P_t v_t = sum_t (P_t s_gt) c_gt - sum_t (P_t s_gt) z_gt
+// so both contractions run on the raw codes, which tensor cores take after one AND per register:
+//   - as E4M3 bytes the patterns 0..15 are c 2^-9 exactly: QK^T is m16n8k32 of the query in two E4M3
+//     terms (hi + lo, exact for BF16 within 2^10 of the row's largest element, 2^-18 of it below);
+//   - as FP16 halves the patterns c and 16 c are (16) c 2^-24 exactly: PV is m16n8k16 of P s in FP16
+//     (11 bits), the factor 16 of odd elements taken out of the result.
+// The rotary part is m16n8k16 in BF16.  All accumulate in FP32.
+//
+// A CTA holds 16 query rows (query tokens x heads) and walks the pages of one or more requests; a page
+// (64 tokens) is one pipeline stage (TMA, 128-byte swizzle, so that ldmatrix reads without conflicts).
+// Each of the 8 warps scores 8 of the page's tokens, weighs them against a reference maximum that moves
+// only when a score passes it by 2^10, and writes P s of each group to shared memory; then each warp
+// adds D/8 latent columns of the page.  Scores of page i + 1 and sums of page i share an iteration, with
+// one barrier, which also carries the vote on moving the references.
+//
+// The pages of all requests are dealt to the CTAs in one equal run each (a run may begin or end inside
+// a request); what is cut is joined by merge_kernel by log-sum-exp.
+#include <algorithm>
+
 #include "int4.cuh"
+#include "kernels.cuh"
 
 namespace rolaq {
 namespace i4 {
 namespace {
 
-constexpr int kWarps = 8;
+constexpr int kThreads = 256, kWarps = 8;
+constexpr int kRows = 16;        // query rows of a CTA
+constexpr int kMinPages = 2;     // least run of pages worth a CTA of its own
+constexpr float kSlack = 10.f;   // log2 of how far a weight may pass its reference
+constexpr float kScaleSlack = 16.f;
+constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
 template <int D, int DR>
-__global__ void __launch_bounds__(kWarps * 32) decode_kernel(DecodeArgs a) {
-  constexpr int E = D / 32, R = DR / 32;  // columns of a lane: E * lane .. and D + R * lane ..
-  __shared__ float part_o[kWarps][D], part_m[kWarps], part_l[kWarps];
-  const int warp = threadIdx.x / 32, lane = threadIdx.x & 31;
-  const int t = blockIdx.x / a.heads, h = blockIdx.x % a.heads, b = blockIdx.y;
-  int len = a.seq_lens[b];
-  if (len > a.max_pages * kPage) {
-    if (threadIdx.x == 0) report(a.err, ROLAQ_DEV_BAD_REQ);
-    len = a.max_pages * kPage;
+struct Cfg {
+  static constexpr int NG = D / kGroup;             // groups of a token
+  static constexpr int CODES = kPage * D / 2, ROPE = kPage * DR * 2, PARAMS = kPage * NG * 8;
+  static constexpr int STAGE = CODES + ROPE + PARAMS;
+  static constexpr int STAGES = D == 512 ? 7 : 12;
+  static constexpr int PBUF = NG * kRows * kPage * 2;  // P s of a page: [group][row][token] FP16
+  static constexpr int SMEM = 1024 + STAGES * STAGE + 2 * PBUF;
+  static constexpr int NT = D / 64;                 // 8-column tiles of a warp's share
+};
+
+__device__ __forceinline__ int pages_of(const DecodeArgs& a, int b) {
+  const int64_t len = min(static_cast<int64_t>(a.seq_lens[b]), static_cast<int64_t>(a.max_pages) * kPage);
+  return len <= 0 ? 0 : static_cast<int>((len + kPage - 1) / kPage);
+}
+
+// Runs are equal shares of the `total` pages: run r of n begins at page total * r / n.
+__device__ __forceinline__ int runs_of(int64_t total, int groups) {
+  return static_cast<int>(min(static_cast<int64_t>(groups), max(int64_t(1), (total + kMinPages - 1) / kMinPages)));
+}
+
+__device__ __forceinline__ void ldsm_x4(uint32_t addr, uint32_t (&r)[4]) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr));
+}
+__device__ __forceinline__ void ldsm_x4_t(uint32_t addr, uint32_t (&r)[4]) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr));
+}
+__device__ __forceinline__ void mma_e4m3(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k32.row.col.f32.e4m3.e4m3.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+      "{%0, %1, %2, %3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint32_t pack_half2(float lo, float hi) {
+  const __half2 h = __floats2half2_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+// The shared-memory offset of 16-byte chunk `chunk` of row `row` under TMA's swizzles.
+__device__ __forceinline__ uint32_t sw128(int row, int chunk) { return row * 128 + ((chunk ^ (row & 7)) << 4); }
+__device__ __forceinline__ uint32_t sw64(int row, int chunk) { return row * 64 + ((chunk ^ ((row >> 1) & 3)) << 4); }
+
+// Sum over a warp's quads' four lanes / maximum over them (lanes that share a row).
+__device__ __forceinline__ float quad_sum(float v) {
+  v += __shfl_xor_sync(0xFFFFFFFFu, v, 1);
+  return v + __shfl_xor_sync(0xFFFFFFFFu, v, 2);
+}
+__device__ __forceinline__ float quad_max(float v) {
+  v = fmaxf(v, __shfl_xor_sync(0xFFFFFFFFu, v, 1));
+  return fmaxf(v, __shfl_xor_sync(0xFFFFFFFFu, v, 2));
+}
+
+// Exclusive prefix over the CTA's threads of v; the total in `total`.
+__device__ __forceinline__ int64_t block_scan(int64_t v, int64_t& total, int64_t* sm) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x / 32;
+  int64_t x = v;
+#pragma unroll
+  for (int o = 1; o < 32; o *= 2) {
+    const int64_t y = __shfl_up_sync(0xFFFFFFFFu, x, o);
+    if (lane >= o) x += y;
   }
-  const int seen = len - a.q_len + t + 1;
-  const uint16_t* qrow = a.q + b * a.q_sb + t * a.q_st + h * a.q_sh;
-  float q[E], q_pe[R], o[E] = {};
-#pragma unroll
-  for (int i = 0; i < E; ++i) q[i] = bf16_lo(qrow[E * lane + i]);
-#pragma unroll
-  for (int i = 0; i < R; ++i) q_pe[i] = bf16_lo(qrow[D + R * lane + i]);
-  float m = -INFINITY, l = 0.f;
-  for (int tok = warp; tok < seen; tok += kWarps) {
-    const int64_t page = a.page_table[b * a.pt_stride + tok / kPage];
-    if (page < 0 || page >= a.cache.num_slots / kPage) {
-      if (lane == 0) report(a.err, ROLAQ_DEV_BAD_PAGE);
-      continue;
-    }
-    const int64_t slot = page * kPage + tok % kPage;
-    const float2 p = reinterpret_cast<const float2*>(a.cache.params)[slot * (D / kGroup) + lane * E / kGroup];
-    float v[E], s = 0.f;
-#pragma unroll
-    for (int k = 0; k < E / 8; ++k) {
-      const uint32_t w = reinterpret_cast<const uint32_t*>(a.cache.codes)[slot * (D / 8) + lane * (E / 8) + k];
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        v[8 * k + i] = value((w >> (4 * i)) & 15u, p.x, p.y);
-        s += q[8 * k + i] * v[8 * k + i];
-      }
-    }
-#pragma unroll
-    for (int i = 0; i < R; ++i) s += q_pe[i] * bf16_lo(a.cache.rope[slot * DR + R * lane + i]);
-#pragma unroll
-    for (int k = 16; k >= 1; k /= 2) s += __shfl_xor_sync(0xFFFFFFFFu, s, k);
-    s *= a.sm_scale;
-    const float m_new = fmaxf(m, s);
-    const float keep = m == -INFINITY ? 0.f : expf(m - m_new), e = expf(s - m_new);
-    l = l * keep + e;
-#pragma unroll
-    for (int i = 0; i < E; ++i) o[i] = o[i] * keep + e * v[i];
-    m = m_new;
-  }
-#pragma unroll
-  for (int i = 0; i < E; ++i) part_o[warp][E * lane + i] = o[i];
-  if (lane == 0) part_m[warp] = m, part_l[warp] = l;
+  if (lane == 31) sm[warp] = x;
   __syncthreads();
-  float top = -INFINITY, sum = 0.f;
-  for (int k = 0; k < kWarps; ++k) top = fmaxf(top, part_m[k]);
-  float share[kWarps];
+  int64_t before = 0;
+  total = 0;
 #pragma unroll
   for (int k = 0; k < kWarps; ++k) {
-    share[k] = part_m[k] == -INFINITY ? 0.f : expf(part_m[k] - top);
-    sum += share[k] * part_l[k];
+    if (k < warp) before += sm[k];
+    total += sm[k];
   }
-  uint16_t* out = a.out + b * a.o_sb + t * a.o_st + h * a.o_sh;
-  for (int c = threadIdx.x; c < D; c += kWarps * 32) {
-    float x = 0.f;
-    for (int k = 0; k < kWarps; ++k) x += share[k] * part_o[k][c];
-    out[c] = __bfloat16_as_ushort(__float2bfloat16_rn(sum == 0.f ? 0.f : x / sum));
+  return before + x - v;
+}
+
+struct Partials {
+  float* o;    // [2 * groups * row blocks][16][D], normalised
+  float* lse;  // [2 * groups * row blocks][16], natural log
+};
+
+template <int D, int DR>
+__global__ void __launch_bounds__(kThreads, 1)
+    decode_kernel(const __grid_constant__ CUtensorMap map_codes, const __grid_constant__ CUtensorMap map_rope,
+                  const DecodeArgs a, const Partials part, const int groups, const int blocks) {
+  using C = Cfg<D, DR>;
+  constexpr int NG = C::NG, NCH = D / 32, KR = DR / 16;
+  extern __shared__ char raw[];
+  char* smem = reinterpret_cast<char*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
+  char* pbuf = smem + C::STAGES * C::STAGE;
+  __shared__ uint64_t full[C::STAGES];
+  __shared__ int bad_page[C::STAGES];
+  __shared__ int64_t scan[kWarps];
+  __shared__ int start[2];
+  __shared__ float unit[NG];                 // 2^-e of each group's scales
+  __shared__ float red_m[kWarps][kRows], red_s[kWarps][NG], red_z[kWarps][kRows][NG];
+
+  const int tid = threadIdx.x, warp = tid / 32, lane = tid & 31, g = lane >> 2, j = lane & 3;
+  const int block = blockIdx.x % blocks, group = blockIdx.x / blocks;
+  const uint32_t stages = smem_u32(smem), pbufs = smem_u32(pbuf);
+  grid_launch_dependents();
+
+  // ---- this CTA's run of pages ----
+  const int per = (a.batch + kThreads - 1) / kThreads;
+  int64_t mine = 0, total;
+  for (int b = tid * per; b < min(a.batch, (tid + 1) * per); ++b) mine += pages_of(a, b);
+  if (tid == 0) {
+    for (int s = 0; s < C::STAGES; ++s) mbar_init(&full[s], 1);
+    fence_mbar_init();
   }
-  if (threadIdx.x == 0 && a.lse)
-    a.lse[(static_cast<int64_t>(b) * a.q_len + t) * a.heads + h] = sum == 0.f ? -INFINITY : top + logf(sum);
+  int64_t before = block_scan(mine, total, scan);
+  const int runs = runs_of(total, groups);
+  if (group >= runs || total == 0) return;
+  const int64_t u0 = total * group / runs;
+  const int n_units = static_cast<int>(total * (group + 1) / runs - u0);
+  if (before <= u0 && u0 < before + mine) {
+    int b = tid * per;
+    for (int n; before + (n = pages_of(a, b)) <= u0; ++b) before += n;
+    start[0] = b;
+    start[1] = static_cast<int>(u0 - before);
+  }
+  __syncthreads();
+  int seg_b = start[0], seg_p = start[1];
+
+  // ---- the page stream (thread 0): stage k holds unit k of the run ----
+  const int pool_pages = static_cast<int>(a.cache.num_slots / kPage);
+  int load_b = seg_b, load_p = seg_p, load_n = 0, load_id = 0, loaded = 0;
+  auto next_id = [&]() {  // the page that (load_b, load_p) names, requested an iteration ahead of its use
+    while (load_p >= load_n) {
+      if (load_n != 0) ++load_b, load_p = 0;
+      load_n = pages_of(a, load_b);
+      if (load_n == 0) ++load_b, load_p = 0;
+    }
+    load_id = a.page_table[load_b * a.pt_stride + load_p++];
+  };
+  auto load = [&]() {
+    const int s = loaded % C::STAGES;
+    const bool ok = load_id >= 0 && load_id < pool_pages;
+    const int page = ok ? load_id : 0;
+    char* dst = smem + s * C::STAGE;
+    bad_page[s] = !ok;
+    if (!ok) report(a.err, ROLAQ_DEV_BAD_PAGE);
+    mbar_expect_tx(&full[s], C::STAGE);
+#pragma unroll
+    for (int k = 0; k < D / 256; ++k) tma_load_2d(dst + k * 8192, &map_codes, &full[s], k * 128, page * kPage);
+    tma_load_2d(dst + C::CODES, &map_rope, &full[s], 0, page * kPage);
+    bulk_load(dst + C::CODES + C::ROPE, a.cache.params + static_cast<int64_t>(page) * (kPage * NG * 2), C::PARAMS,
+              &full[s]);
+    if (++loaded < n_units) next_id();
+  };
+  if (tid == 0) {
+    prefetch_tensormap(&map_codes);
+    prefetch_tensormap(&map_rope);
+    next_id();
+    while (loaded < min(n_units, C::STAGES)) load();
+  }
+
+  bool healthy = true;
+  const float qk_scale = a.sm_scale * kLog2e;
+  int unit_at = 0;  // units of the run done
+  while (unit_at < n_units) {
+    int seg_pages = pages_of(a, seg_b);
+    if (seg_pages == 0) {
+      ++seg_b;
+      continue;
+    }
+    const int p_end = min(seg_pages, seg_p + n_units - unit_at);
+    int len = min(static_cast<int64_t>(a.seq_lens[seg_b]), static_cast<int64_t>(a.max_pages) * kPage);
+    if (tid == 0 && len != a.seq_lens[seg_b]) report(a.err, ROLAQ_DEV_BAD_REQ);
+    const int lim_min = len - a.q_len + 1;
+
+    // ---- the query: two rows per thread (g and g + 8), two E4M3 terms, rotary part in BF16 ----
+    uint32_t q_hi[NCH][4], q_lo[NCH][4], q_pe[KR][4];
+    float q_sum[2][NG], row_scale[2];
+    int lim[2];
+#pragma unroll
+    for (int r = 0; r < 2; ++r) {
+      const int row = block * kRows + g + 8 * r;
+      const bool live = row < a.q_len * a.heads;
+      const int t = live ? row / a.heads : 0, h = live ? row % a.heads : 0;
+      lim[r] = live ? lim_min + t : 0;
+      const uint16_t* src = a.q + seg_b * a.q_sb + t * a.q_st + h * a.q_sh;
+      float top = 0.f, odd = 0.f;
+#pragma unroll
+      for (int c = 0; c < NCH; ++c) {
+        const uint4 w = live ? *reinterpret_cast<const uint4*>(src + 32 * c + 8 * j) : make_uint4(0, 0, 0, 0);
+        const uint32_t v[4] = {w.x, w.y, w.z, w.w};
+        // kept raw until the row's largest element is known
+        q_hi[c][r] = v[0], q_hi[c][r + 2] = v[1], q_lo[c][r] = v[2], q_lo[c][r + 2] = v[3];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          top = fmaxf(top, fmaxf(fabsf(bf16_lo(v[k])), fabsf(bf16_hi(v[k]))));
+          odd += bf16_lo(v[k]) * 0.f + bf16_hi(v[k]) * 0.f;  // NaN where an element is no finite number
+        }
+      }
+      top = quad_max(top);
+      odd = quad_sum(odd);
+      // 2^k with top 2^k in [128, 256)
+      const int k = min(max(7 - (static_cast<int>(__float_as_uint(top) >> 23) - 127), -118), 118);
+      const float up = top > 0.f ? pow2(k) : 1.f;
+      row_scale[r] = odd != 0.f ? __int_as_float(0x7FC00000) : qk_scale * 512.f / up;
+#pragma unroll
+      for (int c = 0; c < NCH; ++c) {
+        const uint32_t v[4] = {q_hi[c][r], q_hi[c][r + 2], q_lo[c][r], q_lo[c][r + 2]};
+        uint32_t hi[2] = {0, 0}, lo[2] = {0, 0};  // even elements, odd elements
+        float sum = 0.f;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float x0 = bf16_lo(v[e]) * up, x1 = bf16_hi(v[e]) * up;
+          const uint32_t h2 = f32x2_to_e4m3x2(x0, x1);
+          const float2 f = __half22float2(e4m3x2_to_half2(h2));
+          const uint32_t l2 = f32x2_to_e4m3x2(x0 - f.x, x1 - f.y);
+          const float2 fl = __half22float2(e4m3x2_to_half2(l2));
+          sum += (f.x + fl.x) + (f.y + fl.y);
+          hi[0] |= (h2 & 0xFFu) << (8 * e), hi[1] |= (h2 >> 8) << (8 * e);
+          lo[0] |= (l2 & 0xFFu) << (8 * e), lo[1] |= (l2 >> 8) << (8 * e);
+        }
+        q_hi[c][r] = hi[0], q_hi[c][r + 2] = hi[1], q_lo[c][r] = lo[0], q_lo[c][r + 2] = lo[1];
+        q_sum[r][c / 4] = (c % 4 == 0 ? 0.f : q_sum[r][c / 4]) + sum;
+      }
+#pragma unroll
+      for (int k2 = 0; k2 < NG; ++k2) q_sum[r][k2] = quad_sum(q_sum[r][k2]) * (1.f / 512.f);
+#pragma unroll
+      for (int c = 0; c < KR; ++c) {
+        q_pe[c][r] = live ? *reinterpret_cast<const uint32_t*>(src + D + 16 * c + 2 * j) : 0;
+        q_pe[c][r + 2] = live ? *reinterpret_cast<const uint32_t*>(src + D + 16 * c + 8 + 2 * j) : 0;
+      }
+    }
+
+    float acc[C::NT][4], zsum[2][NG], l_sum[2] = {0.f, 0.f}, m_ref[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+    for (int n = 0; n < C::NT; ++n)
+#pragma unroll
+      for (int k = 0; k < 4; ++k) acc[n][k] = 0.f;
+#pragma unroll
+    for (int k = 0; k < NG; ++k) zsum[0][k] = zsum[1][k] = 0.f;
+    if (tid < NG) unit[tid] = 0.f;
+    __syncthreads();
+
+    float s_val[4], s_tok[2][NG], z_tok[2][NG], p_val[4];  // scores, params and weights of the warp's 8 tokens
+
+    // Scores of a page: rows (g, g + 8) x tokens (8 warp + 2 j, + 1), in log2 units.
+    auto score = [&](int at, int p) {
+      const uint32_t st = stages + (at % C::STAGES) * C::STAGE;
+      float c_acc[NG][4], r_acc[4] = {0.f, 0.f, 0.f, 0.f};
+      const int row = 8 * warp + (lane & 7);
+#pragma unroll
+      for (int k = 0; k < NG; ++k) {
+        c_acc[k][0] = c_acc[k][1] = c_acc[k][2] = c_acc[k][3] = 0.f;
+        uint32_t w[4];
+        ldsm_x4(st + (k / 2) * 8192 + sw128(row, (k & 1) * 4 + (lane >> 3)), w);
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          const uint32_t b0 = w[c] & 0x0F0F0F0Fu, b1 = (w[c] >> 4) & 0x0F0F0F0Fu;
+          mma_e4m3(c_acc[k], q_hi[4 * k + c], b0, b1);
+          mma_e4m3(c_acc[k], q_lo[4 * k + c], b0, b1);
+        }
+      }
+#pragma unroll
+      for (int c = 0; c < KR; c += 2) {
+        uint32_t w[4];
+        const uint32_t base = st + C::CODES;
+        ldsm_x4(base + (DR == 64 ? sw128(row, 2 * c + (lane >> 3)) : sw64(row, 2 * c + (lane >> 3))), w);
+        mma_bf16_16816(r_acc, q_pe[c][0], q_pe[c][1], q_pe[c][2], q_pe[c][3], w[0], w[1]);
+        mma_bf16_16816(r_acc, q_pe[c + 1][0], q_pe[c + 1][1], q_pe[c + 1][2], q_pe[c + 1][3], w[2], w[3]);
+      }
+      const float4* par = reinterpret_cast<const float4*>(smem + (at % C::STAGES) * C::STAGE + C::CODES + C::ROPE) +
+                          (8 * warp + 2 * j) * (NG / 2);
+#pragma unroll
+      for (int t = 0; t < 2; ++t)
+#pragma unroll
+        for (int k = 0; k < NG; k += 2) {
+          const float4 v = par[t * (NG / 2) + k / 2];
+          s_tok[t][k] = v.x, z_tok[t][k] = v.y, s_tok[t][k + 1] = v.z, z_tok[t][k + 1] = v.w;
+        }
+#pragma unroll
+      for (int x = 0; x < 4; ++x) {
+        float s = 0.f;
+#pragma unroll
+        for (int k = 0; k < NG; ++k) s = fmaf(s_tok[x & 1][k], fmaf(-z_tok[x & 1][k], q_sum[x >> 1][k], c_acc[k][x]), s);
+        s_val[x] = fmaf(s, row_scale[x >> 1], r_acc[x] * qk_scale);
+      }
+      const int bad = bad_page[at % C::STAGES];
+      if ((p + 1) * kPage > lim_min || bad) {  // the request's end, or a page that is not there
+        const int tok = p * kPage + 8 * warp + 2 * j;
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+          if (tok + t >= len || bad)
+#pragma unroll
+            for (int k = 0; k < NG; ++k) s_tok[t][k] = z_tok[t][k] = 0.f;
+#pragma unroll
+          for (int r = 0; r < 2; ++r)
+            if (tok + t >= lim[r] || bad) s_val[2 * r + t] = -INFINITY;
+        }
+      }
+    };
+
+    // Weights against the present references, times each group's scale, to shared memory; true where a
+    // score or a scale has left its reference behind.
+    auto weigh = [&](int at) {
+      bool need = false;
+#pragma unroll
+      for (int x = 0; x < 4; ++x) {
+        const float m = m_ref[x >> 1];
+        need |= s_val[x] > m + kSlack;
+        p_val[x] = ex2_approx(s_val[x] - (m == -INFINITY ? 0.f : m));
+      }
+      char* dst = pbuf + (at & 1) * C::PBUF + 4 * j;
+#pragma unroll
+      for (int k = 0; k < NG; ++k) {
+        const float u = unit[k], s0 = s_tok[0][k] * u, s1 = s_tok[1][k] * u;
+        need |= fmaxf(fabsf(s0), fabsf(s1)) > kScaleSlack;
+#pragma unroll
+        for (int r = 0; r < 2; ++r)
+          *reinterpret_cast<uint32_t*>(dst + k * (kRows * 128) + sw128(g + 8 * r, warp)) =
+              pack_half2(p_val[2 * r] * s0, p_val[2 * r + 1] * s1);
+      }
+      return need;
+    };
+
+    // New references (all threads): the page's maxima, the sums so far brought to them.
+    auto move_references = [&](int at) {
+#pragma unroll
+      for (int r = 0; r < 2; ++r) {
+        const float m = quad_max(fmaxf(s_val[2 * r], s_val[2 * r + 1]));
+        if (j == 0) red_m[warp][g + 8 * r] = m;
+      }
+#pragma unroll
+      for (int k = 0; k < NG; ++k) {
+        const float s = quad_max(fmaxf(fabsf(s_tok[0][k]), fabsf(s_tok[1][k])));
+        if (lane == 0) red_s[warp][k] = s;
+      }
+      __syncthreads();
+      float keep[2], keep_u[NG];
+#pragma unroll
+      for (int r = 0; r < 2; ++r) {
+        float m = m_ref[r];
+        for (int w = 0; w < kWarps; ++w) m = fmaxf(m, red_m[w][g + 8 * r]);
+        keep[r] = m_ref[r] == m ? 1.f : ex2_approx(m_ref[r] - m);
+        m_ref[r] = m;
+        l_sum[r] *= keep[r];
+      }
+      float u_new[NG];
+#pragma unroll
+      for (int k = 0; k < NG; ++k) {
+        float s = 0.f;
+        for (int w = 0; w < kWarps; ++w) s = fmaxf(s, red_s[w][k]);
+        const float u = unit[k];
+        u_new[k] = u;
+        if (s > 0.f && (u == 0.f || s * u > kScaleSlack))
+          u_new[k] = pow2(min(max(127 - static_cast<int>(__float_as_uint(s) >> 23), -120), 120));
+        keep_u[k] = u == 0.f ? 1.f : u_new[k] / u;
+        zsum[0][k] *= keep[0] * keep_u[k];
+        zsum[1][k] *= keep[1] * keep_u[k];
+      }
+      const int own = warp * NG / kWarps;
+      float ku = keep_u[0];
+#pragma unroll
+      for (int k = 1; k < NG; ++k) ku = own == k ? keep_u[k] : ku;
+#pragma unroll
+      for (int n = 0; n < C::NT; ++n)
+#pragma unroll
+        for (int x = 0; x < 4; ++x) acc[n][x] *= keep[x >> 1] * ku;
+      __syncthreads();
+      if (tid < NG) {
+        float u = u_new[0];
+#pragma unroll
+        for (int k = 1; k < NG; ++k) u = tid == k ? u_new[k] : u;
+        unit[tid] = u;
+      }
+      __syncthreads();
+      weigh(at);
+      __syncthreads();
+    };
+
+    // After the references stand: the denominators and the zeros' share.
+    auto add_weights = [&]() {
+      l_sum[0] += p_val[0] + p_val[1];
+      l_sum[1] += p_val[2] + p_val[3];
+#pragma unroll
+      for (int k = 0; k < NG; ++k) {
+        const float u = unit[k];
+        const float a0 = s_tok[0][k] * u * z_tok[0][k], a1 = s_tok[1][k] * u * z_tok[1][k];
+        zsum[0][k] = fmaf(p_val[0], a0, fmaf(p_val[1], a1, zsum[0][k]));
+        zsum[1][k] = fmaf(p_val[2], a0, fmaf(p_val[3], a1, zsum[1][k]));
+      }
+    };
+
+    // The warp's D/8 latent columns of a page: acc += (P s) c.
+    auto gather = [&](int at) {
+      const uint32_t st = stages + (at % C::STAGES) * C::STAGE;
+      const uint32_t pb = pbufs + (at & 1) * C::PBUF + (warp * NG / kWarps) * (kRows * 128);
+#pragma unroll
+      for (int kk = 0; kk < 4; kk += 2) {
+        uint32_t w[2][4], pa[2][4];
+        if constexpr (D == 512) {  // 64 columns: two 16-byte chunks, 16 tokens each
+#pragma unroll
+          for (int i = 0; i < 2; ++i)
+            ldsm_x4_t(st + (warp / 4) * 8192 + sw128((kk + i) * 16 + (lane & 15), 2 * (warp & 3) + (lane >> 4)), w[i]);
+        } else {  // 32 columns: one chunk, 32 tokens
+          ldsm_x4_t(st + sw128(kk * 16 + lane, warp), w[0]);
+        }
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+          ldsm_x4(pb + sw128((lane & 8) + (lane & 7), 2 * (kk + i) + (lane >> 4)), pa[i]);
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+          for (int c = 0; c < D / 256; ++c) {
+            const uint32_t x = D == 512 ? w[i][2 * c] : w[0][2 * i], y = D == 512 ? w[i][2 * c + 1] : w[0][2 * i + 1];
+            const uint32_t x8 = x >> 8, y8 = y >> 8;
+            mma_f16_16816(acc[4 * c], pa[i][0], pa[i][1], pa[i][2], pa[i][3], x & 0x000F000Fu, y & 0x000F000Fu);
+            mma_f16_16816(acc[4 * c + 1], pa[i][0], pa[i][1], pa[i][2], pa[i][3], x & 0x00F000F0u, y & 0x00F000F0u);
+            mma_f16_16816(acc[4 * c + 2], pa[i][0], pa[i][1], pa[i][2], pa[i][3], x8 & 0x000F000Fu, y8 & 0x000F000Fu);
+            mma_f16_16816(acc[4 * c + 3], pa[i][0], pa[i][1], pa[i][2], pa[i][3], x8 & 0x00F000F0u, y8 & 0x00F000F0u);
+          }
+      }
+    };
+    auto wait_for = [&](int at) {
+      if (healthy) healthy = mbar_wait(&full[at % C::STAGES], (at / C::STAGES) & 1, a.err);
+    };
+
+    // ---- the pages ----
+    wait_for(unit_at);
+    score(unit_at, seg_p);
+    if (__syncthreads_or(weigh(unit_at))) move_references(unit_at);
+    add_weights();
+    for (int p = seg_p; p < p_end; ++p, ++unit_at) {
+      bool need = false;
+      const bool more = p + 1 < p_end;
+      if (more) {
+        wait_for(unit_at + 1);
+        score(unit_at + 1, p + 1);
+      }
+      gather(unit_at);
+      if (more) need = weigh(unit_at + 1);
+      const bool move = __syncthreads_or(need);
+      if (tid == 0 && loaded < n_units) load();
+      if (move) move_references(unit_at + 1);
+      if (more) add_weights();
+    }
+
+    // ---- the rows' results ----
+#pragma unroll
+    for (int r = 0; r < 2; ++r) {
+      l_sum[r] = quad_sum(l_sum[r]);
+      if (j == 0) red_m[warp][g + 8 * r] = l_sum[r];
+#pragma unroll
+      for (int k = 0; k < NG; ++k) {
+        const float z = quad_sum(zsum[r][k]);
+        if (j == 0) red_z[warp][g + 8 * r][k] = z;
+      }
+    }
+    __syncthreads();
+    const bool whole = seg_p == 0 && p_end == seg_pages;
+    const int own = warp * NG / kWarps;
+    const float u = unit[own], inv_u = u == 0.f ? 0.f : 1.f / u;
+    // a cut request's partial: slot 0 where the run begins in (or with) this request, else 1
+    const int64_t slot = (static_cast<int64_t>(2 * group + (unit_at - (p_end - seg_p) == 0 ? 0 : 1)) * blocks + block) * kRows;
+#pragma unroll
+    for (int r = 0; r < 2; ++r) {
+      const int row = block * kRows + g + 8 * r;
+      float l = 0.f, z = 0.f;
+      for (int w = 0; w < kWarps; ++w) l += red_m[w][g + 8 * r], z += red_z[w][g + 8 * r][own];
+      const float inv = l == 0.f ? 0.f : inv_u / l;
+      const float lse = l == 0.f ? -INFINITY : (m_ref[r] + log2f(l)) * kLn2;
+      float v[D / 256][8];
+#pragma unroll
+      for (int c = 0; c < D / 256; ++c)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+          for (int k = 0; k < 2; ++k)
+            v[c][4 * k + i] = fmaf(acc[4 * c + i][2 * r + k], i & 1 ? 1048576.f : 16777216.f, -z) * inv;
+      const int col = warp * (D / 8) + 8 * j;
+      if (whole) {
+        if (row < a.q_len * a.heads) {
+          const int t = row / a.heads, h = row % a.heads;
+          uint16_t* out = a.out + seg_b * a.o_sb + t * a.o_st + h * a.o_sh + col;
+#pragma unroll
+          for (int c = 0; c < D / 256; ++c)
+            *reinterpret_cast<uint4*>(out + 32 * c) =
+                make_uint4(pack_bf16x2(v[c][0], v[c][1]), pack_bf16x2(v[c][2], v[c][3]), pack_bf16x2(v[c][4], v[c][5]),
+                           pack_bf16x2(v[c][6], v[c][7]));
+          if (a.lse && warp == 0 && j == 0) a.lse[(static_cast<int64_t>(seg_b) * a.q_len + t) * a.heads + h] = lse;
+        }
+      } else {
+        float* out = part.o + (slot + g + 8 * r) * D + col;
+#pragma unroll
+        for (int c = 0; c < D / 256; ++c) {
+          reinterpret_cast<float4*>(out + 32 * c)[0] = make_float4(v[c][0], v[c][1], v[c][2], v[c][3]);
+          reinterpret_cast<float4*>(out + 32 * c)[1] = make_float4(v[c][4], v[c][5], v[c][6], v[c][7]);
+        }
+        if (warp == 0 && j == 0) part.lse[slot + g + 8 * r] = lse;
+      }
+    }
+    __syncthreads();
+    ++seg_b;
+    seg_p = 0;
+  }
+}
+
+// Joins the partials of the requests that more than one run holds, and writes the rows of requests
+// without a token.  WARPS warps share the partials of 128 columns of one row.
+template <int D, int WARPS>
+__global__ void __launch_bounds__(kThreads) merge_kernel(const DecodeArgs a, const Partials part, const int groups,
+                                                         const int blocks) {
+  constexpr int CHUNKS = D / 128, TASKS = kWarps / WARPS;
+  __shared__ int64_t scan[kWarps], scan2[kWarps];
+  __shared__ float4 red[kWarps][32];
+  const int tid = threadIdx.x, warp = tid / 32, lane = tid & 31, b = blockIdx.y;
+  int64_t sum = 0, below = 0, total, first;
+  for (int i = tid; i < a.batch; i += kThreads) {
+    const int n = pages_of(a, i);
+    sum += n;
+    if (i < b) below += n;
+  }
+  block_scan(sum, total, scan);
+  block_scan(below, first, scan2);
+  const int pages = pages_of(a, b);
+  const int runs = runs_of(total, groups);
+  // the runs that hold the request's first and last page
+  int64_t r0 = 0, r1 = 0;
+  if (pages > 0) {
+    r0 = first * runs / total;
+    while (total * (r0 + 1) / runs <= first) ++r0;
+    r1 = (first + pages - 1) * runs / total;
+    while (total * (r1 + 1) / runs <= first + pages - 1) ++r1;
+  }
+  const int n = pages == 0 ? 0 : static_cast<int>(r1 - r0 + 1);
+  if (n == 1) return;
+  const int task = blockIdx.x * TASKS + warp / WARPS, row = task / CHUNKS, col = (task % CHUNKS) * 128 + 4 * lane;
+  const bool live = row < a.q_len * a.heads;
+  const int share = warp % WARPS;
+  // partial i is run r0 + i's: its first piece, but for a first run that begins in an earlier request
+  const bool late = n > 0 && total * r0 / runs < first;
+  auto slot = [&](int i) {
+    return (static_cast<int64_t>(2 * (r0 + i) + (i == 0 && late ? 1 : 0)) * blocks + row / kRows) * kRows + row % kRows;
+  };
+  grid_dependency_wait();
+  float top = -INFINITY, den = 0.f;
+  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+  if (live) {
+    bool odd = false;
+    for (int i = lane; i < n; i += 32) {
+      const float l = part.lse[slot(i)];
+      odd |= l != l;
+      top = fmaxf(top, l);
+    }
+    top = warp_max_f32(top);
+    if (__any_sync(0xFFFFFFFFu, odd)) top = __int_as_float(0x7FC00000);
+    for (int i = share; i < n; i += WARPS) {
+      const float l = part.lse[slot(i)];
+      if (l == -INFINITY) continue;
+      const float w = ex2_approx((l - top) * kLog2e);
+      const float4 v = *reinterpret_cast<const float4*>(part.o + slot(i) * D + col);
+      den += w;
+      acc.x = fmaf(w, v.x, acc.x), acc.y = fmaf(w, v.y, acc.y), acc.z = fmaf(w, v.z, acc.z), acc.w = fmaf(w, v.w, acc.w);
+    }
+  }
+  if constexpr (WARPS > 1) {
+    __shared__ float dens[kWarps];
+    red[warp][lane] = acc;
+    if (lane == 0) dens[warp] = den;
+    __syncthreads();
+    if (share != 0) return;
+    for (int k = 1; k < WARPS; ++k) {
+      const float4 v = red[warp + k][lane];
+      acc.x += v.x, acc.y += v.y, acc.z += v.z, acc.w += v.w;
+      den += dens[warp + k];
+    }
+  }
+  if (!live) return;
+  const float inv = den == 0.f ? 0.f : 1.f / den;
+  const int t = row / a.heads, h = row % a.heads;
+  *reinterpret_cast<uint2*>(a.out + b * a.o_sb + t * a.o_st + h * a.o_sh + col) =
+      make_uint2(pack_bf16x2(acc.x * inv, acc.y * inv), pack_bf16x2(acc.z * inv, acc.w * inv));
+  if (a.lse && col == 0)
+    a.lse[(static_cast<int64_t>(b) * a.q_len + t) * a.heads + h] = den == 0.f ? -INFINITY : top + logf(den);
+}
+
+int row_blocks(int q_len, int heads) { return (q_len * heads + kRows - 1) / kRows; }
+
+// Runs of pages per row block: one CTA a multiprocessor.
+int run_groups(int blocks) { return std::max(1, sm_count() / blocks); }
+
+bool encode(CUtensorMap* map, const void* base, CUtensorMapDataType type, uint64_t width, uint64_t rows,
+            uint64_t row_bytes, uint32_t box_width, CUtensorMapSwizzle swizzle) {
+  const EncodeTiledFn fn = encode_fn();
+  const cuuint64_t dims[2] = {width, rows}, strides[1] = {row_bytes};
+  const cuuint32_t box[2] = {box_width, kPage}, step[2] = {1, 1};
+  return fn != nullptr && fn(map, type, 2, const_cast<void*>(base), dims, strides, box, step,
+                             CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+template <int D, int DR>
+int launch(const DecodeArgs& a, cudaStream_t s) {
+  using C = Cfg<D, DR>;
+  CUtensorMap codes, rope;
+  if (!encode(&codes, a.cache.codes, CU_TENSOR_MAP_DATA_TYPE_UINT8, D / 2, a.cache.num_slots, D / 2, 128,
+              CU_TENSOR_MAP_SWIZZLE_128B) ||
+      !encode(&rope, a.cache.rope, CU_TENSOR_MAP_DATA_TYPE_UINT16, DR, a.cache.num_slots, DR * 2, DR,
+              DR == 64 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B))
+    return ROLAQ_ECUDA;
+  const int blocks = row_blocks(a.q_len, a.heads), groups = run_groups(blocks);
+  Partials part;
+  part.o = reinterpret_cast<float*>(static_cast<char*>(a.workspace) + kHeaderBytes);
+  part.lse = part.o + int64_t(2) * groups * blocks * kRows * D;
+  if (cudaFuncSetAttribute(decode_kernel<D, DR>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM) != cudaSuccess)
+    return ROLAQ_ECUDA;
+  decode_kernel<D, DR><<<groups * blocks, kThreads, C::SMEM, s>>>(codes, rope, a, part, groups, blocks);
+  if (cudaGetLastError() != cudaSuccess) return ROLAQ_ECUDA;
+
+  // Few requests are cut into many partials: all warps of a CTA share a row's then.
+  const bool wide = groups >= 8 * a.batch;
+  const int tasks = a.q_len * a.heads * (D / 128), per_cta = wide ? 1 : kWarps;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((tasks + per_cta - 1) / per_cta, a.batch);
+  cfg.blockDim = dim3(kThreads);
+  cfg.stream = s;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  const auto kernel = wide ? merge_kernel<D, kWarps> : merge_kernel<D, 1>;
+  return cudaLaunchKernelEx(&cfg, kernel, a, part, groups, blocks) == cudaSuccess ? ROLAQ_OK : ROLAQ_ECUDA;
 }
 
 }  // namespace
 
-int64_t decode_workspace(int batch, int q_len, int heads, int d) { return kHeaderBytes; }
+int64_t decode_workspace(int batch, int q_len, int heads, int d) {
+  const int blocks = row_blocks(q_len, heads);
+  return kHeaderBytes + int64_t(2) * run_groups(blocks) * blocks * kRows * (d + 1) * 4;
+}
 
 int launch_decode(const DecodeArgs& a, cudaStream_t s) {
-  const dim3 grid(a.q_len * a.heads, a.batch);
-  if (a.cache.latent_dim == 512 && a.cache.rope_dim == 64)
-    decode_kernel<512, 64><<<grid, kWarps * 32, 0, s>>>(a);
-  else if (a.cache.latent_dim == 512)
-    decode_kernel<512, 32><<<grid, kWarps * 32, 0, s>>>(a);
-  else if (a.cache.rope_dim == 64)
-    decode_kernel<256, 64><<<grid, kWarps * 32, 0, s>>>(a);
-  else
-    decode_kernel<256, 32><<<grid, kWarps * 32, 0, s>>>(a);
-  return cudaGetLastError() == cudaSuccess ? ROLAQ_OK : ROLAQ_ECUDA;
+  if (a.cache.latent_dim == 512) return a.cache.rope_dim == 64 ? launch<512, 64>(a, s) : launch<512, 32>(a, s);
+  return a.cache.rope_dim == 64 ? launch<256, 64>(a, s) : launch<256, 32>(a, s);
 }
 
 }  // namespace i4
