@@ -4,11 +4,10 @@
 //   q . k_t = sum_g s_gt (q_g . c_gt - z_gt sum q_g) + q_pe . k_pe_t
 //   sum_t P_t v_t = sum_t (P_t s_gt) c_gt - sum_t (P_t s_gt) z_gt
 // so both contractions run on the raw codes, which tensor cores take after one AND per register:
-//   - as E4M3 bytes the patterns 0..15 are c 2^-9 exactly: QK^T is m16n8k32 of the query in two E4M3
-//     terms (hi + lo, exact for BF16 within 2^10 of the row's largest element, 2^-18 of it below);
-//   - as FP16 halves the patterns c and 16 c are (16) c 2^-24 exactly: PV is m16n8k16 of P s in FP16
-//     (11 bits), the factor 16 of odd elements taken out of the result.
-// The rotary part is m16n8k16 in BF16.  All accumulate in FP32.
+// the FP16 patterns 0..15 and 16 * (0..15) are c 2^-24 and 16 c 2^-24 exactly.  The factor 16 of odd
+// elements is taken out of the query before and out of the result after.  The query is FP16 under a
+// power of two of its row (exact for BF16 within 2^26 of the row's largest element), P s is FP16 (11
+// bits), the rotary part stays BF16; all are m16n8k16 products with FP32 sums.
 //
 // A CTA holds 16 query rows (query tokens x heads) and walks the pages of one or more requests; a page
 // (64 tokens) is one pipeline stage (TMA, 128-byte swizzle, so that ldmatrix reads without conflicts).
@@ -66,9 +65,15 @@ __device__ __forceinline__ void ldsm_x4_t(uint32_t addr, uint32_t (&r)[4]) {
                : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
                : "r"(addr));
 }
-__device__ __forceinline__ void mma_e4m3(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-  asm volatile(
-      "mma.sync.aligned.m16n8k32.row.col.f32.e4m3.e4m3.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+// D (16 x 8, FP32) += A (16 x 16) B (16 x 8).  Not volatile: the compiler may interleave them.
+__device__ __forceinline__ void mma_f16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+      "{%0, %1, %2, %3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void mma_bf16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
       "{%0, %1, %2, %3};"
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
@@ -208,7 +213,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     const int lim_min = len - a.q_len + 1;
 
     // ---- the query: two rows per thread (g and g + 8), two E4M3 terms, rotary part in BF16 ----
-    uint32_t q_hi[NCH][4], q_lo[NCH][4], q_pe[KR][4];
+    uint32_t q[2 * NCH][4], q_pe[KR][4];
     float q_sum[2][NG], row_scale[2];
     int lim[2];
 #pragma unroll
@@ -224,7 +229,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         const uint4 w = live ? *reinterpret_cast<const uint4*>(src + 32 * c + 8 * j) : make_uint4(0, 0, 0, 0);
         const uint32_t v[4] = {w.x, w.y, w.z, w.w};
         // kept raw until the row's largest element is known
-        q_hi[c][r] = v[0], q_hi[c][r + 2] = v[1], q_lo[c][r] = v[2], q_lo[c][r + 2] = v[3];
+        q[2 * c][r] = v[0], q[2 * c][r + 2] = v[1], q[2 * c + 1][r] = v[2], q[2 * c + 1][r + 2] = v[3];
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
           top = fmaxf(top, fmaxf(fabsf(bf16_lo(v[k])), fabsf(bf16_hi(v[k]))));
@@ -233,31 +238,26 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       top = quad_max(top);
       odd = quad_sum(odd);
-      // 2^k with top 2^k in [128, 256)
-      const int k = min(max(7 - (static_cast<int>(__float_as_uint(top) >> 23) - 127), -118), 118);
+      // 2^k with top 2^k in [2^13, 2^14)
+      const int k = min(max(13 - (static_cast<int>(__float_as_uint(top) >> 23) - 127), -100), 100);
       const float up = top > 0.f ? pow2(k) : 1.f;
-      row_scale[r] = odd != 0.f ? __int_as_float(0x7FC00000) : qk_scale * 512.f / up;
+      row_scale[r] = odd != 0.f ? __int_as_float(0x7FC00000) : qk_scale * 16777216.f / up;
 #pragma unroll
       for (int c = 0; c < NCH; ++c) {
-        const uint32_t v[4] = {q_hi[c][r], q_hi[c][r + 2], q_lo[c][r], q_lo[c][r + 2]};
-        uint32_t hi[2] = {0, 0}, lo[2] = {0, 0};  // even elements, odd elements
-        float sum = 0.f;
+        const uint32_t v[4] = {q[2 * c][r], q[2 * c][r + 2], q[2 * c + 1][r], q[2 * c + 1][r + 2]};
+        float x[8], sum = 0.f;
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          const float x0 = bf16_lo(v[e]) * up, x1 = bf16_hi(v[e]) * up;
-          const uint32_t h2 = f32x2_to_e4m3x2(x0, x1);
-          const float2 f = __half22float2(e4m3x2_to_half2(h2));
-          const uint32_t l2 = f32x2_to_e4m3x2(x0 - f.x, x1 - f.y);
-          const float2 fl = __half22float2(e4m3x2_to_half2(l2));
-          sum += (f.x + fl.x) + (f.y + fl.y);
-          hi[0] |= (h2 & 0xFFu) << (8 * e), hi[1] |= (h2 >> 8) << (8 * e);
-          lo[0] |= (l2 & 0xFFu) << (8 * e), lo[1] |= (l2 >> 8) << (8 * e);
+          x[2 * e] = bf16_lo(v[e]) * up, x[2 * e + 1] = bf16_hi(v[e]) * up;
+          sum += x[2 * e] + x[2 * e + 1];
         }
-        q_hi[c][r] = hi[0], q_hi[c][r + 2] = hi[1], q_lo[c][r] = lo[0], q_lo[c][r + 2] = lo[1];
+        // a word of codes gives elements (0, 4), 16 (1, 5), (2, 6) and 16 (3, 7)
+        q[2 * c][r] = pack_half2(x[0], x[4]), q[2 * c][r + 2] = pack_half2(x[1] * 0.0625f, x[5] * 0.0625f);
+        q[2 * c + 1][r] = pack_half2(x[2], x[6]), q[2 * c + 1][r + 2] = pack_half2(x[3] * 0.0625f, x[7] * 0.0625f);
         q_sum[r][c / 4] = (c % 4 == 0 ? 0.f : q_sum[r][c / 4]) + sum;
       }
 #pragma unroll
-      for (int k2 = 0; k2 < NG; ++k2) q_sum[r][k2] = quad_sum(q_sum[r][k2]) * (1.f / 512.f);
+      for (int k2 = 0; k2 < NG; ++k2) q_sum[r][k2] = quad_sum(q_sum[r][k2]) * (1.f / 16777216.f);
 #pragma unroll
       for (int c = 0; c < KR; ++c) {
         q_pe[c][r] = live ? *reinterpret_cast<const uint32_t*>(src + D + 16 * c + 2 * j) : 0;
@@ -282,25 +282,24 @@ __global__ void __launch_bounds__(kThreads, 1)
       const uint32_t st = stages + (at % C::STAGES) * C::STAGE;
       float c_acc[NG][4], r_acc[4] = {0.f, 0.f, 0.f, 0.f};
       const int row = 8 * warp + (lane & 7);
+      uint32_t w[NG][4], w_pe[KR / 2][4];
 #pragma unroll
       for (int k = 0; k < NG; ++k) {
         c_acc[k][0] = c_acc[k][1] = c_acc[k][2] = c_acc[k][3] = 0.f;
-        uint32_t w[4];
-        ldsm_x4(st + (k / 2) * 8192 + sw128(row, (k & 1) * 4 + (lane >> 3)), w);
-#pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          const uint32_t b0 = w[c] & 0x0F0F0F0Fu, b1 = (w[c] >> 4) & 0x0F0F0F0Fu;
-          mma_e4m3(c_acc[k], q_hi[4 * k + c], b0, b1);
-          mma_e4m3(c_acc[k], q_lo[4 * k + c], b0, b1);
-        }
+        ldsm_x4(st + (k / 2) * 8192 + sw128(row, (k & 1) * 4 + (lane >> 3)), w[k]);
       }
 #pragma unroll
-      for (int c = 0; c < KR; c += 2) {
-        uint32_t w[4];
-        const uint32_t base = st + C::CODES;
-        ldsm_x4(base + (DR == 64 ? sw128(row, 2 * c + (lane >> 3)) : sw64(row, 2 * c + (lane >> 3))), w);
-        mma_bf16_16816(r_acc, q_pe[c][0], q_pe[c][1], q_pe[c][2], q_pe[c][3], w[0], w[1]);
-        mma_bf16_16816(r_acc, q_pe[c + 1][0], q_pe[c + 1][1], q_pe[c + 1][2], q_pe[c + 1][3], w[2], w[3]);
+      for (int c = 0; c < KR / 2; ++c)
+        ldsm_x4(st + C::CODES + (DR == 64 ? sw128(row, 4 * c + (lane >> 3)) : sw64(row, 4 * c + (lane >> 3))), w_pe[c]);
+      // the groups in turn, so that no product waits for the one before it
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        if (c < KR) mma_bf16(r_acc, q_pe[c], w_pe[c / 2][2 * (c & 1)], w_pe[c / 2][2 * (c & 1) + 1]);
+#pragma unroll
+        for (int k = 0; k < NG; ++k) mma_f16(c_acc[k], q[8 * k + 2 * c], w[k][c] & 0x000F000Fu, w[k][c] & 0x00F000F0u);
+#pragma unroll
+        for (int k = 0; k < NG; ++k)
+          mma_f16(c_acc[k], q[8 * k + 2 * c + 1], (w[k][c] >> 8) & 0x000F000Fu, (w[k][c] >> 8) & 0x00F000F0u);
       }
       const float4* par = reinterpret_cast<const float4*>(smem + (at % C::STAGES) * C::STAGE + C::CODES + C::ROPE) +
                           (8 * warp + 2 * j) * (NG / 2);
@@ -447,10 +446,10 @@ __global__ void __launch_bounds__(kThreads, 1)
           for (int c = 0; c < D / 256; ++c) {
             const uint32_t x = D == 512 ? w[i][2 * c] : w[0][2 * i], y = D == 512 ? w[i][2 * c + 1] : w[0][2 * i + 1];
             const uint32_t x8 = x >> 8, y8 = y >> 8;
-            mma_f16_16816(acc[4 * c], pa[i][0], pa[i][1], pa[i][2], pa[i][3], x & 0x000F000Fu, y & 0x000F000Fu);
-            mma_f16_16816(acc[4 * c + 1], pa[i][0], pa[i][1], pa[i][2], pa[i][3], x & 0x00F000F0u, y & 0x00F000F0u);
-            mma_f16_16816(acc[4 * c + 2], pa[i][0], pa[i][1], pa[i][2], pa[i][3], x8 & 0x000F000Fu, y8 & 0x000F000Fu);
-            mma_f16_16816(acc[4 * c + 3], pa[i][0], pa[i][1], pa[i][2], pa[i][3], x8 & 0x00F000F0u, y8 & 0x00F000F0u);
+            mma_f16(acc[4 * c], pa[i], x & 0x000F000Fu, y & 0x000F000Fu);
+            mma_f16(acc[4 * c + 1], pa[i], x & 0x00F000F0u, y & 0x00F000F0u);
+            mma_f16(acc[4 * c + 2], pa[i], x8 & 0x000F000Fu, y8 & 0x000F000Fu);
+            mma_f16(acc[4 * c + 3], pa[i], x8 & 0x00F000F0u, y8 & 0x00F000F0u);
           }
       }
     };
