@@ -11,10 +11,12 @@
 //
 // A CTA holds 16 query rows (query tokens x heads) and walks the pages of one or more requests; a page
 // (64 tokens) is one pipeline stage (TMA, 128-byte swizzle, so that ldmatrix reads without conflicts).
-// Each of the 8 warps scores 8 of the page's tokens, weighs them against a reference maximum that moves
-// only when a score passes it by 2^10, and writes P s of each group to shared memory; then each warp
-// adds D/8 latent columns of the page.  Scores of page i + 1 and sums of page i share an iteration, with
-// one barrier, which also carries the vote on moving the references.
+// Eight warps score: a pair takes 16 of the page's tokens, each warp of it half of the latent columns
+// (the query's operand registers would not fit otherwise), and they swap partial scores so that each
+// holds 8 tokens' whole ones.  It weighs them against a reference maximum that moves only when a score
+// passes it by 2^10 and writes P s of each group to shared memory.  Four warps add up: each holds D/4
+// latent columns of the result and takes page i while the others score page i + 1.  The scoring warps
+// vote once a page on moving the references; a move leaves the factors for the sums beside the weights.
 //
 // The pages of all requests are dealt to the CTAs in one equal run each (a run may begin or end inside
 // a request); what is cut is joined by merge_kernel by log-sum-exp.
@@ -27,8 +29,9 @@ namespace rolaq {
 namespace i4 {
 namespace {
 
-constexpr int kThreads = 256, kWarps = 8;
-constexpr int kRows = 16;        // query rows of a CTA
+constexpr int kScorers = 8, kAdders = 4;  // warps
+constexpr int kScoreThreads = kScorers * 32, kThreads = (kScorers + kAdders) * 32;
+constexpr int kRows = 16;  // query rows of a CTA
 constexpr int kMinPages = 2;     // least run of pages worth a CTA of its own
 constexpr float kSlack = 10.f;   // log2 of how far a weight may pass its reference
 constexpr float kScaleSlack = 16.f;
@@ -42,8 +45,34 @@ struct Cfg {
   static constexpr int STAGES = D == 512 ? 7 : 12;
   static constexpr int PBUF = NG * kRows * kPage * 2;  // P s of a page: [group][row][token] FP16
   static constexpr int SMEM = 1024 + STAGES * STAGE + 2 * PBUF;
-  static constexpr int NT = D / 64;                 // 8-column tiles of a warp's share
+  static constexpr int HG = NG / 2;                 // groups of a scoring warp
+  static constexpr int NT = D / kAdders / 8;        // 8-column tiles of an adding warp
 };
+
+// What a page's weights carry beside them, and a request's denominators: the scoring warps to the adding.
+template <int NG>
+struct Shared {
+  float4 swap[2][kScorers][32];
+  float red_m[kScorers][kRows], red_s[kScorers][NG];
+  float keep[2][kRows], keep_unit[2][NG];  // factors for the sums before page i (i & 1), where moved[i & 1]
+  int moved[2];
+  float l[kScorers][kRows], z[kScorers][kRows][NG], m[kRows], unit[NG];  // of a finished request
+};
+
+// Named barriers: 1..4 the pairs, 5 all scoring warps, 6 / 7 a request's sums written / read.
+enum { kBarPair = 1, kBarScore = 5, kBarSums = 6, kBarTaken = 7 };
+__device__ __forceinline__ void bar_arrive(int id, int threads) {
+  asm volatile("bar.arrive %0, %1;" ::"r"(id), "r"(threads) : "memory");
+}
+__device__ __forceinline__ bool bar_any(int id, int threads, bool vote) {
+  int any;
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %3, 0;\n\tbar.red.or.pred q, %1, %2, p;\n\tselp.b32 %0, 1, 0, q;\n\t}"
+      : "=r"(any)
+      : "r"(id), "r"(threads), "r"(static_cast<int>(vote))
+      : "memory");
+  return any != 0;
+}
 
 __device__ __forceinline__ int pages_of(const DecodeArgs& a, int b) {
   const int64_t len = min(static_cast<int64_t>(a.seq_lens[b]), static_cast<int64_t>(a.max_pages) * kPage);
@@ -97,6 +126,7 @@ __device__ __forceinline__ float quad_max(float v) {
 }
 
 // Exclusive prefix over the CTA's threads of v; the total in `total`.
+template <int WARPS>
 __device__ __forceinline__ int64_t block_scan(int64_t v, int64_t& total, int64_t* sm) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x / 32;
   int64_t x = v;
@@ -110,7 +140,7 @@ __device__ __forceinline__ int64_t block_scan(int64_t v, int64_t& total, int64_t
   int64_t before = 0;
   total = 0;
 #pragma unroll
-  for (int k = 0; k < kWarps; ++k) {
+  for (int k = 0; k < WARPS; ++k) {
     if (k < warp) before += sm[k];
     total += sm[k];
   }
@@ -127,16 +157,15 @@ __global__ void __launch_bounds__(kThreads, 1)
     decode_kernel(const __grid_constant__ CUtensorMap map_codes, const __grid_constant__ CUtensorMap map_rope,
                   const DecodeArgs a, const Partials part, const int groups, const int blocks) {
   using C = Cfg<D, DR>;
-  constexpr int NG = C::NG, NCH = D / 32, KR = DR / 16;
+  constexpr int NG = C::NG, HG = C::HG, STAGES = C::STAGES;
   extern __shared__ char raw[];
   char* smem = reinterpret_cast<char*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
-  char* pbuf = smem + C::STAGES * C::STAGE;
-  __shared__ uint64_t full[C::STAGES];
-  __shared__ int bad_page[C::STAGES];
-  __shared__ int64_t scan[kWarps];
+  char* pbuf = smem + STAGES * C::STAGE;
+  __shared__ uint64_t full[STAGES], empty[STAGES], p_full[2], p_empty[2];
+  __shared__ int bad_page[STAGES];
+  __shared__ int64_t scan[kThreads / 32];
   __shared__ int start[2];
-  __shared__ float unit[NG];                 // 2^-e of each group's scales
-  __shared__ float red_m[kWarps][kRows], red_s[kWarps][NG], red_z[kWarps][kRows][NG];
+  __shared__ Shared<NG> sh;
 
   const int tid = threadIdx.x, warp = tid / 32, lane = tid & 31, g = lane >> 2, j = lane & 3;
   const int block = blockIdx.x % blocks, group = blockIdx.x / blocks;
@@ -148,10 +177,11 @@ __global__ void __launch_bounds__(kThreads, 1)
   int64_t mine = 0, total;
   for (int b = tid * per; b < min(a.batch, (tid + 1) * per); ++b) mine += pages_of(a, b);
   if (tid == 0) {
-    for (int s = 0; s < C::STAGES; ++s) mbar_init(&full[s], 1);
+    for (int s = 0; s < STAGES; ++s) mbar_init(&full[s], 1), mbar_init(&empty[s], kAdders);
+    for (int s = 0; s < 2; ++s) mbar_init(&p_full[s], 1), mbar_init(&p_empty[s], kAdders);
     fence_mbar_init();
   }
-  int64_t before = block_scan(mine, total, scan);
+  int64_t before = block_scan<kThreads / 32>(mine, total, scan);
   const int runs = runs_of(total, groups);
   if (group >= runs || total == 0) return;
   const int64_t u0 = total * group / runs;
@@ -164,57 +194,176 @@ __global__ void __launch_bounds__(kThreads, 1)
   }
   __syncthreads();
   int seg_b = start[0], seg_p = start[1];
+  int done = 0;       // pages of the run done
+  int stage = 0, lap = 0;  // of page `done`: full[stage]'s phase is lap & 1
+  bool healthy = true;
+  auto wait_for = [&](uint64_t* bar, int phase) {
+    if (healthy) healthy = mbar_wait(bar, phase & 1, a.err);
+  };
+  auto advance = [&]() {
+    ++done;
+    if (++stage == STAGES) stage = 0, ++lap;
+  };
 
-  // ---- the page stream (thread 0): stage k holds unit k of the run ----
-  const int pool_pages = static_cast<int>(a.cache.num_slots / kPage);
-  int load_b = seg_b, load_p = seg_p, load_n = 0, load_id = 0, loaded = 0;
-  auto next_id = [&]() {  // the page that (load_b, load_p) names, requested an iteration ahead of its use
-    while (load_p >= load_n) {
-      if (load_n != 0) ++load_b, load_p = 0;
-      load_n = pages_of(a, load_b);
-      if (load_n == 0) ++load_b, load_p = 0;
-    }
-    load_id = a.page_table[load_b * a.pt_stride + load_p++];
-  };
-  auto load = [&]() {
-    const int s = loaded % C::STAGES;
-    const bool ok = load_id >= 0 && load_id < pool_pages;
-    const int page = ok ? load_id : 0;
-    char* dst = smem + s * C::STAGE;
-    bad_page[s] = !ok;
-    if (!ok) report(a.err, ROLAQ_DEV_BAD_PAGE);
-    mbar_expect_tx(&full[s], C::STAGE);
+  if (warp >= kScorers) {
+    // ================= adding warps: D / 4 latent columns each =================
+    const int w = warp - kScorers;
+    // the page stream (warp 0, lane 0): stage k holds page k of the run
+    const int pool_pages = static_cast<int>(a.cache.num_slots / kPage);
+    int load_b = seg_b, load_p = seg_p, load_n = 0, load_id = 0, loaded = 0, load_stage = 0, load_lap = 0;
+    auto next_id = [&]() {  // the page that (load_b, load_p) names, requested a page ahead of its use
+      while (load_p >= load_n) {
+        if (load_n != 0) ++load_b, load_p = 0;
+        load_n = pages_of(a, load_b);
+        if (load_n == 0) ++load_b, load_p = 0;
+      }
+      load_id = a.page_table[load_b * a.pt_stride + load_p++];
+    };
+    auto load = [&]() {
+      const bool ok = load_id >= 0 && load_id < pool_pages;
+      const int page = ok ? load_id : 0;
+      char* dst = smem + load_stage * C::STAGE;
+      uint64_t* bar = &full[load_stage];
+      bad_page[load_stage] = !ok;
+      if (!ok) report(a.err, ROLAQ_DEV_BAD_PAGE);
+      mbar_expect_tx(bar, C::STAGE);
 #pragma unroll
-    for (int k = 0; k < D / 256; ++k) tma_load_2d(dst + k * 8192, &map_codes, &full[s], k * 128, page * kPage);
-    tma_load_2d(dst + C::CODES, &map_rope, &full[s], 0, page * kPage);
-    bulk_load(dst + C::CODES + C::ROPE, a.cache.params + static_cast<int64_t>(page) * (kPage * NG * 2), C::PARAMS,
-              &full[s]);
-    if (++loaded < n_units) next_id();
-  };
-  if (tid == 0) {
-    prefetch_tensormap(&map_codes);
-    prefetch_tensormap(&map_rope);
-    next_id();
-    while (loaded < min(n_units, C::STAGES)) load();
+      for (int k = 0; k < D / 256; ++k) tma_load_2d(dst + k * 8192, &map_codes, bar, k * 128, page * kPage);
+      tma_load_2d(dst + C::CODES, &map_rope, bar, 0, page * kPage);
+      bulk_load(dst + C::CODES + C::ROPE, a.cache.params + static_cast<int64_t>(page) * (kPage * NG * 2), C::PARAMS, bar);
+      if (++load_stage == STAGES) load_stage = 0, ++load_lap;
+      if (++loaded < n_units) next_id();
+    };
+    if (w == 0 && lane == 0) {
+      prefetch_tensormap(&map_codes);
+      prefetch_tensormap(&map_rope);
+      next_id();
+      while (loaded < min(n_units, STAGES)) load();
+    }
+    const int own = w * NG / kAdders;  // the group of the warp's columns
+    const uint32_t p_off = own * (kRows * 128);
+    constexpr int CH = C::NT / 4;  // 16-byte chunks (32 columns) of the warp
+    while (done < n_units) {
+      const int seg_pages = pages_of(a, seg_b);
+      if (seg_pages == 0) {
+        ++seg_b;
+        continue;
+      }
+      const int count = min(seg_pages - seg_p, n_units - done);
+      const bool first = done == 0;
+      float acc[C::NT][4];
+#pragma unroll
+      for (int n = 0; n < C::NT; ++n)
+#pragma unroll
+        for (int k = 0; k < 4; ++k) acc[n][k] = 0.f;
+      for (int i = 0; i < count; ++i) {
+        const int pb = done & 1;
+        wait_for(&p_full[pb], done >> 1);
+        if (sh.moved[pb]) {
+          const float ku = sh.keep_unit[pb][own], k0 = sh.keep[pb][g] * ku, k1 = sh.keep[pb][g + 8] * ku;
+#pragma unroll
+          for (int n = 0; n < C::NT; ++n) acc[n][0] *= k0, acc[n][1] *= k0, acc[n][2] *= k1, acc[n][3] *= k1;
+        }
+        const uint32_t st = stages + stage * C::STAGE, ps = pbufs + pb * C::PBUF + p_off;
+        uint32_t pa[4][4];
+#pragma unroll
+        for (int kk = 0; kk < 4; ++kk) ldsm_x4(ps + sw128(lane & 15, 2 * kk + (lane >> 4)), pa[kk]);
+#pragma unroll
+        for (int c = 0; c < CH; ++c) {
+          const int chunk = w * CH + c;  // of the row
+          uint32_t x[2][4];              // tokens 0..31, 32..63
+#pragma unroll
+          for (int h = 0; h < 2; ++h) ldsm_x4_t(st + (chunk / 8) * 8192 + sw128(32 * h + lane, chunk & 7), x[h]);
+#pragma unroll
+          for (int kk = 0; kk < 4; ++kk) {
+            const uint32_t u = x[kk / 2][2 * (kk & 1)], v = x[kk / 2][2 * (kk & 1) + 1];
+            const uint32_t u8 = u >> 8, v8 = v >> 8;
+            mma_f16(acc[4 * c], pa[kk], u & 0x000F000Fu, v & 0x000F000Fu);
+            mma_f16(acc[4 * c + 1], pa[kk], u & 0x00F000F0u, v & 0x00F000F0u);
+            mma_f16(acc[4 * c + 2], pa[kk], u8 & 0x000F000Fu, v8 & 0x000F000Fu);
+            mma_f16(acc[4 * c + 3], pa[kk], u8 & 0x00F000F0u, v8 & 0x00F000F0u);
+          }
+        }
+        __syncwarp();
+        if (lane == 0) {
+          mbar_arrive(&p_empty[pb]);
+          mbar_arrive(&empty[stage]);
+        }
+        // refill the stage that all four warps left a page ago
+        if (w == 0 && lane == 0 && loaded < n_units && loaded < done + STAGES) {
+          wait_for(&empty[load_stage], load_lap - 1);
+          load();
+        }
+        advance();
+      }
+      // ---- the rows' results ----
+      named_bar_sync(kBarSums, kThreads);
+      const bool whole = seg_p == 0 && count == seg_pages;
+      const float u = sh.unit[own], inv_u = u == 0.f ? 0.f : 1.f / u;
+      float z[2] = {0.f, 0.f}, l[2] = {0.f, 0.f}, lse[2];
+#pragma unroll
+      for (int r = 0; r < 2; ++r) {
+        for (int k = 0; k < kScorers; ++k) l[r] += sh.l[k][g + 8 * r], z[r] += sh.z[k][g + 8 * r][own];
+        lse[r] = l[r] == 0.f ? -INFINITY : (sh.m[g + 8 * r] + log2f(l[r])) * kLn2;
+      }
+      bar_arrive(kBarTaken, kThreads);
+      // a cut request's partial: slot 0 where the run begins in (or with) this request, else 1
+      const int64_t slot = (static_cast<int64_t>(2 * group + (first ? 0 : 1)) * blocks + block) * kRows;
+#pragma unroll
+      for (int r = 0; r < 2; ++r) {
+        const int row = block * kRows + g + 8 * r;
+        const float inv = l[r] == 0.f ? 0.f : inv_u / l[r];
+        const bool live = row < a.q_len * a.heads;
+        const int t = live ? row / a.heads : 0, h = live ? row % a.heads : 0;
+        uint16_t* out = a.out + seg_b * a.o_sb + t * a.o_st + h * a.o_sh;
+        float* out_part = part.o + (slot + g + 8 * r) * D;
+#pragma unroll
+        for (int c = 0; c < CH; ++c) {
+          const int col = 32 * (w * CH + c) + 8 * j;
+          float v[8];
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int k = 0; k < 2; ++k)
+              v[4 * k + i] = fmaf(acc[4 * c + i][2 * r + k], i & 1 ? 1048576.f : 16777216.f, -z[r]) * inv;
+          if (!whole) {
+            reinterpret_cast<float4*>(out_part + col)[0] = make_float4(v[0], v[1], v[2], v[3]);
+            reinterpret_cast<float4*>(out_part + col)[1] = make_float4(v[4], v[5], v[6], v[7]);
+          } else if (live) {
+            *reinterpret_cast<uint4*>(out + col) = make_uint4(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]),
+                                                              pack_bf16x2(v[4], v[5]), pack_bf16x2(v[6], v[7]));
+          }
+        }
+        if (w == 0 && j == 0) {
+          if (!whole) part.lse[slot + g + 8 * r] = lse[r];
+          else if (live && a.lse) a.lse[(static_cast<int64_t>(seg_b) * a.q_len + t) * a.heads + h] = lse[r];
+        }
+      }
+      ++seg_b;
+      seg_p = 0;
+    }
+    return;
   }
 
-  bool healthy = true;
+  // ================= scoring warps =================
+  const int half = warp & 1, quarter = warp >> 1;  // half of the latent columns, 16 of the page's tokens
+  constexpr int KR = DR / 32;                      // 16-column steps of the rotary part, half of them here
   const float qk_scale = a.sm_scale * kLog2e;
-  int unit_at = 0;  // units of the run done
-  while (unit_at < n_units) {
-    int seg_pages = pages_of(a, seg_b);
+  bool begun = false;
+  while (done < n_units) {
+    const int seg_pages = pages_of(a, seg_b);
     if (seg_pages == 0) {
       ++seg_b;
       continue;
     }
-    const int p_end = min(seg_pages, seg_p + n_units - unit_at);
-    int len = min(static_cast<int64_t>(a.seq_lens[seg_b]), static_cast<int64_t>(a.max_pages) * kPage);
+    const int count = min(seg_pages - seg_p, n_units - done);
+    const int len = min(static_cast<int64_t>(a.seq_lens[seg_b]), static_cast<int64_t>(a.max_pages) * kPage);
     if (tid == 0 && len != a.seq_lens[seg_b]) report(a.err, ROLAQ_DEV_BAD_REQ);
     const int lim_min = len - a.q_len + 1;
 
-    // ---- the query: two rows per thread (g and g + 8), two E4M3 terms, rotary part in BF16 ----
-    uint32_t q[2 * NCH][4], q_pe[KR][4];
-    float q_sum[2][NG], row_scale[2];
+    // ---- the query: rows g and g + 8, this warp's columns ----
+    uint32_t q[8 * HG][4], q_pe[KR][4];
+    float q_sum[2][HG], row_scale[2];
     int lim[2];
 #pragma unroll
     for (int r = 0; r < 2; ++r) {
@@ -224,12 +373,11 @@ __global__ void __launch_bounds__(kThreads, 1)
       lim[r] = live ? lim_min + t : 0;
       const uint16_t* src = a.q + seg_b * a.q_sb + t * a.q_st + h * a.q_sh;
       float top = 0.f, odd = 0.f;
+      uint4 raw_q[D / 32];  // the whole row: both halves scale it alike
 #pragma unroll
-      for (int c = 0; c < NCH; ++c) {
-        const uint4 w = live ? *reinterpret_cast<const uint4*>(src + 32 * c + 8 * j) : make_uint4(0, 0, 0, 0);
-        const uint32_t v[4] = {w.x, w.y, w.z, w.w};
-        // kept raw until the row's largest element is known
-        q[2 * c][r] = v[0], q[2 * c][r + 2] = v[1], q[2 * c + 1][r] = v[2], q[2 * c + 1][r + 2] = v[3];
+      for (int c = 0; c < D / 32; ++c) {
+        raw_q[c] = live ? *reinterpret_cast<const uint4*>(src + 32 * c + 8 * j) : make_uint4(0, 0, 0, 0);
+        const uint32_t v[4] = {raw_q[c].x, raw_q[c].y, raw_q[c].z, raw_q[c].w};
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
           top = fmaxf(top, fmaxf(fabsf(bf16_lo(v[k])), fabsf(bf16_hi(v[k]))));
@@ -241,10 +389,11 @@ __global__ void __launch_bounds__(kThreads, 1)
       // 2^k with top 2^k in [2^13, 2^14)
       const int k = min(max(13 - (static_cast<int>(__float_as_uint(top) >> 23) - 127), -100), 100);
       const float up = top > 0.f ? pow2(k) : 1.f;
-      row_scale[r] = odd != 0.f ? __int_as_float(0x7FC00000) : qk_scale * 16777216.f / up;
+      row_scale[r] = odd != 0.f ? __int_as_float(0x7FC00000) : qk_scale * (16777216.f / up);
 #pragma unroll
-      for (int c = 0; c < NCH; ++c) {
-        const uint32_t v[4] = {q[2 * c][r], q[2 * c][r + 2], q[2 * c + 1][r], q[2 * c + 1][r + 2]};
+      for (int c = 0; c < 4 * HG; ++c) {
+        const uint4 pick = half ? raw_q[4 * HG + c] : raw_q[c];
+        const uint32_t v[4] = {pick.x, pick.y, pick.z, pick.w};
         float x[8], sum = 0.f;
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
@@ -257,52 +406,102 @@ __global__ void __launch_bounds__(kThreads, 1)
         q_sum[r][c / 4] = (c % 4 == 0 ? 0.f : q_sum[r][c / 4]) + sum;
       }
 #pragma unroll
-      for (int k2 = 0; k2 < NG; ++k2) q_sum[r][k2] = quad_sum(q_sum[r][k2]) * (1.f / 16777216.f);
+      for (int i = 0; i < HG; ++i) q_sum[r][i] = quad_sum(q_sum[r][i]) * (1.f / 16777216.f);
+      // the rotary part under the same power of two (exact), so that both parts add up
+      const float down = up * (1.f / 16777216.f);
 #pragma unroll
-      for (int c = 0; c < KR; ++c) {
-        q_pe[c][r] = live ? *reinterpret_cast<const uint32_t*>(src + D + 16 * c + 2 * j) : 0;
-        q_pe[c][r + 2] = live ? *reinterpret_cast<const uint32_t*>(src + D + 16 * c + 8 + 2 * j) : 0;
-      }
+      for (int c = 0; c < KR; ++c)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const uint32_t v = live ? *reinterpret_cast<const uint32_t*>(src + D + 16 * (half * KR + c) + 8 * e + 2 * j) : 0;
+          q_pe[c][r + 2 * e] = pack_bf16x2(bf16_lo(v) * down, bf16_hi(v) * down);
+        }
     }
 
-    float acc[C::NT][4], zsum[2][NG], l_sum[2] = {0.f, 0.f}, m_ref[2] = {-INFINITY, -INFINITY};
+    float zsum[2][NG], unit[NG], l_sum[2] = {0.f, 0.f}, m_ref[2] = {-INFINITY, -INFINITY};
 #pragma unroll
-    for (int n = 0; n < C::NT; ++n)
-#pragma unroll
-      for (int k = 0; k < 4; ++k) acc[n][k] = 0.f;
-#pragma unroll
-    for (int k = 0; k < NG; ++k) zsum[0][k] = zsum[1][k] = 0.f;
-    if (tid < NG) unit[tid] = 0.f;
-    __syncthreads();
+    for (int k = 0; k < NG; ++k) zsum[0][k] = zsum[1][k] = unit[k] = 0.f;
 
-    float s_val[4], s_tok[2][NG], z_tok[2][NG], p_val[4];  // scores, params and weights of the warp's 8 tokens
-
-    // Scores of a page: rows (g, g + 8) x tokens (8 warp + 2 j, + 1), in log2 units.
-    auto score = [&](int at, int p) {
-      const uint32_t st = stages + (at % C::STAGES) * C::STAGE;
-      float c_acc[NG][4], r_acc[4] = {0.f, 0.f, 0.f, 0.f};
-      const int row = 8 * warp + (lane & 7);
-      uint32_t w[NG][4], w_pe[KR / 2][4];
+    for (int i = 0; i < count; ++i) {
+      const int p = seg_p + i, pb = done & 1;
+      wait_for(&full[stage], lap);
+      const uint32_t st = stages + stage * C::STAGE;
+      const char* st_ptr = smem + stage * C::STAGE;
+      // ---- partial scores of 16 tokens: tile 0 the warp's own eight, tile 1 its partner's ----
+      float part_s[2][4];
+      {
+        float c_acc[2][HG][4], r_acc[2][4];
+        uint32_t w[2][HG][4], w_pe[2][4];
 #pragma unroll
-      for (int k = 0; k < NG; ++k) {
-        c_acc[k][0] = c_acc[k][1] = c_acc[k][2] = c_acc[k][3] = 0.f;
-        ldsm_x4(st + (k / 2) * 8192 + sw128(row, (k & 1) * 4 + (lane >> 3)), w[k]);
+        for (int n = 0; n < 2; ++n) {
+          const int row = 16 * quarter + 8 * (half ^ n) + (lane & 7);
+#pragma unroll
+          for (int k = 0; k < HG; ++k)
+            ldsm_x4(D == 512 ? st + half * 8192 + sw128(row, 4 * k + (lane >> 3)) : st + sw128(row, 4 * half + (lane >> 3)),
+                    w[n][k]);
+          if (DR == 64)
+            ldsm_x4(st + C::CODES + sw128(row, 4 * half + (lane >> 3)), w_pe[n]);
+#pragma unroll
+          for (int x = 0; x < 4; ++x) {
+            r_acc[n][x] = 0.f;
+#pragma unroll
+            for (int k = 0; k < HG; ++k) c_acc[n][k][x] = 0.f;
+          }
+        }
+        if (DR == 32) {  // both tiles' two chunks at once
+          const int n = lane >> 4, row = 16 * quarter + 8 * (half ^ n) + (lane & 7);
+          uint32_t both[4];
+          ldsm_x4(st + C::CODES + sw64(row, 2 * half + ((lane >> 3) & 1)), both);
+          w_pe[0][0] = both[0], w_pe[0][1] = both[1], w_pe[1][0] = both[2], w_pe[1][1] = both[3];
+        }
+        // the accumulators in turn, so that no product waits for the one before it
+#pragma unroll
+        for (int c = 0; c < KR; ++c)
+#pragma unroll
+          for (int n = 0; n < 2; ++n) mma_bf16(r_acc[n], q_pe[c], w_pe[n][2 * c], w_pe[n][2 * c + 1]);
+#pragma unroll
+        for (int c = 0; c < 4; ++c)
+#pragma unroll
+          for (int e = 0; e < 2; ++e)
+#pragma unroll
+            for (int k = 0; k < HG; ++k)
+#pragma unroll
+              for (int n = 0; n < 2; ++n) {
+                const uint32_t v = e ? w[n][k][c] >> 8 : w[n][k][c];
+                mma_f16(c_acc[n][k], q[8 * k + 2 * c + e], v & 0x000F000Fu, v & 0x00F000F0u);
+              }
+#pragma unroll
+        for (int n = 0; n < 2; ++n) {
+          const int tok = 16 * quarter + 8 * (half ^ n) + 2 * j;
+          float s[2][HG], z[2][HG];
+          const float* par = reinterpret_cast<const float*>(st_ptr + C::CODES + C::ROPE) + tok * (NG * 2) + half * (HG * 2);
+#pragma unroll
+          for (int t = 0; t < 2; ++t) {
+            if constexpr (HG == 2) {
+              const float4 v = *reinterpret_cast<const float4*>(par + t * (NG * 2));
+              s[t][0] = v.x, z[t][0] = v.y, s[t][1] = v.z, z[t][1] = v.w;
+            } else {
+              const float2 v = *reinterpret_cast<const float2*>(par + t * (NG * 2));
+              s[t][0] = v.x, z[t][0] = v.y;
+            }
+          }
+#pragma unroll
+          for (int x = 0; x < 4; ++x) {
+            float v = r_acc[n][x];
+#pragma unroll
+            for (int k = 0; k < HG; ++k) v = fmaf(s[x & 1][k], fmaf(-z[x & 1][k], q_sum[x >> 1][k], c_acc[n][k][x]), v);
+            part_s[n][x] = v;
+          }
+        }
       }
-#pragma unroll
-      for (int c = 0; c < KR / 2; ++c)
-        ldsm_x4(st + C::CODES + (DR == 64 ? sw128(row, 4 * c + (lane >> 3)) : sw64(row, 4 * c + (lane >> 3))), w_pe[c]);
-      // the groups in turn, so that no product waits for the one before it
-#pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        if (c < KR) mma_bf16(r_acc, q_pe[c], w_pe[c / 2][2 * (c & 1)], w_pe[c / 2][2 * (c & 1) + 1]);
-#pragma unroll
-        for (int k = 0; k < NG; ++k) mma_f16(c_acc[k], q[8 * k + 2 * c], w[k][c] & 0x000F000Fu, w[k][c] & 0x00F000F0u);
-#pragma unroll
-        for (int k = 0; k < NG; ++k)
-          mma_f16(c_acc[k], q[8 * k + 2 * c + 1], (w[k][c] >> 8) & 0x000F000Fu, (w[k][c] >> 8) & 0x00F000F0u);
-      }
-      const float4* par = reinterpret_cast<const float4*>(smem + (at % C::STAGES) * C::STAGE + C::CODES + C::ROPE) +
-                          (8 * warp + 2 * j) * (NG / 2);
+      sh.swap[pb][warp][lane] = make_float4(part_s[1][0], part_s[1][1], part_s[1][2], part_s[1][3]);
+      named_bar_sync(kBarPair + quarter, 64);
+      const float4 theirs = sh.swap[pb][warp ^ 1][lane];
+      // ---- scores of the warp's 8 tokens, in log2 units; their params ----
+      float s_val[4] = {(part_s[0][0] + theirs.x) * row_scale[0], (part_s[0][1] + theirs.y) * row_scale[0],
+                        (part_s[0][2] + theirs.z) * row_scale[1], (part_s[0][3] + theirs.w) * row_scale[1]};
+      float s_tok[2][NG], z_tok[2][NG], p_val[4];
+      const float4* par = reinterpret_cast<const float4*>(st_ptr + C::CODES + C::ROPE) + (8 * warp + 2 * j) * (NG / 2);
 #pragma unroll
       for (int t = 0; t < 2; ++t)
 #pragma unroll
@@ -310,14 +509,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           const float4 v = par[t * (NG / 2) + k / 2];
           s_tok[t][k] = v.x, z_tok[t][k] = v.y, s_tok[t][k + 1] = v.z, z_tok[t][k + 1] = v.w;
         }
-#pragma unroll
-      for (int x = 0; x < 4; ++x) {
-        float s = 0.f;
-#pragma unroll
-        for (int k = 0; k < NG; ++k) s = fmaf(s_tok[x & 1][k], fmaf(-z_tok[x & 1][k], q_sum[x >> 1][k], c_acc[k][x]), s);
-        s_val[x] = fmaf(s, row_scale[x >> 1], r_acc[x] * qk_scale);
-      }
-      const int bad = bad_page[at % C::STAGES];
+      const int bad = bad_page[stage];
       if ((p + 1) * kPage > lim_min || bad) {  // the request's end, or a page that is not there
         const int tok = p * kPage + 8 * warp + 2 * j;
 #pragma unroll
@@ -330,230 +522,127 @@ __global__ void __launch_bounds__(kThreads, 1)
             if (tok + t >= lim[r] || bad) s_val[2 * r + t] = -INFINITY;
         }
       }
-    };
+      if (done >= 2) wait_for(&p_empty[pb], (done >> 1) - 1);
 
-    // Weights against the present references, times each group's scale, to shared memory; true where a
-    // score or a scale has left its reference behind.
-    auto weigh = [&](int at) {
-      bool need = false;
+      // Weights against the present references, times each group's scale, to shared memory; true where
+      // a score or a scale has left its reference behind.
+      auto weigh = [&]() {
+        bool need = false;
 #pragma unroll
-      for (int x = 0; x < 4; ++x) {
-        const float m = m_ref[x >> 1];
-        need |= s_val[x] > m + kSlack;
-        p_val[x] = ex2_approx(s_val[x] - (m == -INFINITY ? 0.f : m));
+        for (int x = 0; x < 4; ++x) {
+          const float m = m_ref[x >> 1];
+          need |= s_val[x] > m + kSlack;
+          p_val[x] = ex2_approx(s_val[x] - (m == -INFINITY ? 0.f : m));
+        }
+        char* dst = pbuf + pb * C::PBUF + 4 * j;
+#pragma unroll
+        for (int k = 0; k < NG; ++k) {
+          const float s0 = s_tok[0][k] * unit[k], s1 = s_tok[1][k] * unit[k];
+          need |= fmaxf(fabsf(s0), fabsf(s1)) > kScaleSlack;
+#pragma unroll
+          for (int r = 0; r < 2; ++r)
+            *reinterpret_cast<uint32_t*>(dst + k * (kRows * 128) + sw128(g + 8 * r, warp)) =
+                pack_half2(p_val[2 * r] * s0, p_val[2 * r + 1] * s1);
+        }
+        return need;
+      };
+      const bool move = bar_any(kBarScore, kScoreThreads, weigh());
+      if (move) {  // new references: the page's maxima; the sums so far are brought to them
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+          const float m = quad_max(fmaxf(s_val[2 * r], s_val[2 * r + 1]));
+          if (j == 0) sh.red_m[warp][g + 8 * r] = m;
+        }
+#pragma unroll
+        for (int k = 0; k < NG; ++k) {
+          const float s = quad_max(fmaxf(fabsf(s_tok[0][k]), fabsf(s_tok[1][k])));
+          if (lane == 0) sh.red_s[warp][k] = s;
+        }
+        named_bar_sync(kBarScore, kScoreThreads);
+        float keep[2];
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+          float m = m_ref[r];
+          for (int w = 0; w < kScorers; ++w) m = fmaxf(m, sh.red_m[w][g + 8 * r]);
+          keep[r] = m_ref[r] == m ? 1.f : ex2_approx(m_ref[r] - m);
+          m_ref[r] = m;
+          l_sum[r] *= keep[r];
+          if (warp == 0 && j == 0) sh.keep[pb][g + 8 * r] = keep[r];
+        }
+#pragma unroll
+        for (int k = 0; k < NG; ++k) {
+          float s = 0.f;
+          for (int w = 0; w < kScorers; ++w) s = fmaxf(s, sh.red_s[w][k]);
+          float keep_unit = 1.f;
+          if (s > 0.f && (unit[k] == 0.f || s * unit[k] > kScaleSlack)) {
+            const float u = pow2(min(max(127 - static_cast<int>(__float_as_uint(s) >> 23), -120), 120));
+            if (unit[k] != 0.f) keep_unit = u / unit[k];
+            unit[k] = u;
+          }
+          if (tid == 0) sh.keep_unit[pb][k] = keep_unit;
+          zsum[0][k] *= keep[0] * keep_unit;
+          zsum[1][k] *= keep[1] * keep_unit;
+        }
+        weigh();
+        named_bar_sync(kBarScore, kScoreThreads);
       }
-      char* dst = pbuf + (at & 1) * C::PBUF + 4 * j;
-#pragma unroll
-      for (int k = 0; k < NG; ++k) {
-        const float u = unit[k], s0 = s_tok[0][k] * u, s1 = s_tok[1][k] * u;
-        need |= fmaxf(fabsf(s0), fabsf(s1)) > kScaleSlack;
-#pragma unroll
-        for (int r = 0; r < 2; ++r)
-          *reinterpret_cast<uint32_t*>(dst + k * (kRows * 128) + sw128(g + 8 * r, warp)) =
-              pack_half2(p_val[2 * r] * s0, p_val[2 * r + 1] * s1);
+      if (tid == 0) {
+        sh.moved[pb] = move;
+        mbar_arrive(&p_full[pb]);
       }
-      return need;
-    };
-
-    // New references (all threads): the page's maxima, the sums so far brought to them.
-    auto move_references = [&](int at) {
-#pragma unroll
-      for (int r = 0; r < 2; ++r) {
-        const float m = quad_max(fmaxf(s_val[2 * r], s_val[2 * r + 1]));
-        if (j == 0) red_m[warp][g + 8 * r] = m;
-      }
-#pragma unroll
-      for (int k = 0; k < NG; ++k) {
-        const float s = quad_max(fmaxf(fabsf(s_tok[0][k]), fabsf(s_tok[1][k])));
-        if (lane == 0) red_s[warp][k] = s;
-      }
-      __syncthreads();
-      float keep[2], keep_u[NG];
-#pragma unroll
-      for (int r = 0; r < 2; ++r) {
-        float m = m_ref[r];
-        for (int w = 0; w < kWarps; ++w) m = fmaxf(m, red_m[w][g + 8 * r]);
-        keep[r] = m_ref[r] == m ? 1.f : ex2_approx(m_ref[r] - m);
-        m_ref[r] = m;
-        l_sum[r] *= keep[r];
-      }
-      float u_new[NG];
-#pragma unroll
-      for (int k = 0; k < NG; ++k) {
-        float s = 0.f;
-        for (int w = 0; w < kWarps; ++w) s = fmaxf(s, red_s[w][k]);
-        const float u = unit[k];
-        u_new[k] = u;
-        if (s > 0.f && (u == 0.f || s * u > kScaleSlack))
-          u_new[k] = pow2(min(max(127 - static_cast<int>(__float_as_uint(s) >> 23), -120), 120));
-        keep_u[k] = u == 0.f ? 1.f : u_new[k] / u;
-        zsum[0][k] *= keep[0] * keep_u[k];
-        zsum[1][k] *= keep[1] * keep_u[k];
-      }
-      const int own = warp * NG / kWarps;
-      float ku = keep_u[0];
-#pragma unroll
-      for (int k = 1; k < NG; ++k) ku = own == k ? keep_u[k] : ku;
-#pragma unroll
-      for (int n = 0; n < C::NT; ++n)
-#pragma unroll
-        for (int x = 0; x < 4; ++x) acc[n][x] *= keep[x >> 1] * ku;
-      __syncthreads();
-      if (tid < NG) {
-        float u = u_new[0];
-#pragma unroll
-        for (int k = 1; k < NG; ++k) u = tid == k ? u_new[k] : u;
-        unit[tid] = u;
-      }
-      __syncthreads();
-      weigh(at);
-      __syncthreads();
-    };
-
-    // After the references stand: the denominators and the zeros' share.
-    auto add_weights = [&]() {
       l_sum[0] += p_val[0] + p_val[1];
       l_sum[1] += p_val[2] + p_val[3];
 #pragma unroll
       for (int k = 0; k < NG; ++k) {
-        const float u = unit[k];
-        const float a0 = s_tok[0][k] * u * z_tok[0][k], a1 = s_tok[1][k] * u * z_tok[1][k];
+        const float a0 = s_tok[0][k] * unit[k] * z_tok[0][k], a1 = s_tok[1][k] * unit[k] * z_tok[1][k];
         zsum[0][k] = fmaf(p_val[0], a0, fmaf(p_val[1], a1, zsum[0][k]));
         zsum[1][k] = fmaf(p_val[2], a0, fmaf(p_val[3], a1, zsum[1][k]));
       }
-    };
-
-    // The warp's D/8 latent columns of a page: acc += (P s) c.
-    auto gather = [&](int at) {
-      const uint32_t st = stages + (at % C::STAGES) * C::STAGE;
-      const uint32_t pb = pbufs + (at & 1) * C::PBUF + (warp * NG / kWarps) * (kRows * 128);
-#pragma unroll
-      for (int kk = 0; kk < 4; kk += 2) {
-        uint32_t w[2][4], pa[2][4];
-        if constexpr (D == 512) {  // 64 columns: two 16-byte chunks, 16 tokens each
-#pragma unroll
-          for (int i = 0; i < 2; ++i)
-            ldsm_x4_t(st + (warp / 4) * 8192 + sw128((kk + i) * 16 + (lane & 15), 2 * (warp & 3) + (lane >> 4)), w[i]);
-        } else {  // 32 columns: one chunk, 32 tokens
-          ldsm_x4_t(st + sw128(kk * 16 + lane, warp), w[0]);
-        }
-#pragma unroll
-        for (int i = 0; i < 2; ++i)
-          ldsm_x4(pb + sw128((lane & 8) + (lane & 7), 2 * (kk + i) + (lane >> 4)), pa[i]);
-#pragma unroll
-        for (int i = 0; i < 2; ++i)
-#pragma unroll
-          for (int c = 0; c < D / 256; ++c) {
-            const uint32_t x = D == 512 ? w[i][2 * c] : w[0][2 * i], y = D == 512 ? w[i][2 * c + 1] : w[0][2 * i + 1];
-            const uint32_t x8 = x >> 8, y8 = y >> 8;
-            mma_f16(acc[4 * c], pa[i], x & 0x000F000Fu, y & 0x000F000Fu);
-            mma_f16(acc[4 * c + 1], pa[i], x & 0x00F000F0u, y & 0x00F000F0u);
-            mma_f16(acc[4 * c + 2], pa[i], x8 & 0x000F000Fu, y8 & 0x000F000Fu);
-            mma_f16(acc[4 * c + 3], pa[i], x8 & 0x00F000F0u, y8 & 0x00F000F0u);
-          }
-      }
-    };
-    auto wait_for = [&](int at) {
-      if (healthy) healthy = mbar_wait(&full[at % C::STAGES], (at / C::STAGES) & 1, a.err);
-    };
-
-    // ---- the pages ----
-    wait_for(unit_at);
-    score(unit_at, seg_p);
-    if (__syncthreads_or(weigh(unit_at))) move_references(unit_at);
-    add_weights();
-    for (int p = seg_p; p < p_end; ++p, ++unit_at) {
-      bool need = false;
-      const bool more = p + 1 < p_end;
-      if (more) {
-        wait_for(unit_at + 1);
-        score(unit_at + 1, p + 1);
-      }
-      gather(unit_at);
-      if (more) need = weigh(unit_at + 1);
-      const bool move = __syncthreads_or(need);
-      if (tid == 0 && loaded < n_units) load();
-      if (move) move_references(unit_at + 1);
-      if (more) add_weights();
+      advance();
     }
-
-    // ---- the rows' results ----
+    // ---- the request's denominators, for the adding warps ----
+    if (begun) named_bar_sync(kBarTaken, kThreads);  // they have taken the last request's
+    begun = true;
 #pragma unroll
     for (int r = 0; r < 2; ++r) {
-      l_sum[r] = quad_sum(l_sum[r]);
-      if (j == 0) red_m[warp][g + 8 * r] = l_sum[r];
+      const float l = quad_sum(l_sum[r]);
+      if (j == 0) sh.l[warp][g + 8 * r] = l;
+      if (warp == 0 && j == 0) sh.m[g + 8 * r] = m_ref[r];
 #pragma unroll
       for (int k = 0; k < NG; ++k) {
         const float z = quad_sum(zsum[r][k]);
-        if (j == 0) red_z[warp][g + 8 * r][k] = z;
+        if (j == 0) sh.z[warp][g + 8 * r][k] = z;
       }
     }
-    __syncthreads();
-    const bool whole = seg_p == 0 && p_end == seg_pages;
-    const int own = warp * NG / kWarps;
-    const float u = unit[own], inv_u = u == 0.f ? 0.f : 1.f / u;
-    // a cut request's partial: slot 0 where the run begins in (or with) this request, else 1
-    const int64_t slot = (static_cast<int64_t>(2 * group + (unit_at - (p_end - seg_p) == 0 ? 0 : 1)) * blocks + block) * kRows;
+    if (tid == 0)
 #pragma unroll
-    for (int r = 0; r < 2; ++r) {
-      const int row = block * kRows + g + 8 * r;
-      float l = 0.f, z = 0.f;
-      for (int w = 0; w < kWarps; ++w) l += red_m[w][g + 8 * r], z += red_z[w][g + 8 * r][own];
-      const float inv = l == 0.f ? 0.f : inv_u / l;
-      const float lse = l == 0.f ? -INFINITY : (m_ref[r] + log2f(l)) * kLn2;
-      float v[D / 256][8];
-#pragma unroll
-      for (int c = 0; c < D / 256; ++c)
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-#pragma unroll
-          for (int k = 0; k < 2; ++k)
-            v[c][4 * k + i] = fmaf(acc[4 * c + i][2 * r + k], i & 1 ? 1048576.f : 16777216.f, -z) * inv;
-      const int col = warp * (D / 8) + 8 * j;
-      if (whole) {
-        if (row < a.q_len * a.heads) {
-          const int t = row / a.heads, h = row % a.heads;
-          uint16_t* out = a.out + seg_b * a.o_sb + t * a.o_st + h * a.o_sh + col;
-#pragma unroll
-          for (int c = 0; c < D / 256; ++c)
-            *reinterpret_cast<uint4*>(out + 32 * c) =
-                make_uint4(pack_bf16x2(v[c][0], v[c][1]), pack_bf16x2(v[c][2], v[c][3]), pack_bf16x2(v[c][4], v[c][5]),
-                           pack_bf16x2(v[c][6], v[c][7]));
-          if (a.lse && warp == 0 && j == 0) a.lse[(static_cast<int64_t>(seg_b) * a.q_len + t) * a.heads + h] = lse;
-        }
-      } else {
-        float* out = part.o + (slot + g + 8 * r) * D + col;
-#pragma unroll
-        for (int c = 0; c < D / 256; ++c) {
-          reinterpret_cast<float4*>(out + 32 * c)[0] = make_float4(v[c][0], v[c][1], v[c][2], v[c][3]);
-          reinterpret_cast<float4*>(out + 32 * c)[1] = make_float4(v[c][4], v[c][5], v[c][6], v[c][7]);
-        }
-        if (warp == 0 && j == 0) part.lse[slot + g + 8 * r] = lse;
-      }
-    }
-    __syncthreads();
+      for (int k = 0; k < NG; ++k) sh.unit[k] = unit[k];
+    bar_arrive(kBarSums, kThreads);
     ++seg_b;
     seg_p = 0;
   }
+  if (begun) named_bar_sync(kBarTaken, kThreads);
 }
+
+constexpr int kMergeWarps = 8, kMergeThreads = kMergeWarps * 32;
 
 // Joins the partials of the requests that more than one run holds, and writes the rows of requests
 // without a token.  WARPS warps share the partials of 128 columns of one row.
 template <int D, int WARPS>
-__global__ void __launch_bounds__(kThreads) merge_kernel(const DecodeArgs a, const Partials part, const int groups,
+__global__ void __launch_bounds__(kMergeThreads) merge_kernel(const DecodeArgs a, const Partials part, const int groups,
                                                          const int blocks) {
-  constexpr int CHUNKS = D / 128, TASKS = kWarps / WARPS;
-  __shared__ int64_t scan[kWarps], scan2[kWarps];
-  __shared__ float4 red[kWarps][32];
+  constexpr int CHUNKS = D / 128, TASKS = kMergeWarps / WARPS;
+  __shared__ int64_t scan[kMergeWarps], scan2[kMergeWarps];
+  __shared__ float4 red[kMergeWarps][32];
   const int tid = threadIdx.x, warp = tid / 32, lane = tid & 31, b = blockIdx.y;
   int64_t sum = 0, below = 0, total, first;
-  for (int i = tid; i < a.batch; i += kThreads) {
+  for (int i = tid; i < a.batch; i += kMergeThreads) {
     const int n = pages_of(a, i);
     sum += n;
     if (i < b) below += n;
   }
-  block_scan(sum, total, scan);
-  block_scan(below, first, scan2);
+  block_scan<kMergeWarps>(sum, total, scan);
+  block_scan<kMergeWarps>(below, first, scan2);
   const int pages = pages_of(a, b);
   const int runs = runs_of(total, groups);
   // the runs that hold the request's first and last page
@@ -596,7 +685,7 @@ __global__ void __launch_bounds__(kThreads) merge_kernel(const DecodeArgs a, con
     }
   }
   if constexpr (WARPS > 1) {
-    __shared__ float dens[kWarps];
+    __shared__ float dens[kMergeWarps];
     red[warp][lane] = acc;
     if (lane == 0) dens[warp] = den;
     __syncthreads();
@@ -651,17 +740,17 @@ int launch(const DecodeArgs& a, cudaStream_t s) {
 
   // Few requests are cut into many partials: all warps of a CTA share a row's then.
   const bool wide = groups >= 8 * a.batch;
-  const int tasks = a.q_len * a.heads * (D / 128), per_cta = wide ? 1 : kWarps;
+  const int tasks = a.q_len * a.heads * (D / 128), per_cta = wide ? 1 : kMergeWarps;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((tasks + per_cta - 1) / per_cta, a.batch);
-  cfg.blockDim = dim3(kThreads);
+  cfg.blockDim = dim3(kMergeThreads);
   cfg.stream = s;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  const auto kernel = wide ? merge_kernel<D, kWarps> : merge_kernel<D, 1>;
+  const auto kernel = wide ? merge_kernel<D, kMergeWarps> : merge_kernel<D, 1>;
   return cudaLaunchKernelEx(&cfg, kernel, a, part, groups, blocks) == cudaSuccess ? ROLAQ_OK : ROLAQ_ECUDA;
 }
 
