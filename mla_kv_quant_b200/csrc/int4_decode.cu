@@ -11,12 +11,13 @@
 //
 // A CTA holds 16 query rows (query tokens x heads) and walks the pages of one or more requests; a page
 // (64 tokens) is one pipeline stage (TMA, 128-byte swizzle, so that ldmatrix reads without conflicts).
-// Eight warps score: a pair takes 16 of the page's tokens, each warp of it half of the latent columns
-// (the query's operand registers would not fit otherwise), and they swap partial scores so that each
-// holds 8 tokens' whole ones.  It weighs them against a reference maximum that moves only when a score
-// passes it by 2^10 and writes P s of each group to shared memory.  Four warps add up: each holds D/4
-// latent columns of the result and takes page i while the others score page i + 1.  The scoring warps
-// vote once a page on moving the references; a move leaves the factors for the sums beside the weights.
+// The 8 warps form pairs: a pair scores 16 of the page's tokens, each warp of it over half of the latent
+// columns (the query's operand registers would not fit otherwise), and swaps partial scores so that each
+// warp holds 8 tokens' whole ones.  It weighs them against a reference maximum that moves only when a
+// score passes it by 2^10 and writes P s of each group to shared memory.  Each warp adds up D/8 latent
+// columns of the result.  Page i + 1 is scored and page i added up in one iteration, so that the products
+// of the one hide the latencies of the other; the iteration's one CTA-wide barrier also carries the
+// vote on moving the references.  One warp more feeds the stages.
 //
 // The pages of all requests are dealt to the CTAs in one equal run each (a run may begin or end inside
 // a request); what is cut is joined by merge_kernel by log-sum-exp.
@@ -29,8 +30,10 @@ namespace rolaq {
 namespace i4 {
 namespace {
 
-constexpr int kScorers = 8, kAdders = 4;  // warps
-constexpr int kScoreThreads = kScorers * 32, kThreads = (kScorers + kAdders) * 32;
+// Eight working warps and a warpgroup of which one warp loads.  Of the 168 registers a thread that a block of
+// 384 is launched with, the loaders hand most to the workers: 232 + 232 + 40 = 3 * 168.
+constexpr int kWarps = 8, kWorkers = kWarps * 32, kThreads = kWorkers + 128;
+constexpr int kWorkerRegs = 232, kLoaderRegs = 40;
 constexpr int kRows = 16;  // query rows of a CTA
 constexpr int kMinPages = 2;     // least run of pages worth a CTA of its own
 constexpr float kSlack = 10.f;   // log2 of how far a weight may pass its reference
@@ -45,31 +48,25 @@ struct Cfg {
   static constexpr int STAGES = D == 512 ? 7 : 12;
   static constexpr int PBUF = NG * kRows * kPage * 2;  // P s of a page: [group][row][token] FP16
   static constexpr int SMEM = 1024 + STAGES * STAGE + 2 * PBUF;
-  static constexpr int HG = NG / 2;                 // groups of a scoring warp
-  static constexpr int NT = D / kAdders / 8;        // 8-column tiles of an adding warp
+  static constexpr int HG = NG / 2;                 // groups that a warp scores
+  static constexpr int CH = D / kWarps / 32;        // 32-column chunks that a warp adds up
 };
 
-// What a page's weights carry beside them, and a request's denominators: the scoring warps to the adding.
 template <int NG>
 struct Shared {
-  float4 swap[2][kScorers][32];
-  float red_m[kScorers][kRows], red_s[kScorers][NG];
-  float keep[2][kRows], keep_unit[2][NG];  // factors for the sums before page i (i & 1), where moved[i & 1]
-  int moved[2];
-  float l[kScorers][kRows], z[kScorers][kRows][NG], m[kRows], unit[NG];  // of a finished request
+  float4 swap[2][kWarps][32];
+  float red_m[kWarps][kRows], red_s[kWarps][NG], red_z[kWarps][kRows][NG];
 };
 
-// Named barriers: 1..4 the pairs, 5 all scoring warps, 6 / 7 a request's sums written / read.
-enum { kBarPair = 1, kBarScore = 5, kBarSums = 6, kBarTaken = 7 };
-__device__ __forceinline__ void bar_arrive(int id, int threads) {
-  asm volatile("bar.arrive %0, %1;" ::"r"(id), "r"(threads) : "memory");
-}
-__device__ __forceinline__ bool bar_any(int id, int threads, bool vote) {
+// Named barriers: 1..4 the pairs, 5 all working warps.
+constexpr int kBarPair = 1, kBarWork = 5;
+__device__ __forceinline__ void work_sync() { named_bar_sync(kBarWork, kWorkers); }
+__device__ __forceinline__ bool work_any(bool vote) {
   int any;
   asm volatile(
       "{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %3, 0;\n\tbar.red.or.pred q, %1, %2, p;\n\tselp.b32 %0, 1, 0, q;\n\t}"
       : "=r"(any)
-      : "r"(id), "r"(threads), "r"(static_cast<int>(vote))
+      : "n"(kBarWork), "n"(kWorkers), "r"(static_cast<int>(vote))
       : "memory");
   return any != 0;
 }
@@ -157,11 +154,12 @@ __global__ void __launch_bounds__(kThreads, 1)
     decode_kernel(const __grid_constant__ CUtensorMap map_codes, const __grid_constant__ CUtensorMap map_rope,
                   const DecodeArgs a, const Partials part, const int groups, const int blocks) {
   using C = Cfg<D, DR>;
-  constexpr int NG = C::NG, HG = C::HG, STAGES = C::STAGES;
+  constexpr int NG = C::NG, HG = C::HG, CH = C::CH, STAGES = C::STAGES;
+  constexpr int KR = DR / 32;  // 16-column steps of the rotary part that a warp scores
   extern __shared__ char raw[];
   char* smem = reinterpret_cast<char*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
   char* pbuf = smem + STAGES * C::STAGE;
-  __shared__ uint64_t full[STAGES], empty[STAGES], p_full[2], p_empty[2];
+  __shared__ uint64_t full[STAGES], empty[STAGES];
   __shared__ int bad_page[STAGES];
   __shared__ int64_t scan[kThreads / 32];
   __shared__ int start[2];
@@ -169,7 +167,6 @@ __global__ void __launch_bounds__(kThreads, 1)
 
   const int tid = threadIdx.x, warp = tid / 32, lane = tid & 31, g = lane >> 2, j = lane & 3;
   const int block = blockIdx.x % blocks, group = blockIdx.x / blocks;
-  const uint32_t stages = smem_u32(smem), pbufs = smem_u32(pbuf);
   grid_launch_dependents();
 
   // ---- this CTA's run of pages ----
@@ -177,8 +174,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   int64_t mine = 0, total;
   for (int b = tid * per; b < min(a.batch, (tid + 1) * per); ++b) mine += pages_of(a, b);
   if (tid == 0) {
-    for (int s = 0; s < STAGES; ++s) mbar_init(&full[s], 1), mbar_init(&empty[s], kAdders);
-    for (int s = 0; s < 2; ++s) mbar_init(&p_full[s], 1), mbar_init(&p_empty[s], kAdders);
+    for (int s = 0; s < STAGES; ++s) mbar_init(&full[s], 1), mbar_init(&empty[s], 1);
     fence_mbar_init();
   }
   int64_t before = block_scan<kThreads / 32>(mine, total, scan);
@@ -194,168 +190,69 @@ __global__ void __launch_bounds__(kThreads, 1)
   }
   __syncthreads();
   int seg_b = start[0], seg_p = start[1];
-  int done = 0;       // pages of the run done
-  int stage = 0, lap = 0;  // of page `done`: full[stage]'s phase is lap & 1
   bool healthy = true;
   auto wait_for = [&](uint64_t* bar, int phase) {
     if (healthy) healthy = mbar_wait(bar, phase & 1, a.err);
   };
-  auto advance = [&]() {
-    ++done;
-    if (++stage == STAGES) stage = 0, ++lap;
-  };
 
-  if (warp >= kScorers) {
-    // ================= adding warps: D / 4 latent columns each =================
-    const int w = warp - kScorers;
-    // the page stream (warp 0, lane 0): stage k holds page k of the run
+  if (warp >= kWarps) {  // ================= the loading warp: stage k holds page k of the run =================
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kLoaderRegs));
+    if (tid != kWorkers) return;
+    prefetch_tensormap(&map_codes);
+    prefetch_tensormap(&map_rope);
     const int pool_pages = static_cast<int>(a.cache.num_slots / kPage);
-    int load_b = seg_b, load_p = seg_p, load_n = 0, load_id = 0, loaded = 0, load_stage = 0, load_lap = 0;
-    auto next_id = [&]() {  // the page that (load_b, load_p) names, requested a page ahead of its use
-      while (load_p >= load_n) {
-        if (load_n != 0) ++load_b, load_p = 0;
-        load_n = pages_of(a, load_b);
-        if (load_n == 0) ++load_b, load_p = 0;
+    int n = pages_of(a, seg_b), stage = 0, lap = 0;
+    int next = a.page_table[seg_b * a.pt_stride + seg_p];
+    for (int i = 0; i < n_units; ++i) {
+      const int id = next;
+      if (i + 1 < n_units) {  // the next page's id is on its way while this page's stage is awaited
+        if (++seg_p == n) {
+          seg_p = 0;
+          do n = pages_of(a, ++seg_b);
+          while (n == 0);
+        }
+        next = a.page_table[seg_b * a.pt_stride + seg_p];
       }
-      load_id = a.page_table[load_b * a.pt_stride + load_p++];
-    };
-    auto load = [&]() {
-      const bool ok = load_id >= 0 && load_id < pool_pages;
-      const int page = ok ? load_id : 0;
-      char* dst = smem + load_stage * C::STAGE;
-      uint64_t* bar = &full[load_stage];
-      bad_page[load_stage] = !ok;
+      if (lap > 0) wait_for(&empty[stage], lap - 1);
+      const bool ok = id >= 0 && id < pool_pages;
+      const int page = ok ? id : 0;
+      char* dst = smem + stage * C::STAGE;
+      uint64_t* bar = &full[stage];
+      bad_page[stage] = !ok;
       if (!ok) report(a.err, ROLAQ_DEV_BAD_PAGE);
       mbar_expect_tx(bar, C::STAGE);
 #pragma unroll
       for (int k = 0; k < D / 256; ++k) tma_load_2d(dst + k * 8192, &map_codes, bar, k * 128, page * kPage);
       tma_load_2d(dst + C::CODES, &map_rope, bar, 0, page * kPage);
       bulk_load(dst + C::CODES + C::ROPE, a.cache.params + static_cast<int64_t>(page) * (kPage * NG * 2), C::PARAMS, bar);
-      if (++load_stage == STAGES) load_stage = 0, ++load_lap;
-      if (++loaded < n_units) next_id();
-    };
-    if (w == 0 && lane == 0) {
-      prefetch_tensormap(&map_codes);
-      prefetch_tensormap(&map_rope);
-      next_id();
-      while (loaded < min(n_units, STAGES)) load();
-    }
-    const int own = w * NG / kAdders;  // the group of the warp's columns
-    const uint32_t p_off = own * (kRows * 128);
-    constexpr int CH = C::NT / 4;  // 16-byte chunks (32 columns) of the warp
-    while (done < n_units) {
-      const int seg_pages = pages_of(a, seg_b);
-      if (seg_pages == 0) {
-        ++seg_b;
-        continue;
-      }
-      const int count = min(seg_pages - seg_p, n_units - done);
-      const bool first = done == 0;
-      float acc[C::NT][4];
-#pragma unroll
-      for (int n = 0; n < C::NT; ++n)
-#pragma unroll
-        for (int k = 0; k < 4; ++k) acc[n][k] = 0.f;
-      for (int i = 0; i < count; ++i) {
-        const int pb = done & 1;
-        wait_for(&p_full[pb], done >> 1);
-        if (sh.moved[pb]) {
-          const float ku = sh.keep_unit[pb][own], k0 = sh.keep[pb][g] * ku, k1 = sh.keep[pb][g + 8] * ku;
-#pragma unroll
-          for (int n = 0; n < C::NT; ++n) acc[n][0] *= k0, acc[n][1] *= k0, acc[n][2] *= k1, acc[n][3] *= k1;
-        }
-        const uint32_t st = stages + stage * C::STAGE, ps = pbufs + pb * C::PBUF + p_off;
-        uint32_t pa[4][4];
-#pragma unroll
-        for (int kk = 0; kk < 4; ++kk) ldsm_x4(ps + sw128(lane & 15, 2 * kk + (lane >> 4)), pa[kk]);
-#pragma unroll
-        for (int c = 0; c < CH; ++c) {
-          const int chunk = w * CH + c;  // of the row
-          uint32_t x[2][4];              // tokens 0..31, 32..63
-#pragma unroll
-          for (int h = 0; h < 2; ++h) ldsm_x4_t(st + (chunk / 8) * 8192 + sw128(32 * h + lane, chunk & 7), x[h]);
-#pragma unroll
-          for (int kk = 0; kk < 4; ++kk) {
-            const uint32_t u = x[kk / 2][2 * (kk & 1)], v = x[kk / 2][2 * (kk & 1) + 1];
-            const uint32_t u8 = u >> 8, v8 = v >> 8;
-            mma_f16(acc[4 * c], pa[kk], u & 0x000F000Fu, v & 0x000F000Fu);
-            mma_f16(acc[4 * c + 1], pa[kk], u & 0x00F000F0u, v & 0x00F000F0u);
-            mma_f16(acc[4 * c + 2], pa[kk], u8 & 0x000F000Fu, v8 & 0x000F000Fu);
-            mma_f16(acc[4 * c + 3], pa[kk], u8 & 0x00F000F0u, v8 & 0x00F000F0u);
-          }
-        }
-        __syncwarp();
-        if (lane == 0) {
-          mbar_arrive(&p_empty[pb]);
-          mbar_arrive(&empty[stage]);
-        }
-        // refill the stage that all four warps left a page ago
-        if (w == 0 && lane == 0 && loaded < n_units && loaded < done + STAGES) {
-          wait_for(&empty[load_stage], load_lap - 1);
-          load();
-        }
-        advance();
-      }
-      // ---- the rows' results ----
-      named_bar_sync(kBarSums, kThreads);
-      const bool whole = seg_p == 0 && count == seg_pages;
-      const float u = sh.unit[own], inv_u = u == 0.f ? 0.f : 1.f / u;
-      float z[2] = {0.f, 0.f}, l[2] = {0.f, 0.f}, lse[2];
-#pragma unroll
-      for (int r = 0; r < 2; ++r) {
-        for (int k = 0; k < kScorers; ++k) l[r] += sh.l[k][g + 8 * r], z[r] += sh.z[k][g + 8 * r][own];
-        lse[r] = l[r] == 0.f ? -INFINITY : (sh.m[g + 8 * r] + log2f(l[r])) * kLn2;
-      }
-      bar_arrive(kBarTaken, kThreads);
-      // a cut request's partial: slot 0 where the run begins in (or with) this request, else 1
-      const int64_t slot = (static_cast<int64_t>(2 * group + (first ? 0 : 1)) * blocks + block) * kRows;
-#pragma unroll
-      for (int r = 0; r < 2; ++r) {
-        const int row = block * kRows + g + 8 * r;
-        const float inv = l[r] == 0.f ? 0.f : inv_u / l[r];
-        const bool live = row < a.q_len * a.heads;
-        const int t = live ? row / a.heads : 0, h = live ? row % a.heads : 0;
-        uint16_t* out = a.out + seg_b * a.o_sb + t * a.o_st + h * a.o_sh;
-        float* out_part = part.o + (slot + g + 8 * r) * D;
-#pragma unroll
-        for (int c = 0; c < CH; ++c) {
-          const int col = 32 * (w * CH + c) + 8 * j;
-          float v[8];
-#pragma unroll
-          for (int i = 0; i < 4; ++i)
-#pragma unroll
-            for (int k = 0; k < 2; ++k)
-              v[4 * k + i] = fmaf(acc[4 * c + i][2 * r + k], i & 1 ? 1048576.f : 16777216.f, -z[r]) * inv;
-          if (!whole) {
-            reinterpret_cast<float4*>(out_part + col)[0] = make_float4(v[0], v[1], v[2], v[3]);
-            reinterpret_cast<float4*>(out_part + col)[1] = make_float4(v[4], v[5], v[6], v[7]);
-          } else if (live) {
-            *reinterpret_cast<uint4*>(out + col) = make_uint4(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]),
-                                                              pack_bf16x2(v[4], v[5]), pack_bf16x2(v[6], v[7]));
-          }
-        }
-        if (w == 0 && j == 0) {
-          if (!whole) part.lse[slot + g + 8 * r] = lse[r];
-          else if (live && a.lse) a.lse[(static_cast<int64_t>(seg_b) * a.q_len + t) * a.heads + h] = lse[r];
-        }
-      }
-      ++seg_b;
-      seg_p = 0;
+      if (++stage == STAGES) stage = 0, ++lap;
     }
     return;
   }
 
-  // ================= scoring warps =================
+  asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kWorkerRegs));
   const int half = warp & 1, quarter = warp >> 1;  // half of the latent columns, 16 of the page's tokens
-  constexpr int KR = DR / 32;                      // 16-column steps of the rotary part, half of them here
+  const int own = warp * NG / kWarps;              // the group of the columns that the warp adds up
+  // Offsets of the lane's ldmatrix rows from a 1024-byte boundary.  Chunk c of a row lies at c ^ row % 8, so
+  // chunk c ^ x is at the address ^ 16 x.
+  const uint32_t stages = smem_u32(smem), pbufs = smem_u32(pbuf);
+  const int tok_row = 16 * quarter + 8 * half + (lane & 7);  // tile 0: the warp's own tokens; tile 1: row ^ 8
+  const uint32_t code_off = D == 512 ? half * 8192 + sw128(tok_row, lane >> 3) : sw128(tok_row, 4 * half + (lane >> 3));
+  const uint32_t rope_off = C::CODES + (DR == 64 ? sw128(tok_row, 4 * half + (lane >> 3))
+                                                 : sw64(tok_row ^ ((lane >> 4) * 8), 2 * half + ((lane >> 3) & 1)));
+  const uint32_t add_off = (warp * CH / 8) * 8192 + sw128(lane, (warp * CH) & 7);
+  const uint32_t p_off = own * (kRows * 128) + sw128(lane & 15, lane >> 4);
+  const uint32_t p_dst = g * 128 + ((warp ^ g) << 4) + 4 * j;
   const float qk_scale = a.sm_scale * kLog2e;
-  bool begun = false;
+  int done = 0, stage = 0, lap = 0;  // pages of the run added up; the stage of page `done`, its phase
+
   while (done < n_units) {
     const int seg_pages = pages_of(a, seg_b);
     if (seg_pages == 0) {
       ++seg_b;
       continue;
     }
+    const bool first = done == 0;
     const int count = min(seg_pages - seg_p, n_units - done);
     const int len = min(static_cast<int64_t>(a.seq_lens[seg_b]), static_cast<int64_t>(a.max_pages) * kPage);
     if (tid == 0 && len != a.seq_lens[seg_b]) report(a.err, ROLAQ_DEV_BAD_REQ);
@@ -418,90 +315,91 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
     }
 
-    float zsum[2][NG], unit[NG], l_sum[2] = {0.f, 0.f}, m_ref[2] = {-INFINITY, -INFINITY};
+    float acc[4 * CH][4], zsum[2][NG], unit[NG], l_sum[2] = {0.f, 0.f}, m_ref[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+    for (int n = 0; n < 4 * CH; ++n) acc[n][0] = acc[n][1] = acc[n][2] = acc[n][3] = 0.f;
 #pragma unroll
     for (int k = 0; k < NG; ++k) zsum[0][k] = zsum[1][k] = unit[k] = 0.f;
 
-    for (int i = 0; i < count; ++i) {
-      const int p = seg_p + i, pb = done & 1;
-      wait_for(&full[stage], lap);
-      const uint32_t st = stages + stage * C::STAGE;
-      const char* st_ptr = smem + stage * C::STAGE;
-      // ---- partial scores of 16 tokens: tile 0 the warp's own eight, tile 1 its partner's ----
-      float part_s[2][4];
-      {
-        float c_acc[2][HG][4], r_acc[2][4];
-        uint32_t w[2][HG][4], w_pe[2][4];
+    float s_val[4], s_tok[2][NG], z_tok[2][NG], p_val[4];  // of the warp's 8 tokens of the page being scored
+
+    // Partial scores of 16 tokens into the pair's swap.
+    float mine_s[4];
+    auto score = [&](int st_at, int pb) {
+      const uint32_t st = stages + st_at * C::STAGE;
+      float c_acc[2][HG][4], r_acc[2][4];
+      uint32_t w[2][HG][4], w_pe[2][4];
 #pragma unroll
-        for (int n = 0; n < 2; ++n) {
-          const int row = 16 * quarter + 8 * (half ^ n) + (lane & 7);
+      for (int n = 0; n < 2; ++n) {
 #pragma unroll
-          for (int k = 0; k < HG; ++k)
-            ldsm_x4(D == 512 ? st + half * 8192 + sw128(row, 4 * k + (lane >> 3)) : st + sw128(row, 4 * half + (lane >> 3)),
-                    w[n][k]);
-          if (DR == 64)
-            ldsm_x4(st + C::CODES + sw128(row, 4 * half + (lane >> 3)), w_pe[n]);
+        for (int k = 0; k < HG; ++k) ldsm_x4((st + (code_off ^ (n << 10))) ^ (k << 6), w[n][k]);
+        if (DR == 64) ldsm_x4(st + (rope_off ^ (n << 10)), w_pe[n]);
 #pragma unroll
-          for (int x = 0; x < 4; ++x) {
-            r_acc[n][x] = 0.f;
+        for (int x = 0; x < 4; ++x) {
+          r_acc[n][x] = 0.f;
 #pragma unroll
-            for (int k = 0; k < HG; ++k) c_acc[n][k][x] = 0.f;
-          }
-        }
-        if (DR == 32) {  // both tiles' two chunks at once
-          const int n = lane >> 4, row = 16 * quarter + 8 * (half ^ n) + (lane & 7);
-          uint32_t both[4];
-          ldsm_x4(st + C::CODES + sw64(row, 2 * half + ((lane >> 3) & 1)), both);
-          w_pe[0][0] = both[0], w_pe[0][1] = both[1], w_pe[1][0] = both[2], w_pe[1][1] = both[3];
-        }
-        // the accumulators in turn, so that no product waits for the one before it
-#pragma unroll
-        for (int c = 0; c < KR; ++c)
-#pragma unroll
-          for (int n = 0; n < 2; ++n) mma_bf16(r_acc[n], q_pe[c], w_pe[n][2 * c], w_pe[n][2 * c + 1]);
-#pragma unroll
-        for (int c = 0; c < 4; ++c)
-#pragma unroll
-          for (int e = 0; e < 2; ++e)
-#pragma unroll
-            for (int k = 0; k < HG; ++k)
-#pragma unroll
-              for (int n = 0; n < 2; ++n) {
-                const uint32_t v = e ? w[n][k][c] >> 8 : w[n][k][c];
-                mma_f16(c_acc[n][k], q[8 * k + 2 * c + e], v & 0x000F000Fu, v & 0x00F000F0u);
-              }
-#pragma unroll
-        for (int n = 0; n < 2; ++n) {
-          const int tok = 16 * quarter + 8 * (half ^ n) + 2 * j;
-          float s[2][HG], z[2][HG];
-          const float* par = reinterpret_cast<const float*>(st_ptr + C::CODES + C::ROPE) + tok * (NG * 2) + half * (HG * 2);
-#pragma unroll
-          for (int t = 0; t < 2; ++t) {
-            if constexpr (HG == 2) {
-              const float4 v = *reinterpret_cast<const float4*>(par + t * (NG * 2));
-              s[t][0] = v.x, z[t][0] = v.y, s[t][1] = v.z, z[t][1] = v.w;
-            } else {
-              const float2 v = *reinterpret_cast<const float2*>(par + t * (NG * 2));
-              s[t][0] = v.x, z[t][0] = v.y;
-            }
-          }
-#pragma unroll
-          for (int x = 0; x < 4; ++x) {
-            float v = r_acc[n][x];
-#pragma unroll
-            for (int k = 0; k < HG; ++k) v = fmaf(s[x & 1][k], fmaf(-z[x & 1][k], q_sum[x >> 1][k], c_acc[n][k][x]), v);
-            part_s[n][x] = v;
-          }
+          for (int k = 0; k < HG; ++k) c_acc[n][k][x] = 0.f;
         }
       }
-      sh.swap[pb][warp][lane] = make_float4(part_s[1][0], part_s[1][1], part_s[1][2], part_s[1][3]);
+      if (DR == 32) {  // both tiles' two chunks at once
+        uint32_t both[4];
+        ldsm_x4(st + rope_off, both);
+        w_pe[0][0] = both[0], w_pe[0][1] = both[1], w_pe[1][0] = both[2], w_pe[1][1] = both[3];
+      }
+      // the accumulators in turn, so that no product waits for the one before it
+#pragma unroll
+      for (int c = 0; c < KR; ++c)
+#pragma unroll
+        for (int n = 0; n < 2; ++n) mma_bf16(r_acc[n], q_pe[c], w_pe[n][2 * c], w_pe[n][2 * c + 1]);
+#pragma unroll
+      for (int c = 0; c < 4; ++c)
+#pragma unroll
+        for (int e = 0; e < 2; ++e)
+#pragma unroll
+          for (int k = 0; k < HG; ++k)
+#pragma unroll
+            for (int n = 0; n < 2; ++n) {
+              const uint32_t v = e ? w[n][k][c] >> 8 : w[n][k][c];
+              mma_f16(c_acc[n][k], q[8 * k + 2 * c + e], v & 0x000F000Fu, v & 0x00F000F0u);
+            }
+      float sum[2][4];
+      const char* params = smem + st_at * C::STAGE + C::CODES + C::ROPE + half * (HG * 8);
+#pragma unroll
+      for (int n = 0; n < 2; ++n) {
+        const float* par = reinterpret_cast<const float*>(params) + ((8 * warp) ^ (8 * n)) * (NG * 2) + 2 * j * (NG * 2);
+        float s[2][HG], z[2][HG];
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+          if constexpr (HG == 2) {
+            const float4 v = *reinterpret_cast<const float4*>(par + t * (NG * 2));
+            s[t][0] = v.x, z[t][0] = v.y, s[t][1] = v.z, z[t][1] = v.w;
+          } else {
+            const float2 v = *reinterpret_cast<const float2*>(par + t * (NG * 2));
+            s[t][0] = v.x, z[t][0] = v.y;
+          }
+        }
+#pragma unroll
+        for (int x = 0; x < 4; ++x) {
+          sum[n][x] = r_acc[n][x];
+#pragma unroll
+          for (int k = 0; k < HG; ++k)
+            sum[n][x] = fmaf(s[x & 1][k], fmaf(-z[x & 1][k], q_sum[x >> 1][k], c_acc[n][k][x]), sum[n][x]);
+        }
+      }
+#pragma unroll
+      for (int x = 0; x < 4; ++x) mine_s[x] = sum[0][x];
+      sh.swap[pb][warp][lane] = make_float4(sum[1][0], sum[1][1], sum[1][2], sum[1][3]);
+    };
+
+    // The whole scores of the warp's 8 tokens, in log2 units, and their params.
+    auto join = [&](int st_at, int pb, int p) {
       named_bar_sync(kBarPair + quarter, 64);
       const float4 theirs = sh.swap[pb][warp ^ 1][lane];
-      // ---- scores of the warp's 8 tokens, in log2 units; their params ----
-      float s_val[4] = {(part_s[0][0] + theirs.x) * row_scale[0], (part_s[0][1] + theirs.y) * row_scale[0],
-                        (part_s[0][2] + theirs.z) * row_scale[1], (part_s[0][3] + theirs.w) * row_scale[1]};
-      float s_tok[2][NG], z_tok[2][NG], p_val[4];
-      const float4* par = reinterpret_cast<const float4*>(st_ptr + C::CODES + C::ROPE) + (8 * warp + 2 * j) * (NG / 2);
+      s_val[0] = (mine_s[0] + theirs.x) * row_scale[0];
+      s_val[1] = (mine_s[1] + theirs.y) * row_scale[0];
+      s_val[2] = (mine_s[2] + theirs.z) * row_scale[1];
+      s_val[3] = (mine_s[3] + theirs.w) * row_scale[1];
+      const float4* par = reinterpret_cast<const float4*>(smem + st_at * C::STAGE + C::CODES + C::ROPE) + (8 * warp + 2 * j) * (NG / 2);
 #pragma unroll
       for (int t = 0; t < 2; ++t)
 #pragma unroll
@@ -509,7 +407,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           const float4 v = par[t * (NG / 2) + k / 2];
           s_tok[t][k] = v.x, z_tok[t][k] = v.y, s_tok[t][k + 1] = v.z, z_tok[t][k + 1] = v.w;
         }
-      const int bad = bad_page[stage];
+      const int bad = bad_page[st_at];
       if ((p + 1) * kPage > lim_min || bad) {  // the request's end, or a page that is not there
         const int tok = p * kPage + 8 * warp + 2 * j;
 #pragma unroll
@@ -522,74 +420,76 @@ __global__ void __launch_bounds__(kThreads, 1)
             if (tok + t >= lim[r] || bad) s_val[2 * r + t] = -INFINITY;
         }
       }
-      if (done >= 2) wait_for(&p_empty[pb], (done >> 1) - 1);
+    };
 
-      // Weights against the present references, times each group's scale, to shared memory; true where
-      // a score or a scale has left its reference behind.
-      auto weigh = [&]() {
-        bool need = false;
+    // Weights against the present references, times each group's scale, to shared memory; true where a
+    // score or a scale has left its reference behind.
+    auto weigh = [&](int pb) {
+      bool need = false;
 #pragma unroll
-        for (int x = 0; x < 4; ++x) {
-          const float m = m_ref[x >> 1];
-          need |= s_val[x] > m + kSlack;
-          p_val[x] = ex2_approx(s_val[x] - (m == -INFINITY ? 0.f : m));
-        }
-        char* dst = pbuf + pb * C::PBUF + 4 * j;
-#pragma unroll
-        for (int k = 0; k < NG; ++k) {
-          const float s0 = s_tok[0][k] * unit[k], s1 = s_tok[1][k] * unit[k];
-          need |= fmaxf(fabsf(s0), fabsf(s1)) > kScaleSlack;
-#pragma unroll
-          for (int r = 0; r < 2; ++r)
-            *reinterpret_cast<uint32_t*>(dst + k * (kRows * 128) + sw128(g + 8 * r, warp)) =
-                pack_half2(p_val[2 * r] * s0, p_val[2 * r + 1] * s1);
-        }
-        return need;
-      };
-      const bool move = bar_any(kBarScore, kScoreThreads, weigh());
-      if (move) {  // new references: the page's maxima; the sums so far are brought to them
-#pragma unroll
-        for (int r = 0; r < 2; ++r) {
-          const float m = quad_max(fmaxf(s_val[2 * r], s_val[2 * r + 1]));
-          if (j == 0) sh.red_m[warp][g + 8 * r] = m;
-        }
-#pragma unroll
-        for (int k = 0; k < NG; ++k) {
-          const float s = quad_max(fmaxf(fabsf(s_tok[0][k]), fabsf(s_tok[1][k])));
-          if (lane == 0) sh.red_s[warp][k] = s;
-        }
-        named_bar_sync(kBarScore, kScoreThreads);
-        float keep[2];
-#pragma unroll
-        for (int r = 0; r < 2; ++r) {
-          float m = m_ref[r];
-          for (int w = 0; w < kScorers; ++w) m = fmaxf(m, sh.red_m[w][g + 8 * r]);
-          keep[r] = m_ref[r] == m ? 1.f : ex2_approx(m_ref[r] - m);
-          m_ref[r] = m;
-          l_sum[r] *= keep[r];
-          if (warp == 0 && j == 0) sh.keep[pb][g + 8 * r] = keep[r];
-        }
-#pragma unroll
-        for (int k = 0; k < NG; ++k) {
-          float s = 0.f;
-          for (int w = 0; w < kScorers; ++w) s = fmaxf(s, sh.red_s[w][k]);
-          float keep_unit = 1.f;
-          if (s > 0.f && (unit[k] == 0.f || s * unit[k] > kScaleSlack)) {
-            const float u = pow2(min(max(127 - static_cast<int>(__float_as_uint(s) >> 23), -120), 120));
-            if (unit[k] != 0.f) keep_unit = u / unit[k];
-            unit[k] = u;
-          }
-          if (tid == 0) sh.keep_unit[pb][k] = keep_unit;
-          zsum[0][k] *= keep[0] * keep_unit;
-          zsum[1][k] *= keep[1] * keep_unit;
-        }
-        weigh();
-        named_bar_sync(kBarScore, kScoreThreads);
+      for (int x = 0; x < 4; ++x) {
+        const float m = m_ref[x >> 1];
+        need |= s_val[x] > m + kSlack;
+        p_val[x] = ex2_approx(s_val[x] - (m == -INFINITY ? 0.f : m));
       }
-      if (tid == 0) {
-        sh.moved[pb] = move;
-        mbar_arrive(&p_full[pb]);
+      char* dst = pbuf + pb * C::PBUF + p_dst;
+#pragma unroll
+      for (int k = 0; k < NG; ++k) {
+        const float s0 = s_tok[0][k] * unit[k], s1 = s_tok[1][k] * unit[k];
+        need |= fmaxf(fabsf(s0), fabsf(s1)) > kScaleSlack;
+#pragma unroll
+        for (int r = 0; r < 2; ++r)
+          *reinterpret_cast<uint32_t*>(dst + k * (kRows * 128) + r * 1024) = pack_half2(p_val[2 * r] * s0, p_val[2 * r + 1] * s1);
       }
+      return need;
+    };
+
+    // New references: the page's maxima; the sums so far are brought to them.
+    auto move_references = [&](int pb) {
+#pragma unroll
+      for (int r = 0; r < 2; ++r) {
+        const float m = quad_max(fmaxf(s_val[2 * r], s_val[2 * r + 1]));
+        if (j == 0) sh.red_m[warp][g + 8 * r] = m;
+      }
+#pragma unroll
+      for (int k = 0; k < NG; ++k) {
+        const float s = quad_max(fmaxf(fabsf(s_tok[0][k]), fabsf(s_tok[1][k])));
+        if (lane == 0) sh.red_s[warp][k] = s;
+      }
+      work_sync();
+      float keep[2], keep_own = 1.f;
+#pragma unroll
+      for (int r = 0; r < 2; ++r) {
+        float m = m_ref[r];
+        for (int w = 0; w < kWarps; ++w) m = fmaxf(m, sh.red_m[w][g + 8 * r]);
+        keep[r] = m_ref[r] == m ? 1.f : ex2_approx(m_ref[r] - m);
+        m_ref[r] = m;
+        l_sum[r] *= keep[r];
+      }
+#pragma unroll
+      for (int k = 0; k < NG; ++k) {
+        float s = 0.f;
+        for (int w = 0; w < kWarps; ++w) s = fmaxf(s, sh.red_s[w][k]);
+        float keep_unit = 1.f;
+        if (s > 0.f && (unit[k] == 0.f || s * unit[k] > kScaleSlack)) {
+          const float u = pow2(min(max(127 - static_cast<int>(__float_as_uint(s) >> 23), -120), 120));
+          if (unit[k] != 0.f) keep_unit = u / unit[k];
+          unit[k] = u;
+        }
+        if (k == own) keep_own = keep_unit;
+        zsum[0][k] *= keep[0] * keep_unit;
+        zsum[1][k] *= keep[1] * keep_unit;
+      }
+#pragma unroll
+      for (int n = 0; n < 4 * CH; ++n)
+#pragma unroll
+        for (int x = 0; x < 4; ++x) acc[n][x] *= keep[x >> 1] * keep_own;
+      weigh(pb);
+      work_sync();
+    };
+
+    // After the references stand: the denominators and the zeros' share.
+    auto add_weights = [&]() {
       l_sum[0] += p_val[0] + p_val[1];
       l_sum[1] += p_val[2] + p_val[3];
 #pragma unroll
@@ -598,30 +498,109 @@ __global__ void __launch_bounds__(kThreads, 1)
         zsum[0][k] = fmaf(p_val[0], a0, fmaf(p_val[1], a1, zsum[0][k]));
         zsum[1][k] = fmaf(p_val[2], a0, fmaf(p_val[3], a1, zsum[1][k]));
       }
-      advance();
+    };
+
+    // acc += (P s) c over tokens 32 h .. 32 h + 31 of a page, the warp's columns.
+    auto gather = [&](int st_at, int pb, int h) {
+      const uint32_t st = stages + st_at * C::STAGE + add_off, ps = pbufs + pb * C::PBUF + p_off;
+      uint32_t pa[2][4], x[CH][4];
+#pragma unroll
+      for (int i = 0; i < 2; ++i) ldsm_x4(ps ^ ((2 * h + i) << 5), pa[i]);
+#pragma unroll
+      for (int c = 0; c < CH; ++c) ldsm_x4_t((st + h * 4096) ^ (c << 4), x[c]);
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int c = 0; c < CH; ++c) {
+          const uint32_t u = x[c][2 * i], v = x[c][2 * i + 1], u8 = u >> 8, v8 = v >> 8;
+          mma_f16(acc[4 * c], pa[i], u & 0x000F000Fu, v & 0x000F000Fu);
+          mma_f16(acc[4 * c + 1], pa[i], u & 0x00F000F0u, v & 0x00F000F0u);
+          mma_f16(acc[4 * c + 2], pa[i], u8 & 0x000F000Fu, v8 & 0x000F000Fu);
+          mma_f16(acc[4 * c + 3], pa[i], u8 & 0x00F000F0u, v8 & 0x00F000F0u);
+        }
+    };
+
+    // ---- the pages ----
+    wait_for(&full[stage], lap);
+    score(stage, done & 1);
+    join(stage, done & 1, seg_p);
+    if (work_any(weigh(done & 1))) move_references(done & 1);
+    add_weights();
+    for (int i = 1; i < count; ++i) {
+      const int pb = done & 1, was = stage;
+      if (++stage == STAGES) stage = 0, ++lap;
+      wait_for(&full[stage], lap);
+      score(stage, pb ^ 1);
+      gather(was, pb, 0);
+      join(stage, pb ^ 1, seg_p + i);
+      gather(was, pb, 1);
+      const bool move = work_any(weigh(pb ^ 1));
+      if (tid == 0) mbar_arrive(&empty[was]);
+      if (move) move_references(pb ^ 1);
+      add_weights();
+      ++done;
     }
-    // ---- the request's denominators, for the adding warps ----
-    if (begun) named_bar_sync(kBarTaken, kThreads);  // they have taken the last request's
-    begun = true;
+    gather(stage, done & 1, 0);
+    gather(stage, done & 1, 1);
+    // ---- the rows' results ----
 #pragma unroll
     for (int r = 0; r < 2; ++r) {
-      const float l = quad_sum(l_sum[r]);
-      if (j == 0) sh.l[warp][g + 8 * r] = l;
-      if (warp == 0 && j == 0) sh.m[g + 8 * r] = m_ref[r];
+      l_sum[r] = quad_sum(l_sum[r]);
+      if (j == 0) sh.red_m[warp][g + 8 * r] = l_sum[r];
 #pragma unroll
       for (int k = 0; k < NG; ++k) {
         const float z = quad_sum(zsum[r][k]);
-        if (j == 0) sh.z[warp][g + 8 * r][k] = z;
+        if (j == 0) sh.red_z[warp][g + 8 * r][k] = z;
       }
     }
-    if (tid == 0)
+    work_sync();
+    if (tid == 0) mbar_arrive(&empty[stage]);
+    ++done;
+    if (++stage == STAGES) stage = 0, ++lap;
+    const bool whole = seg_p == 0 && count == seg_pages;
+    float u = unit[0];
 #pragma unroll
-      for (int k = 0; k < NG; ++k) sh.unit[k] = unit[k];
-    bar_arrive(kBarSums, kThreads);
+    for (int k = 1; k < NG; ++k) u = own == k ? unit[k] : u;
+    const float inv_u = u == 0.f ? 0.f : 1.f / u;
+    // a cut request's partial: slot 0 where the run begins in (or with) this request, else 1
+    const int64_t slot = (static_cast<int64_t>(2 * group + (first ? 0 : 1)) * blocks + block) * kRows;
+#pragma unroll
+    for (int r = 0; r < 2; ++r) {
+      const int row = block * kRows + g + 8 * r;
+      float l = 0.f, z = 0.f;
+      for (int w = 0; w < kWarps; ++w) l += sh.red_m[w][g + 8 * r], z += sh.red_z[w][g + 8 * r][own];
+      const float inv = l == 0.f ? 0.f : inv_u / l;
+      const float lse = l == 0.f ? -INFINITY : (m_ref[r] + log2f(l)) * kLn2;
+      const bool live = row < a.q_len * a.heads;
+      const int t = live ? row / a.heads : 0, h = live ? row % a.heads : 0;
+      uint16_t* out = a.out + seg_b * a.o_sb + t * a.o_st + h * a.o_sh;
+      float* out_part = part.o + (slot + g + 8 * r) * D;
+#pragma unroll
+      for (int c = 0; c < CH; ++c) {
+        const int col = 32 * (warp * CH + c) + 8 * j;
+        float v[8];
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+          for (int k = 0; k < 2; ++k)
+            v[4 * k + i] = fmaf(acc[4 * c + i][2 * r + k], i & 1 ? 1048576.f : 16777216.f, -z) * inv;
+        if (!whole) {
+          reinterpret_cast<float4*>(out_part + col)[0] = make_float4(v[0], v[1], v[2], v[3]);
+          reinterpret_cast<float4*>(out_part + col)[1] = make_float4(v[4], v[5], v[6], v[7]);
+        } else if (live) {
+          *reinterpret_cast<uint4*>(out + col) = make_uint4(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]),
+                                                            pack_bf16x2(v[4], v[5]), pack_bf16x2(v[6], v[7]));
+        }
+      }
+      if (warp == 0 && j == 0) {
+        if (!whole) part.lse[slot + g + 8 * r] = lse;
+        else if (live && a.lse) a.lse[(static_cast<int64_t>(seg_b) * a.q_len + t) * a.heads + h] = lse;
+      }
+    }
+    work_sync();
     ++seg_b;
     seg_p = 0;
   }
-  if (begun) named_bar_sync(kBarTaken, kThreads);
 }
 
 constexpr int kMergeWarps = 8, kMergeThreads = kMergeWarps * 32;
