@@ -11,13 +11,14 @@
 //
 // A CTA holds 16 query rows (query tokens x heads) and walks the pages of one or more requests; a page
 // (64 tokens) is one pipeline stage (TMA, 128-byte swizzle, so that ldmatrix reads without conflicts).
-// The 8 warps form pairs: a pair scores 16 of the page's tokens, each warp of it over half of the latent
-// columns (the query's operand registers would not fit otherwise), and swaps partial scores so that each
-// warp holds 8 tokens' whole ones.  It weighs them against a reference maximum that moves only when a
-// score passes it by 2^10 and writes P s of each group to shared memory.  Each warp adds up D/8 latent
-// columns of the result.  Page i + 1 is scored and page i added up in one iteration, so that the products
-// of the one hide the latencies of the other; the iteration's one CTA-wide barrier also carries the
-// vote on moving the references.  One warp more feeds the stages.
+// The 8 working warps form pairs: a pair scores 16 of a page's tokens, each warp of it over half of the
+// latent columns (the query's operand registers would not fit otherwise), and swaps partial scores, so
+// that a tick later each warp weighs 8 tokens: against a reference maximum that moves only when a score
+// passes it by 2^10, P s of each group going to shared memory.  Another tick later each warp adds D/8
+// latent columns of the page up.  So three pages are under way in a tick, with nothing to wait for between
+// their parts, and one barrier ends it: it publishes the swap and the weights, carries the vote on
+// moving the references, and joins the loading warp, which waits for the next page's arrival before it
+// and refills the stage that became free after it.
 //
 // The pages of all requests are dealt to the CTAs in one equal run each (a run may begin or end inside
 // a request); what is cut is joined by merge_kernel by log-sum-exp.
@@ -36,8 +37,8 @@ constexpr int kWarps = 8, kWorkers = kWarps * 32, kThreads = kWorkers + 128;
 constexpr int kWorkerRegs = 232, kLoaderRegs = 40;
 constexpr int kRows = 16;  // query rows of a CTA
 constexpr int kMinPages = 2;     // least run of pages worth a CTA of its own
-constexpr float kSlack = 10.f;   // log2 of how far a weight may pass its reference
-constexpr float kScaleSlack = 16.f;
+constexpr float kSlack = 1024.f, kScaleSlack = 32.f;  // how far weights and scales may pass their references (P s <= 2^15)
+constexpr float kNoMax = -1e30f, kNoUnit = 1.329227995784916e36f;  // references not yet set: the first token passes them
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
 template <int D, int DR>
@@ -55,18 +56,18 @@ struct Cfg {
 template <int NG>
 struct Shared {
   float4 swap[2][kWarps][32];
-  float red_m[kWarps][kRows], red_s[kWarps][NG], red_z[kWarps][kRows][NG];
+  float red_m[kWarps][kRows], red_s[kWarps][NG], red_l[kWarps][kRows], red_z[kWarps][kRows][NG];
 };
 
-// Named barriers: 1..4 the pairs, 5 all working warps.
-constexpr int kBarPair = 1, kBarWork = 5;
+// Named barriers: the end of a tick (working and loading warps), and the working warps'.
+constexpr int kBarTick = 1, kBarWork = 2;
 __device__ __forceinline__ void work_sync() { named_bar_sync(kBarWork, kWorkers); }
-__device__ __forceinline__ bool work_any(bool vote) {
+__device__ __forceinline__ bool tick(bool vote) {
   int any;
   asm volatile(
       "{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %3, 0;\n\tbar.red.or.pred q, %1, %2, p;\n\tselp.b32 %0, 1, 0, q;\n\t}"
       : "=r"(any)
-      : "n"(kBarWork), "n"(kWorkers), "r"(static_cast<int>(vote))
+      : "n"(kBarTick), "n"(kWorkers + 32), "r"(static_cast<int>(vote))
       : "memory");
   return any != 0;
 }
@@ -104,6 +105,8 @@ __device__ __forceinline__ void mma_bf16(float (&d)[4], const uint32_t (&a)[4], 
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
+// Bytes 1 and 3 as 16-bit halves.
+__device__ __forceinline__ uint32_t odd_bytes(uint32_t w) { return prmt(w, 0u, 0x4341u); }
 __device__ __forceinline__ uint32_t pack_half2(float lo, float hi) {
   const __half2 h = __floats2half2_rn(lo, hi);
   return *reinterpret_cast<const uint32_t*>(&h);
@@ -159,7 +162,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   extern __shared__ char raw[];
   char* smem = reinterpret_cast<char*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
   char* pbuf = smem + STAGES * C::STAGE;
-  __shared__ uint64_t full[STAGES], empty[STAGES];
+  __shared__ uint64_t full[STAGES];
   __shared__ int bad_page[STAGES];
   __shared__ int64_t scan[kThreads / 32];
   __shared__ int start[2];
@@ -174,7 +177,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   int64_t mine = 0, total;
   for (int b = tid * per; b < min(a.batch, (tid + 1) * per); ++b) mine += pages_of(a, b);
   if (tid == 0) {
-    for (int s = 0; s < STAGES; ++s) mbar_init(&full[s], 1), mbar_init(&empty[s], 1);
+    for (int s = 0; s < STAGES; ++s) mbar_init(&full[s], 1);
     fence_mbar_init();
   }
   int64_t before = block_scan<kThreads / 32>(mine, total, scan);
@@ -190,42 +193,61 @@ __global__ void __launch_bounds__(kThreads, 1)
   }
   __syncthreads();
   int seg_b = start[0], seg_p = start[1];
-  bool healthy = true;
-  auto wait_for = [&](uint64_t* bar, int phase) {
-    if (healthy) healthy = mbar_wait(bar, phase & 1, a.err);
-  };
 
   if (warp >= kWarps) {  // ================= the loading warp: stage k holds page k of the run =================
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kLoaderRegs));
-    if (tid != kWorkers) return;
-    prefetch_tensormap(&map_codes);
-    prefetch_tensormap(&map_rope);
+    if (warp > kWarps) return;
     const int pool_pages = static_cast<int>(a.cache.num_slots / kPage);
-    int n = pages_of(a, seg_b), stage = 0, lap = 0;
-    int next = a.page_table[seg_b * a.pt_stride + seg_p];
-    for (int i = 0; i < n_units; ++i) {
+    int load_b = seg_b, load_p = seg_p, load_n = pages_of(a, seg_b), load_stage = 0, loaded = 0, next = 0;
+    auto load = [&]() {
+      if (loaded == n_units) return;
       const int id = next;
-      if (i + 1 < n_units) {  // the next page's id is on its way while this page's stage is awaited
-        if (++seg_p == n) {
-          seg_p = 0;
-          do n = pages_of(a, ++seg_b);
-          while (n == 0);
+      if (++loaded < n_units) {  // the next page's id is on its way until the next call
+        if (++load_p == load_n) {
+          load_p = 0;
+          do load_n = pages_of(a, ++load_b);
+          while (load_n == 0);
         }
-        next = a.page_table[seg_b * a.pt_stride + seg_p];
+        next = a.page_table[load_b * a.pt_stride + load_p];
       }
-      if (lap > 0) wait_for(&empty[stage], lap - 1);
       const bool ok = id >= 0 && id < pool_pages;
       const int page = ok ? id : 0;
-      char* dst = smem + stage * C::STAGE;
-      uint64_t* bar = &full[stage];
-      bad_page[stage] = !ok;
-      if (!ok) report(a.err, ROLAQ_DEV_BAD_PAGE);
-      mbar_expect_tx(bar, C::STAGE);
+      if (lane == 0) {
+        char* dst = smem + load_stage * C::STAGE;
+        uint64_t* bar = &full[load_stage];
+        bad_page[load_stage] = !ok;
+        if (!ok) report(a.err, ROLAQ_DEV_BAD_PAGE);
+        mbar_expect_tx(bar, C::STAGE);
 #pragma unroll
-      for (int k = 0; k < D / 256; ++k) tma_load_2d(dst + k * 8192, &map_codes, bar, k * 128, page * kPage);
-      tma_load_2d(dst + C::CODES, &map_rope, bar, 0, page * kPage);
-      bulk_load(dst + C::CODES + C::ROPE, a.cache.params + static_cast<int64_t>(page) * (kPage * NG * 2), C::PARAMS, bar);
+        for (int k = 0; k < D / 256; ++k) tma_load_2d(dst + k * 8192, &map_codes, bar, k * 128, page * kPage);
+        tma_load_2d(dst + C::CODES, &map_rope, bar, 0, page * kPage);
+        bulk_load(dst + C::CODES + C::ROPE, a.cache.params + static_cast<int64_t>(page) * (kPage * NG * 2), C::PARAMS, bar);
+      }
+      __syncwarp();
+      if (++load_stage == STAGES) load_stage = 0;
+    };
+    next = a.page_table[load_b * a.pt_stride + load_p];
+    for (int i = 0; i < STAGES; ++i) load();
+    int stage = 0, lap = 0, arrived = 0;
+    bool healthy = true;
+    auto await = [&]() {  // the next page of the run; after one that did not come in time the rest is not awaited
+      if (arrived == n_units) return;
+      if (healthy) healthy = mbar_wait(&full[stage], lap & 1, a.err);
+      __syncwarp();
+      ++arrived;
       if (++stage == STAGES) stage = 0, ++lap;
+    };
+    await();
+    tick(false);
+    for (int done = 0; done < n_units; ++seg_b, seg_p = 0) {
+      const int count = min(pages_of(a, seg_b) - seg_p, n_units - done);
+      if (count <= 0) continue;
+      for (int t = 0; t < count + 2; ++t) {
+        if (t + 1 < count || t == count + 1) await();  // the page that the next tick scores
+        tick(false);
+        if (t >= 2) load();  // page t - 2 has been added up
+      }
+      done += count;
     }
     return;
   }
@@ -244,7 +266,8 @@ __global__ void __launch_bounds__(kThreads, 1)
   const uint32_t p_off = own * (kRows * 128) + sw128(lane & 15, lane >> 4);
   const uint32_t p_dst = g * 128 + ((warp ^ g) << 4) + 4 * j;
   const float qk_scale = a.sm_scale * kLog2e;
-  int done = 0, stage = 0, lap = 0;  // pages of the run added up; the stage of page `done`, its phase
+  int done = 0, stage = 0;  // pages of the run; the stage of the page scored next
+  tick(false);              // the first page is there
 
   while (done < n_units) {
     const int seg_pages = pages_of(a, seg_b);
@@ -319,11 +342,11 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
     for (int n = 0; n < 4 * CH; ++n) acc[n][0] = acc[n][1] = acc[n][2] = acc[n][3] = 0.f;
 #pragma unroll
-    for (int k = 0; k < NG; ++k) zsum[0][k] = zsum[1][k] = unit[k] = 0.f;
+    for (int k = 0; k < NG; ++k) zsum[0][k] = zsum[1][k] = 0.f, unit[k] = kNoUnit;
 
-    float s_val[4], s_tok[2][NG], z_tok[2][NG], p_val[4];  // of the warp's 8 tokens of the page being scored
+    float m_use[2] = {kNoMax, kNoMax};  // m_ref, or kNoMax where that is -inf
 
-    // Partial scores of 16 tokens into the pair's swap.
+    // Partial scores of 16 tokens: the warp's own eight in mine_s, the partner's to the swap.
     float mine_s[4];
     auto score = [&](int st_at, int pb) {
       const uint32_t st = stages + st_at * C::STAGE;
@@ -359,8 +382,8 @@ __global__ void __launch_bounds__(kThreads, 1)
           for (int k = 0; k < HG; ++k)
 #pragma unroll
             for (int n = 0; n < 2; ++n) {
-              const uint32_t v = e ? w[n][k][c] >> 8 : w[n][k][c];
-              mma_f16(c_acc[n][k], q[8 * k + 2 * c + e], v & 0x000F000Fu, v & 0x00F000F0u);
+              const uint32_t v = e ? odd_bytes(w[n][k][c]) : w[n][k][c], low = v & 0x000F000Fu;
+              mma_f16(c_acc[n][k], q[8 * k + 2 * c + e], low, e ? v - low : v & 0x00F000F0u);
             }
       float sum[2][4];
       const char* params = smem + st_at * C::STAGE + C::CODES + C::ROPE + half * (HG * 8);
@@ -391,14 +414,14 @@ __global__ void __launch_bounds__(kThreads, 1)
       sh.swap[pb][warp][lane] = make_float4(sum[1][0], sum[1][1], sum[1][2], sum[1][3]);
     };
 
-    // The whole scores of the warp's 8 tokens, in log2 units, and their params.
-    auto join = [&](int st_at, int pb, int p) {
-      named_bar_sync(kBarPair + quarter, 64);
+    // A page's weights.  s_val: the whole scores of the warp's 8 tokens in log2 units.
+    float s_val[4], s_tok[2][NG], z_tok[2][NG], p_val[4];
+    auto join = [&](int st_at, int pb, int p, const float (&own_s)[4]) {
       const float4 theirs = sh.swap[pb][warp ^ 1][lane];
-      s_val[0] = (mine_s[0] + theirs.x) * row_scale[0];
-      s_val[1] = (mine_s[1] + theirs.y) * row_scale[0];
-      s_val[2] = (mine_s[2] + theirs.z) * row_scale[1];
-      s_val[3] = (mine_s[3] + theirs.w) * row_scale[1];
+      s_val[0] = (own_s[0] + theirs.x) * row_scale[0];
+      s_val[1] = (own_s[1] + theirs.y) * row_scale[0];
+      s_val[2] = (own_s[2] + theirs.z) * row_scale[1];
+      s_val[3] = (own_s[3] + theirs.w) * row_scale[1];
       const float4* par = reinterpret_cast<const float4*>(smem + st_at * C::STAGE + C::CODES + C::ROPE) + (8 * warp + 2 * j) * (NG / 2);
 #pragma unroll
       for (int t = 0; t < 2; ++t)
@@ -423,25 +446,22 @@ __global__ void __launch_bounds__(kThreads, 1)
     };
 
     // Weights against the present references, times each group's scale, to shared memory; true where a
-    // score or a scale has left its reference behind.
+    // weight or a scale has left its reference behind (their sums: moving early does no harm), or is NaN.
     auto weigh = [&](int pb) {
-      bool need = false;
 #pragma unroll
-      for (int x = 0; x < 4; ++x) {
-        const float m = m_ref[x >> 1];
-        need |= s_val[x] > m + kSlack;
-        p_val[x] = ex2_approx(s_val[x] - (m == -INFINITY ? 0.f : m));
-      }
+      for (int x = 0; x < 4; ++x) p_val[x] = ex2_approx(s_val[x] - m_use[x >> 1]);
+      float sizes = 0.f;
       char* dst = pbuf + pb * C::PBUF + p_dst;
 #pragma unroll
       for (int k = 0; k < NG; ++k) {
         const float s0 = s_tok[0][k] * unit[k], s1 = s_tok[1][k] * unit[k];
-        need |= fmaxf(fabsf(s0), fabsf(s1)) > kScaleSlack;
+        sizes += fabsf(s0) + fabsf(s1);
 #pragma unroll
         for (int r = 0; r < 2; ++r)
           *reinterpret_cast<uint32_t*>(dst + k * (kRows * 128) + r * 1024) = pack_half2(p_val[2 * r] * s0, p_val[2 * r + 1] * s1);
       }
-      return need;
+      const float weights = (p_val[0] + p_val[1]) + (p_val[2] + p_val[3]);
+      return !(weights <= kSlack) || !(sizes <= kScaleSlack);
     };
 
     // New references: the page's maxima; the sums so far are brought to them.
@@ -464,6 +484,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         for (int w = 0; w < kWarps; ++w) m = fmaxf(m, sh.red_m[w][g + 8 * r]);
         keep[r] = m_ref[r] == m ? 1.f : ex2_approx(m_ref[r] - m);
         m_ref[r] = m;
+        m_use[r] = m == -INFINITY ? kNoMax : m;
         l_sum[r] *= keep[r];
       }
 #pragma unroll
@@ -471,9 +492,9 @@ __global__ void __launch_bounds__(kThreads, 1)
         float s = 0.f;
         for (int w = 0; w < kWarps; ++w) s = fmaxf(s, sh.red_s[w][k]);
         float keep_unit = 1.f;
-        if (s > 0.f && (unit[k] == 0.f || s * unit[k] > kScaleSlack)) {
-          const float u = pow2(min(max(127 - static_cast<int>(__float_as_uint(s) >> 23), -120), 120));
-          if (unit[k] != 0.f) keep_unit = u / unit[k];
+        if (s * unit[k] > 2.f) {  // bring the largest scale into [1, 2)
+          const float u = pow2(min(max(127 - static_cast<int>(__float_as_uint(s) >> 23), -100), 100));
+          keep_unit = u / unit[k];
           unit[k] = u;
         }
         if (k == own) keep_own = keep_unit;
@@ -512,63 +533,76 @@ __global__ void __launch_bounds__(kThreads, 1)
       for (int i = 0; i < 2; ++i)
 #pragma unroll
         for (int c = 0; c < CH; ++c) {
-          const uint32_t u = x[c][2 * i], v = x[c][2 * i + 1], u8 = u >> 8, v8 = v >> 8;
+          // of four elements e: e0, e0 + 16 e1, e2, e2 + 16 e3
+          const uint32_t u = x[c][2 * i], v = x[c][2 * i + 1], u8 = odd_bytes(u), v8 = odd_bytes(v);
           mma_f16(acc[4 * c], pa[i], u & 0x000F000Fu, v & 0x000F000Fu);
-          mma_f16(acc[4 * c + 1], pa[i], u & 0x00F000F0u, v & 0x00F000F0u);
+          mma_f16(acc[4 * c + 1], pa[i], u & 0x00FF00FFu, v & 0x00FF00FFu);
           mma_f16(acc[4 * c + 2], pa[i], u8 & 0x000F000Fu, v8 & 0x000F000Fu);
-          mma_f16(acc[4 * c + 3], pa[i], u8 & 0x00F000F0u, v8 & 0x00F000F0u);
+          mma_f16(acc[4 * c + 3], pa[i], u8, v8);
         }
     };
 
-    // ---- the pages ----
-    wait_for(&full[stage], lap);
-    score(stage, done & 1);
-    join(stage, done & 1, seg_p);
-    if (work_any(weigh(done & 1))) move_references(done & 1);
-    add_weights();
-    for (int i = 1; i < count; ++i) {
-      const int pb = done & 1, was = stage;
-      if (++stage == STAGES) stage = 0, ++lap;
-      wait_for(&full[stage], lap);
-      score(stage, pb ^ 1);
-      gather(was, pb, 0);
-      join(stage, pb ^ 1, seg_p + i);
-      gather(was, pb, 1);
-      const bool move = work_any(weigh(pb ^ 1));
-      if (tid == 0) mbar_arrive(&empty[was]);
+    // ---- the pages: tick t scores page t, weighs page t - 1 and adds page t - 2 up ----
+    auto after = [](int s, int n) { return s + n >= STAGES ? s + n - STAGES : s + n; };
+    score(stage, 0);
+    tick(false);
+    {
+      const float own_s[4] = {mine_s[0], mine_s[1], mine_s[2], mine_s[3]};
+      if (count > 1) score(after(stage, 1), 1);
+      join(stage, 0, seg_p, own_s);
+      if (tick(weigh(0))) move_references(0);
+      add_weights();
+    }
+    for (int t = 2; t < count; ++t) {
+      const float own_s[4] = {mine_s[0], mine_s[1], mine_s[2], mine_s[3]};
+      const int pb = t & 1;
+      score(after(stage, 2), pb);
+      gather(stage, pb, 0);
+      join(after(stage, 1), pb ^ 1, seg_p + t - 1, own_s);
+      gather(stage, pb, 1);
+      const bool move = tick(weigh(pb ^ 1));
       if (move) move_references(pb ^ 1);
       add_weights();
-      ++done;
+      stage = after(stage, 1);
     }
-    gather(stage, done & 1, 0);
-    gather(stage, done & 1, 1);
+    if (count > 1) {
+      const int pb = count & 1;
+      gather(stage, pb, 0);
+      join(after(stage, 1), pb ^ 1, seg_p + count - 1, mine_s);
+      gather(stage, pb, 1);
+      const bool move = tick(weigh(pb ^ 1));
+      if (move) move_references(pb ^ 1);
+      add_weights();
+      stage = after(stage, 1);
+    }
+    gather(stage, (count - 1) & 1, 0);
+    gather(stage, (count - 1) & 1, 1);
+    stage = after(stage, 1);
+    done += count;
     // ---- the rows' results ----
 #pragma unroll
     for (int r = 0; r < 2; ++r) {
       l_sum[r] = quad_sum(l_sum[r]);
-      if (j == 0) sh.red_m[warp][g + 8 * r] = l_sum[r];
+      if (j == 0) sh.red_l[warp][g + 8 * r] = l_sum[r];
 #pragma unroll
       for (int k = 0; k < NG; ++k) {
         const float z = quad_sum(zsum[r][k]);
         if (j == 0) sh.red_z[warp][g + 8 * r][k] = z;
       }
     }
-    work_sync();
-    if (tid == 0) mbar_arrive(&empty[stage]);
-    ++done;
-    if (++stage == STAGES) stage = 0, ++lap;
+    tick(false);
     const bool whole = seg_p == 0 && count == seg_pages;
     float u = unit[0];
 #pragma unroll
     for (int k = 1; k < NG; ++k) u = own == k ? unit[k] : u;
-    const float inv_u = u == 0.f ? 0.f : 1.f / u;
+    const float inv_u = 1.f / u;
     // a cut request's partial: slot 0 where the run begins in (or with) this request, else 1
     const int64_t slot = (static_cast<int64_t>(2 * group + (first ? 0 : 1)) * blocks + block) * kRows;
 #pragma unroll
     for (int r = 0; r < 2; ++r) {
       const int row = block * kRows + g + 8 * r;
       float l = 0.f, z = 0.f;
-      for (int w = 0; w < kWarps; ++w) l += sh.red_m[w][g + 8 * r], z += sh.red_z[w][g + 8 * r][own];
+      for (int w = 0; w < kWarps; ++w) l += sh.red_l[w][g + 8 * r], z += sh.red_z[w][g + 8 * r][own];
       const float inv = l == 0.f ? 0.f : inv_u / l;
       const float lse = l == 0.f ? -INFINITY : (m_ref[r] + log2f(l)) * kLn2;
       const bool live = row < a.q_len * a.heads;
@@ -583,7 +617,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         for (int i = 0; i < 4; ++i)
 #pragma unroll
           for (int k = 0; k < 2; ++k)
-            v[4 * k + i] = fmaf(acc[4 * c + i][2 * r + k], i & 1 ? 1048576.f : 16777216.f, -z) * inv;
+            v[4 * k + i] = fmaf(i & 1 ? acc[4 * c + i][2 * r + k] - acc[4 * c + i - 1][2 * r + k] : acc[4 * c + i][2 * r + k],
+                                i & 1 ? 1048576.f : 16777216.f, -z) * inv;
         if (!whole) {
           reinterpret_cast<float4*>(out_part + col)[0] = make_float4(v[0], v[1], v[2], v[3]);
           reinterpret_cast<float4*>(out_part + col)[1] = make_float4(v[4], v[5], v[6], v[7]);
@@ -597,7 +632,6 @@ __global__ void __launch_bounds__(kThreads, 1)
         else if (live && a.lse) a.lse[(static_cast<int64_t>(seg_b) * a.q_len + t) * a.heads + h] = lse;
       }
     }
-    work_sync();
     ++seg_b;
     seg_p = 0;
   }
