@@ -9,16 +9,18 @@
 // power of two of its row (exact for BF16 within 2^26 of the row's largest element), P s is FP16 (11
 // bits), the rotary part stays BF16; all are m16n8k16 products with FP32 sums.
 //
-// A CTA holds 16 query rows (query tokens x heads) and walks the pages of one or more requests; a page
-// (64 tokens) is one pipeline stage (TMA, 128-byte swizzle, so that ldmatrix reads without conflicts).
+// Codes are the 16-high side of the products, the query rows (query tokens x heads) the 8-wide side: a CTA holds
+// NH tiles of 8 rows (one or two for D = 512, up to five for D = 256, where 40 heads then are one pass) and
+// walks the pages of one or more requests; a page (64 tokens) is one pipeline stage (TMA, 128-byte swizzle,
+// so that ldmatrix reads without conflicts).
 // The 8 working warps form pairs: a pair scores 16 of a page's tokens, each warp of it over half of the
 // latent columns (the query's operand registers would not fit otherwise), and swaps partial scores, so
-// that a tick later each warp weighs 8 tokens: against a reference maximum that moves only when a score
-// passes it by 2^10, P s of each group going to shared memory.  Another tick later each warp adds D/8
+// that a tick later each warp weighs 8 tokens: against a reference maximum that moves only when weights
+// pass it by 2^10, P s of each group going to shared memory.  Another tick later each warp adds D/8
 // latent columns of the page up.  So three pages are under way in a tick, with nothing to wait for between
 // their parts, and one barrier ends it: it publishes the swap and the weights, carries the vote on
-// moving the references, and joins the loading warp, which waits for the next page's arrival before it
-// and refills the stage that became free after it.
+// moving the references, and joins two helping warps: one waits for the next page's arrival before it,
+// one refills the stage that became free after it (either would cost a working warp hundreds of cycles).
 //
 // The pages of all requests are dealt to the CTAs in one equal run each (a run may begin or end inside
 // a request); what is cut is joined by merge_kernel by log-sum-exp.
@@ -31,32 +33,34 @@ namespace rolaq {
 namespace i4 {
 namespace {
 
-// Eight working warps and a warpgroup of which one warp loads.  Of the 168 registers a thread that a block of
-// 384 is launched with, the loaders hand most to the workers: 232 + 232 + 40 = 3 * 168.
+// Eight working warps and a warpgroup of which two warps load.  Of the 168 registers a thread that a block of
+// 384 is launched with, the loaders hand most to the workers: 2 * 224 + 56 = 2 * 232 + 40 = 3 * 168.
 constexpr int kWarps = 8, kWorkers = kWarps * 32, kThreads = kWorkers + 128;
-constexpr int kWorkerRegs = 232, kLoaderRegs = 40;
-constexpr int kRows = 16;  // query rows of a CTA
 constexpr int kMinPages = 2;     // least run of pages worth a CTA of its own
 constexpr float kSlack = 1024.f, kScaleSlack = 32.f;  // how far weights and scales may pass their references (P s <= 2^15)
 constexpr float kNoMax = -1e30f, kNoUnit = 1.329227995784916e36f;  // references not yet set: the first token passes them
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
-template <int D, int DR>
+template <int D, int DR, int NH>
 struct Cfg {
   static constexpr int NG = D / kGroup;             // groups of a token
   static constexpr int CODES = kPage * D / 2, ROPE = kPage * DR * 2, PARAMS = kPage * NG * 8;
   static constexpr int STAGE = CODES + ROPE + PARAMS;
-  static constexpr int STAGES = D == 512 ? 7 : 12;
-  static constexpr int PBUF = NG * kRows * kPage * 2;  // P s of a page: [group][row][token] FP16
+  static constexpr int STAGES = D == 512 ? 7 : DR == 64 ? 10 : 12;
+  static constexpr int PTILE = kPage * 16;          // P s of a page, a group and 8 rows: [token][row] FP16
+  static constexpr int PBUF = NG * NH * PTILE;
   static constexpr int SMEM = 1024 + STAGES * STAGE + 2 * PBUF;
   static constexpr int HG = NG / 2;                 // groups that a warp scores
   static constexpr int CH = D / kWarps / 32;        // 32-column chunks that a warp adds up
+  static constexpr int ROWS = 8 * NH;
+  static constexpr int WORKER_REGS = NH < 4 ? 224 : 232, LOADER_REGS = NH < 4 ? 56 : 40;
 };
 
-template <int NG>
+template <int NG, int NH>
 struct Shared {
-  float4 swap[2][kWarps][32];
-  float red_m[kWarps][kRows], red_s[kWarps][NG], red_l[kWarps][kRows], red_z[kWarps][kRows][NG];
+  float2 swap[2][kWarps][NH][32];
+  float red_m[kWarps][8 * NH], red_s[kWarps][NG], red_l[kWarps][8 * NH], red_z[kWarps][NG][8 * NH];
+  float q_sum[NG][8 * NH], row_scale[8 * NH];
 };
 
 // Named barriers: the end of a tick (working and loading warps), and the working warps'.
@@ -67,7 +71,7 @@ __device__ __forceinline__ bool tick(bool vote) {
   asm volatile(
       "{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %3, 0;\n\tbar.red.or.pred q, %1, %2, p;\n\tselp.b32 %0, 1, 0, q;\n\t}"
       : "=r"(any)
-      : "n"(kBarTick), "n"(kWorkers + 32), "r"(static_cast<int>(vote))
+      : "n"(kBarTick), "n"(kWorkers + 64), "r"(static_cast<int>(vote))
       : "memory");
   return any != 0;
 }
@@ -115,7 +119,7 @@ __device__ __forceinline__ uint32_t pack_half2(float lo, float hi) {
 __device__ __forceinline__ uint32_t sw128(int row, int chunk) { return row * 128 + ((chunk ^ (row & 7)) << 4); }
 __device__ __forceinline__ uint32_t sw64(int row, int chunk) { return row * 64 + ((chunk ^ ((row >> 1) & 3)) << 4); }
 
-// Sum over a warp's quads' four lanes / maximum over them (lanes that share a row).
+// Sum over a quad's four lanes / maximum over them, and over the eight lanes of the same place in their quads.
 __device__ __forceinline__ float quad_sum(float v) {
   v += __shfl_xor_sync(0xFFFFFFFFu, v, 1);
   return v + __shfl_xor_sync(0xFFFFFFFFu, v, 2);
@@ -123,6 +127,17 @@ __device__ __forceinline__ float quad_sum(float v) {
 __device__ __forceinline__ float quad_max(float v) {
   v = fmaxf(v, __shfl_xor_sync(0xFFFFFFFFu, v, 1));
   return fmaxf(v, __shfl_xor_sync(0xFFFFFFFFu, v, 2));
+}
+
+__device__ __forceinline__ float oct_sum(float v) {
+#pragma unroll
+  for (int o = 4; o < 32; o *= 2) v += __shfl_xor_sync(0xFFFFFFFFu, v, o);
+  return v;
+}
+__device__ __forceinline__ float oct_max(float v) {
+#pragma unroll
+  for (int o = 4; o < 32; o *= 2) v = fmaxf(v, __shfl_xor_sync(0xFFFFFFFFu, v, o));
+  return v;
 }
 
 // Exclusive prefix over the CTA's threads of v; the total in `total`.
@@ -148,16 +163,17 @@ __device__ __forceinline__ int64_t block_scan(int64_t v, int64_t& total, int64_t
 }
 
 struct Partials {
-  float* o;    // [2 * groups * row blocks][16][D], normalised
-  float* lse;  // [2 * groups * row blocks][16], natural log
+  float* o;    // [2 * groups * row blocks][rows of a CTA][D], normalised
+  float* lse;  // [2 * groups * row blocks][rows of a CTA], natural log
+  int rows;    // of a CTA
 };
 
-template <int D, int DR>
+template <int D, int DR, int NH>
 __global__ void __launch_bounds__(kThreads, 1)
     decode_kernel(const __grid_constant__ CUtensorMap map_codes, const __grid_constant__ CUtensorMap map_rope,
                   const DecodeArgs a, const Partials part, const int groups, const int blocks) {
-  using C = Cfg<D, DR>;
-  constexpr int NG = C::NG, HG = C::HG, CH = C::CH, STAGES = C::STAGES;
+  using C = Cfg<D, DR, NH>;
+  constexpr int NG = C::NG, HG = C::HG, CH = C::CH, STAGES = C::STAGES, ROWS = C::ROWS;
   constexpr int KR = DR / 32;  // 16-column steps of the rotary part that a warp scores
   extern __shared__ char raw[];
   char* smem = reinterpret_cast<char*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
@@ -166,7 +182,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   __shared__ int bad_page[STAGES];
   __shared__ int64_t scan[kThreads / 32];
   __shared__ int start[2];
-  __shared__ Shared<NG> sh;
+  __shared__ Shared<NG, NH> sh;
 
   const int tid = threadIdx.x, warp = tid / 32, lane = tid & 31, g = lane >> 2, j = lane & 3;
   const int block = blockIdx.x % blocks, group = blockIdx.x / blocks;
@@ -194,40 +210,48 @@ __global__ void __launch_bounds__(kThreads, 1)
   __syncthreads();
   int seg_b = start[0], seg_p = start[1];
 
-  if (warp >= kWarps) {  // ================= the loading warp: stage k holds page k of the run =================
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kLoaderRegs));
-    if (warp > kWarps) return;
+  if (warp >= kWarps) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(C::LOADER_REGS));
+    if (warp > kWarps + 1) return;
+    const bool loader = warp == kWarps;
+    // ================= the loading warp: stage k holds page k of the run =================
+    // Lane l holds the id of page `base` + l of the run; the next 32 are requested 32 pages ahead of their use.
     const int pool_pages = static_cast<int>(a.cache.num_slots / kPage);
-    int load_b = seg_b, load_p = seg_p, load_n = pages_of(a, seg_b), load_stage = 0, loaded = 0, next = 0;
+    int id_b = seg_b, id_p = seg_p + lane, ids = -1, next_ids = -1, loaded = 0, load_stage = 0;
+    auto fetch_ids = [&](int first) {
+      int id = -1;
+      if (first + lane < n_units) {
+        for (int n; id_p >= (n = pages_of(a, id_b)); ++id_b) id_p -= n;
+        id = a.page_table[id_b * a.pt_stride + id_p];
+      }
+      id_p += 32;
+      return id;
+    };
     auto load = [&]() {
       if (loaded == n_units) return;
-      const int id = next;
-      if (++loaded < n_units) {  // the next page's id is on its way until the next call
-        if (++load_p == load_n) {
-          load_p = 0;
-          do load_n = pages_of(a, ++load_b);
-          while (load_n == 0);
-        }
-        next = a.page_table[load_b * a.pt_stride + load_p];
+      if ((loaded & 31) == 0) {
+        ids = next_ids;
+        next_ids = fetch_ids(loaded + 32);
       }
+      const int id = __shfl_sync(0xFFFFFFFFu, ids, loaded & 31);
+      ++loaded;
       const bool ok = id >= 0 && id < pool_pages;
       const int page = ok ? id : 0;
       if (lane == 0) {
         char* dst = smem + load_stage * C::STAGE;
         uint64_t* bar = &full[load_stage];
         bad_page[load_stage] = !ok;
-        if (!ok) report(a.err, ROLAQ_DEV_BAD_PAGE);
         mbar_expect_tx(bar, C::STAGE);
 #pragma unroll
         for (int k = 0; k < D / 256; ++k) tma_load_2d(dst + k * 8192, &map_codes, bar, k * 128, page * kPage);
         tma_load_2d(dst + C::CODES, &map_rope, bar, 0, page * kPage);
         bulk_load(dst + C::CODES + C::ROPE, a.cache.params + static_cast<int64_t>(page) * (kPage * NG * 2), C::PARAMS, bar);
+        if (!ok) report(a.err, ROLAQ_DEV_BAD_PAGE);
       }
       __syncwarp();
       if (++load_stage == STAGES) load_stage = 0;
     };
-    next = a.page_table[load_b * a.pt_stride + load_p];
-    for (int i = 0; i < STAGES; ++i) load();
+    // ================= the awaiting warp =================
     int stage = 0, lap = 0, arrived = 0;
     bool healthy = true;
     auto await = [&]() {  // the next page of the run; after one that did not come in time the rest is not awaited
@@ -237,35 +261,40 @@ __global__ void __launch_bounds__(kThreads, 1)
       ++arrived;
       if (++stage == STAGES) stage = 0, ++lap;
     };
-    await();
+    if (loader) {
+      next_ids = fetch_ids(0);
+      for (int i = 0; i < STAGES; ++i) load();
+    } else {
+      await();
+    }
     tick(false);
     for (int done = 0; done < n_units; ++seg_b, seg_p = 0) {
       const int count = min(pages_of(a, seg_b) - seg_p, n_units - done);
       if (count <= 0) continue;
       for (int t = 0; t < count + 2; ++t) {
-        if (t + 1 < count || t == count + 1) await();  // the page that the next tick scores
+        if (!loader && (t + 1 < count || t == count + 1)) await();  // the page that the next tick scores
         tick(false);
-        if (t >= 2) load();  // page t - 2 has been added up
+        if (loader && t >= 2) load();  // page t - 2 has been added up
       }
       done += count;
     }
     return;
   }
 
-  asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kWorkerRegs));
+  asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(C::WORKER_REGS));
   const int half = warp & 1, quarter = warp >> 1;  // half of the latent columns, 16 of the page's tokens
   const int own = warp * NG / kWarps;              // the group of the columns that the warp adds up
   // Offsets of the lane's ldmatrix rows from a 1024-byte boundary.  Chunk c of a row lies at c ^ row % 8, so
-  // chunk c ^ x is at the address ^ 16 x.
+  // chunk c ^ x is at the address ^ 16 x.  Of the pair's 16 tokens the warp's own eight come first.
   const uint32_t stages = smem_u32(smem), pbufs = smem_u32(pbuf);
-  const int tok_row = 16 * quarter + 8 * half + (lane & 7);  // tile 0: the warp's own tokens; tile 1: row ^ 8
-  const uint32_t code_off = D == 512 ? half * 8192 + sw128(tok_row, lane >> 3) : sw128(tok_row, 4 * half + (lane >> 3));
-  const uint32_t rope_off = C::CODES + (DR == 64 ? sw128(tok_row, 4 * half + (lane >> 3))
-                                                 : sw64(tok_row ^ ((lane >> 4) * 8), 2 * half + ((lane >> 3) & 1)));
+  const int tok_row = 16 * quarter + ((8 * half + (lane & 15)) & 15);
+  const uint32_t code_off = D == 512 ? half * 8192 + sw128(tok_row, lane >> 4) : sw128(tok_row, 4 * half + (lane >> 4));
+  const uint32_t rope_off = C::CODES + (DR == 64 ? sw128(tok_row, 4 * half + (lane >> 4)) : sw64(tok_row, 2 * half + (lane >> 4)));
   const uint32_t add_off = (warp * CH / 8) * 8192 + sw128(lane, (warp * CH) & 7);
-  const uint32_t p_off = own * (kRows * 128) + sw128(lane & 15, lane >> 4);
-  const uint32_t p_dst = g * 128 + ((warp ^ g) << 4) + 4 * j;
+  const uint32_t p_off = own * (NH * C::PTILE) + lane * 16;
+  const uint32_t p_dst = (8 * warp + g) * 16 + 4 * j;
   const float qk_scale = a.sm_scale * kLog2e;
+  const int rows = a.q_len * a.heads, row0 = block * ROWS;
   int done = 0, stage = 0;  // pages of the run; the stage of the page scored next
   tick(false);              // the first page is there
 
@@ -281,16 +310,13 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (tid == 0 && len != a.seq_lens[seg_b]) report(a.err, ROLAQ_DEV_BAD_REQ);
     const int lim_min = len - a.q_len + 1;
 
-    // ---- the query: rows g and g + 8, this warp's columns ----
-    uint32_t q[8 * HG][4], q_pe[KR][4];
-    float q_sum[2][HG], row_scale[2];
-    int lim[2];
+    // ---- the query: row g of each tile, this warp's columns ----
+    uint32_t q[NH][8 * HG][2], q_pe[NH][KR][2];
 #pragma unroll
-    for (int r = 0; r < 2; ++r) {
-      const int row = block * kRows + g + 8 * r;
-      const bool live = row < a.q_len * a.heads;
+    for (int n = 0; n < NH; ++n) {
+      const int row = row0 + 8 * n + g;
+      const bool live = row < rows;
       const int t = live ? row / a.heads : 0, h = live ? row % a.heads : 0;
-      lim[r] = live ? lim_min + t : 0;
       const uint16_t* src = a.q + seg_b * a.q_sb + t * a.q_st + h * a.q_sh;
       float top = 0.f, odd = 0.f;
       uint4 raw_q[D / 32];  // the whole row: both halves scale it alike
@@ -309,24 +335,29 @@ __global__ void __launch_bounds__(kThreads, 1)
       // 2^k with top 2^k in [2^13, 2^14)
       const int k = min(max(13 - (static_cast<int>(__float_as_uint(top) >> 23) - 127), -100), 100);
       const float up = top > 0.f ? pow2(k) : 1.f;
-      row_scale[r] = odd != 0.f ? __int_as_float(0x7FC00000) : qk_scale * (16777216.f / up);
+      if (warp == 0 && j == 0)
+        sh.row_scale[8 * n + g] = odd != 0.f ? __int_as_float(0x7FC00000) : qk_scale * (16777216.f / up);
+      float sum[HG];
 #pragma unroll
       for (int c = 0; c < 4 * HG; ++c) {
         const uint4 pick = half ? raw_q[4 * HG + c] : raw_q[c];
         const uint32_t v[4] = {pick.x, pick.y, pick.z, pick.w};
-        float x[8], sum = 0.f;
+        float x[8];
+        if (c % 4 == 0) sum[c / 4] = 0.f;
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           x[2 * e] = bf16_lo(v[e]) * up, x[2 * e + 1] = bf16_hi(v[e]) * up;
-          sum += x[2 * e] + x[2 * e + 1];
+          sum[c / 4] += x[2 * e] + x[2 * e + 1];
         }
         // a word of codes gives elements (0, 4), 16 (1, 5), (2, 6) and 16 (3, 7)
-        q[2 * c][r] = pack_half2(x[0], x[4]), q[2 * c][r + 2] = pack_half2(x[1] * 0.0625f, x[5] * 0.0625f);
-        q[2 * c + 1][r] = pack_half2(x[2], x[6]), q[2 * c + 1][r + 2] = pack_half2(x[3] * 0.0625f, x[7] * 0.0625f);
-        q_sum[r][c / 4] = (c % 4 == 0 ? 0.f : q_sum[r][c / 4]) + sum;
+        q[n][2 * c][0] = pack_half2(x[0], x[4]), q[n][2 * c][1] = pack_half2(x[1] * 0.0625f, x[5] * 0.0625f);
+        q[n][2 * c + 1][0] = pack_half2(x[2], x[6]), q[n][2 * c + 1][1] = pack_half2(x[3] * 0.0625f, x[7] * 0.0625f);
       }
 #pragma unroll
-      for (int i = 0; i < HG; ++i) q_sum[r][i] = quad_sum(q_sum[r][i]) * (1.f / 16777216.f);
+      for (int i = 0; i < HG; ++i) {
+        sum[i] = quad_sum(sum[i]) * (1.f / 16777216.f);
+        if (quarter == 0 && j == 0) sh.q_sum[half * HG + i][8 * n + g] = sum[i];
+      }
       // the rotary part under the same power of two (exact), so that both parts add up
       const float down = up * (1.f / 16777216.f);
 #pragma unroll
@@ -334,228 +365,263 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
           const uint32_t v = live ? *reinterpret_cast<const uint32_t*>(src + D + 16 * (half * KR + c) + 8 * e + 2 * j) : 0;
-          q_pe[c][r + 2 * e] = pack_bf16x2(bf16_lo(v) * down, bf16_hi(v) * down);
+          q_pe[n][c][e] = pack_bf16x2(bf16_lo(v) * down, bf16_hi(v) * down);
         }
     }
-
-    float acc[4 * CH][4], zsum[2][NG], unit[NG], l_sum[2] = {0.f, 0.f}, m_ref[2] = {-INFINITY, -INFINITY};
+    work_sync();
+    // the rows' factors: held where few, read again each page where many
+    float2 held_sum[NH <= 2 ? HG : 1][NH <= 2 ? NH : 1], held_scale[NH <= 2 ? NH : 1];
+    auto q_sum_of = [&](int k, int n) { return *reinterpret_cast<const float2*>(&sh.q_sum[half * HG + k][8 * n + 2 * j]); };
+    auto scale_of = [&](int n) { return *reinterpret_cast<const float2*>(&sh.row_scale[8 * n + 2 * j]); };
+    if constexpr (NH <= 2) {
 #pragma unroll
-    for (int n = 0; n < 4 * CH; ++n) acc[n][0] = acc[n][1] = acc[n][2] = acc[n][3] = 0.f;
+      for (int n = 0; n < NH; ++n) {
+        held_scale[n] = scale_of(n);
 #pragma unroll
-    for (int k = 0; k < NG; ++k) zsum[0][k] = zsum[1][k] = 0.f, unit[k] = kNoUnit;
+        for (int k = 0; k < HG; ++k) held_sum[k][n] = q_sum_of(k, n);
+      }
+    }
 
-    float m_use[2] = {kNoMax, kNoMax};  // m_ref, or kNoMax where that is -inf
+    // accumulators: tile 2 c + h of chunk c holds columns 4 g + 2 h (and that + 16 times the next one) x rows 2 j, + 1
+    float acc[2 * CH][NH][4], zsum[NH][2][NG], unit[NG], l_sum[NH][2], m_use[NH][2];
+#pragma unroll
+    for (int n = 0; n < NH; ++n) {
+#pragma unroll
+      for (int c = 0; c < 2 * CH; ++c) acc[c][n][0] = acc[c][n][1] = acc[c][n][2] = acc[c][n][3] = 0.f;
+#pragma unroll
+      for (int x = 0; x < 2; ++x) {
+        l_sum[n][x] = 0.f, m_use[n][x] = kNoMax;
+#pragma unroll
+        for (int k = 0; k < NG; ++k) zsum[n][x][k] = 0.f;
+      }
+    }
+#pragma unroll
+    for (int k = 0; k < NG; ++k) unit[k] = kNoUnit;
 
-    // Partial scores of 16 tokens: the warp's own eight in mine_s, the partner's to the swap.
-    float mine_s[4];
+    // Partial scores of the pair's 16 tokens: the warp's own eight in mine_s, the partner's to the swap.
+    float mine_s[NH][2];
     auto score = [&](int st_at, int pb) {
       const uint32_t st = stages + st_at * C::STAGE;
-      float c_acc[2][HG][4], r_acc[2][4];
-      uint32_t w[2][HG][4], w_pe[2][4];
+      float c_acc[HG][NH][4], r_acc[NH][4];
+      uint32_t w[HG][2][4], w_pe[KR][4];
 #pragma unroll
-      for (int n = 0; n < 2; ++n) {
+      for (int k = 0; k < HG; ++k)
 #pragma unroll
-        for (int k = 0; k < HG; ++k) ldsm_x4((st + (code_off ^ (n << 10))) ^ (k << 6), w[n][k]);
-        if (DR == 64) ldsm_x4(st + (rope_off ^ (n << 10)), w_pe[n]);
+        for (int i = 0; i < 2; ++i) ldsm_x4((st + code_off) ^ (k << 6) ^ (i << 5), w[k][i]);
+#pragma unroll
+      for (int c = 0; c < KR; ++c) ldsm_x4((st + rope_off) ^ (c << 5), w_pe[c]);
+#pragma unroll
+      for (int n = 0; n < NH; ++n)
 #pragma unroll
         for (int x = 0; x < 4; ++x) {
           r_acc[n][x] = 0.f;
 #pragma unroll
-          for (int k = 0; k < HG; ++k) c_acc[n][k][x] = 0.f;
+          for (int k = 0; k < HG; ++k) c_acc[k][n][x] = 0.f;
         }
-      }
-      if (DR == 32) {  // both tiles' two chunks at once
-        uint32_t both[4];
-        ldsm_x4(st + rope_off, both);
-        w_pe[0][0] = both[0], w_pe[0][1] = both[1], w_pe[1][0] = both[2], w_pe[1][1] = both[3];
-      }
       // the accumulators in turn, so that no product waits for the one before it
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int c = 0; c < 2; ++c)
+#pragma unroll
+          for (int e = 0; e < 2; ++e)
+#pragma unroll
+            for (int k = 0; k < HG; ++k) {
+              const uint32_t lo = e ? odd_bytes(w[k][i][2 * c]) : w[k][i][2 * c], hi = e ? odd_bytes(w[k][i][2 * c + 1]) : w[k][i][2 * c + 1];
+              const uint32_t lo0 = lo & 0x000F000Fu, hi0 = hi & 0x000F000Fu;
+              const uint32_t codes[4] = {lo0, hi0, e ? lo - lo0 : lo & 0x00F000F0u, e ? hi - hi0 : hi & 0x00F000F0u};
+#pragma unroll
+              for (int n = 0; n < NH; ++n) mma_f16(c_acc[k][n], codes, q[n][8 * k + 4 * i + 2 * c + e][0], q[n][8 * k + 4 * i + 2 * c + e][1]);
+            }
 #pragma unroll
       for (int c = 0; c < KR; ++c)
 #pragma unroll
-        for (int n = 0; n < 2; ++n) mma_bf16(r_acc[n], q_pe[c], w_pe[n][2 * c], w_pe[n][2 * c + 1]);
+        for (int n = 0; n < NH; ++n) mma_bf16(r_acc[n], w_pe[c], q_pe[n][c][0], q_pe[n][c][1]);
+      // tokens g (own) and g + 8 (the partner's)
+      float s[2][HG], z[2][HG];
 #pragma unroll
-      for (int c = 0; c < 4; ++c)
-#pragma unroll
-        for (int e = 0; e < 2; ++e)
-#pragma unroll
-          for (int k = 0; k < HG; ++k)
-#pragma unroll
-            for (int n = 0; n < 2; ++n) {
-              const uint32_t v = e ? odd_bytes(w[n][k][c]) : w[n][k][c], low = v & 0x000F000Fu;
-              mma_f16(c_acc[n][k], q[8 * k + 2 * c + e], low, e ? v - low : v & 0x00F000F0u);
-            }
-      float sum[2][4];
-      const char* params = smem + st_at * C::STAGE + C::CODES + C::ROPE + half * (HG * 8);
-#pragma unroll
-      for (int n = 0; n < 2; ++n) {
-        const float* par = reinterpret_cast<const float*>(params) + ((8 * warp) ^ (8 * n)) * (NG * 2) + 2 * j * (NG * 2);
-        float s[2][HG], z[2][HG];
-#pragma unroll
-        for (int t = 0; t < 2; ++t) {
-          if constexpr (HG == 2) {
-            const float4 v = *reinterpret_cast<const float4*>(par + t * (NG * 2));
-            s[t][0] = v.x, z[t][0] = v.y, s[t][1] = v.z, z[t][1] = v.w;
-          } else {
-            const float2 v = *reinterpret_cast<const float2*>(par + t * (NG * 2));
-            s[t][0] = v.x, z[t][0] = v.y;
-          }
-        }
-#pragma unroll
-        for (int x = 0; x < 4; ++x) {
-          sum[n][x] = r_acc[n][x];
-#pragma unroll
-          for (int k = 0; k < HG; ++k)
-            sum[n][x] = fmaf(s[x & 1][k], fmaf(-z[x & 1][k], q_sum[x >> 1][k], c_acc[n][k][x]), sum[n][x]);
+      for (int t = 0; t < 2; ++t) {
+        const char* par = smem + st_at * C::STAGE + C::CODES + C::ROPE + ((8 * (warp ^ t)) + g) * (NG * 8) + half * (HG * 8);
+        if constexpr (HG == 2) {
+          const float4 v = *reinterpret_cast<const float4*>(par);
+          s[t][0] = v.x, z[t][0] = v.y, s[t][1] = v.z, z[t][1] = v.w;
+        } else {
+          const float2 v = *reinterpret_cast<const float2*>(par);
+          s[t][0] = v.x, z[t][0] = v.y;
         }
       }
 #pragma unroll
-      for (int x = 0; x < 4; ++x) mine_s[x] = sum[0][x];
-      sh.swap[pb][warp][lane] = make_float4(sum[1][0], sum[1][1], sum[1][2], sum[1][3]);
+      for (int n = 0; n < NH; ++n) {
+        float sum[4] = {r_acc[n][0], r_acc[n][1], r_acc[n][2], r_acc[n][3]};
+#pragma unroll
+        for (int k = 0; k < HG; ++k) {
+          float2 qs;
+          if constexpr (NH <= 2) qs = held_sum[k][n];
+          else qs = q_sum_of(k, n);
+#pragma unroll
+          for (int x = 0; x < 4; ++x)
+            sum[x] = fmaf(s[x >> 1][k], fmaf(-z[x >> 1][k], x & 1 ? qs.y : qs.x, c_acc[k][n][x]), sum[x]);
+        }
+        mine_s[n][0] = sum[0], mine_s[n][1] = sum[1];
+        sh.swap[pb][warp][n][lane] = make_float2(sum[2], sum[3]);
+      }
     };
 
-    // A page's weights.  s_val: the whole scores of the warp's 8 tokens in log2 units.
-    float s_val[4], s_tok[2][NG], z_tok[2][NG], p_val[4];
-    auto join = [&](int st_at, int pb, int p, const float (&own_s)[4]) {
-      const float4 theirs = sh.swap[pb][warp ^ 1][lane];
-      s_val[0] = (own_s[0] + theirs.x) * row_scale[0];
-      s_val[1] = (own_s[1] + theirs.y) * row_scale[0];
-      s_val[2] = (own_s[2] + theirs.z) * row_scale[1];
-      s_val[3] = (own_s[3] + theirs.w) * row_scale[1];
-      const float4* par = reinterpret_cast<const float4*>(smem + st_at * C::STAGE + C::CODES + C::ROPE) + (8 * warp + 2 * j) * (NG / 2);
+    // A page's weights.  s_val: the whole scores of the warp's 8 tokens (the thread's: token g) in log2 units.
+    float s_val[NH][2], s_tok[NG], z_tok[NG], p_val[NH][2];
+    auto join = [&](int st_at, int pb, int p, const float (&own_s)[NH][2]) {
 #pragma unroll
-      for (int t = 0; t < 2; ++t)
+      for (int n = 0; n < NH; ++n) {
+        const float2 theirs = sh.swap[pb][warp ^ 1][n][lane];
+        float2 scale;
+        if constexpr (NH <= 2) scale = held_scale[n];
+        else scale = scale_of(n);
+        s_val[n][0] = (own_s[n][0] + theirs.x) * scale.x;
+        s_val[n][1] = (own_s[n][1] + theirs.y) * scale.y;
+      }
+      const float4* par = reinterpret_cast<const float4*>(smem + st_at * C::STAGE + C::CODES + C::ROPE) + (8 * warp + g) * (NG / 2);
 #pragma unroll
-        for (int k = 0; k < NG; k += 2) {
-          const float4 v = par[t * (NG / 2) + k / 2];
-          s_tok[t][k] = v.x, z_tok[t][k] = v.y, s_tok[t][k + 1] = v.z, z_tok[t][k + 1] = v.w;
-        }
+      for (int k = 0; k < NG; k += 2) {
+        const float4 v = par[k / 2];
+        s_tok[k] = v.x, z_tok[k] = v.y, s_tok[k + 1] = v.z, z_tok[k + 1] = v.w;
+      }
       const int bad = bad_page[st_at];
       if ((p + 1) * kPage > lim_min || bad) {  // the request's end, or a page that is not there
-        const int tok = p * kPage + 8 * warp + 2 * j;
+        const int tok = p * kPage + 8 * warp + g;
+        if (tok >= len || bad)
 #pragma unroll
-        for (int t = 0; t < 2; ++t) {
-          if (tok + t >= len || bad)
+          for (int k = 0; k < NG; ++k) s_tok[k] = z_tok[k] = 0.f;
 #pragma unroll
-            for (int k = 0; k < NG; ++k) s_tok[t][k] = z_tok[t][k] = 0.f;
+        for (int n = 0; n < NH; ++n)
 #pragma unroll
-          for (int r = 0; r < 2; ++r)
-            if (tok + t >= lim[r] || bad) s_val[2 * r + t] = -INFINITY;
-        }
+          for (int x = 0; x < 2; ++x)
+            if (bad || tok >= lim_min + (row0 + 8 * n + 2 * j + x) / a.heads) s_val[n][x] = -INFINITY;
       }
     };
 
     // Weights against the present references, times each group's scale, to shared memory; true where a
     // weight or a scale has left its reference behind (their sums: moving early does no harm), or is NaN.
     auto weigh = [&](int pb) {
+      float weights = 0.f, sizes = 0.f;
 #pragma unroll
-      for (int x = 0; x < 4; ++x) p_val[x] = ex2_approx(s_val[x] - m_use[x >> 1]);
-      float sizes = 0.f;
+      for (int n = 0; n < NH; ++n) {
+        p_val[n][0] = ex2_approx(s_val[n][0] - m_use[n][0]);
+        p_val[n][1] = ex2_approx(s_val[n][1] - m_use[n][1]);
+        weights += p_val[n][0] + p_val[n][1];
+      }
       char* dst = pbuf + pb * C::PBUF + p_dst;
 #pragma unroll
       for (int k = 0; k < NG; ++k) {
-        const float s0 = s_tok[0][k] * unit[k], s1 = s_tok[1][k] * unit[k];
-        sizes += fabsf(s0) + fabsf(s1);
+        const float s = s_tok[k] * unit[k];
+        sizes += fabsf(s);
 #pragma unroll
-        for (int r = 0; r < 2; ++r)
-          *reinterpret_cast<uint32_t*>(dst + k * (kRows * 128) + r * 1024) = pack_half2(p_val[2 * r] * s0, p_val[2 * r + 1] * s1);
+        for (int n = 0; n < NH; ++n)
+          *reinterpret_cast<uint32_t*>(dst + (k * NH + n) * C::PTILE) = pack_half2(p_val[n][0] * s, p_val[n][1] * s);
       }
-      const float weights = (p_val[0] + p_val[1]) + (p_val[2] + p_val[3]);
       return !(weights <= kSlack) || !(sizes <= kScaleSlack);
     };
 
     // New references: the page's maxima; the sums so far are brought to them.
     auto move_references = [&](int pb) {
 #pragma unroll
-      for (int r = 0; r < 2; ++r) {
-        const float m = quad_max(fmaxf(s_val[2 * r], s_val[2 * r + 1]));
-        if (j == 0) sh.red_m[warp][g + 8 * r] = m;
-      }
+      for (int n = 0; n < NH; ++n)
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+          const float m = oct_max(s_val[n][x]);
+          if (g == 0) sh.red_m[warp][8 * n + 2 * j + x] = m;
+        }
 #pragma unroll
       for (int k = 0; k < NG; ++k) {
-        const float s = quad_max(fmaxf(fabsf(s_tok[0][k]), fabsf(s_tok[1][k])));
+        const float s = oct_max(fabsf(s_tok[k]));
         if (lane == 0) sh.red_s[warp][k] = s;
       }
       work_sync();
-      float keep[2], keep_own = 1.f;
-#pragma unroll
-      for (int r = 0; r < 2; ++r) {
-        float m = m_ref[r];
-        for (int w = 0; w < kWarps; ++w) m = fmaxf(m, sh.red_m[w][g + 8 * r]);
-        keep[r] = m_ref[r] == m ? 1.f : ex2_approx(m_ref[r] - m);
-        m_ref[r] = m;
-        m_use[r] = m == -INFINITY ? kNoMax : m;
-        l_sum[r] *= keep[r];
-      }
+      float keep_unit[NG], keep_own = 1.f;
 #pragma unroll
       for (int k = 0; k < NG; ++k) {
         float s = 0.f;
         for (int w = 0; w < kWarps; ++w) s = fmaxf(s, sh.red_s[w][k]);
-        float keep_unit = 1.f;
+        keep_unit[k] = 1.f;
         if (s * unit[k] > 2.f) {  // bring the largest scale into [1, 2)
           const float u = pow2(min(max(127 - static_cast<int>(__float_as_uint(s) >> 23), -100), 100));
-          keep_unit = u / unit[k];
+          keep_unit[k] = u / unit[k];
           unit[k] = u;
         }
-        if (k == own) keep_own = keep_unit;
-        zsum[0][k] *= keep[0] * keep_unit;
-        zsum[1][k] *= keep[1] * keep_unit;
+        if (k == own) keep_own = keep_unit[k];
       }
 #pragma unroll
-      for (int n = 0; n < 4 * CH; ++n)
+      for (int n = 0; n < NH; ++n)
 #pragma unroll
-        for (int x = 0; x < 4; ++x) acc[n][x] *= keep[x >> 1] * keep_own;
+        for (int x = 0; x < 2; ++x) {
+          float m = m_use[n][x];
+          for (int w = 0; w < kWarps; ++w) m = fmaxf(m, sh.red_m[w][8 * n + 2 * j + x]);
+          const float keep = ex2_approx(m_use[n][x] - m);
+          m_use[n][x] = m;
+          l_sum[n][x] *= keep;
+#pragma unroll
+          for (int k = 0; k < NG; ++k) zsum[n][x][k] *= keep * keep_unit[k];
+#pragma unroll
+          for (int c = 0; c < 2 * CH; ++c) acc[c][n][x] *= keep * keep_own, acc[c][n][x + 2] *= keep * keep_own;
+        }
       weigh(pb);
       work_sync();
     };
 
     // After the references stand: the denominators and the zeros' share.
     auto add_weights = [&]() {
-      l_sum[0] += p_val[0] + p_val[1];
-      l_sum[1] += p_val[2] + p_val[3];
+#pragma unroll
+      for (int n = 0; n < NH; ++n) l_sum[n][0] += p_val[n][0], l_sum[n][1] += p_val[n][1];
 #pragma unroll
       for (int k = 0; k < NG; ++k) {
-        const float a0 = s_tok[0][k] * unit[k] * z_tok[0][k], a1 = s_tok[1][k] * unit[k] * z_tok[1][k];
-        zsum[0][k] = fmaf(p_val[0], a0, fmaf(p_val[1], a1, zsum[0][k]));
-        zsum[1][k] = fmaf(p_val[2], a0, fmaf(p_val[3], a1, zsum[1][k]));
+        const float f = s_tok[k] * unit[k] * z_tok[k];
+#pragma unroll
+        for (int n = 0; n < NH; ++n)
+          zsum[n][0][k] = fmaf(p_val[n][0], f, zsum[n][0][k]), zsum[n][1][k] = fmaf(p_val[n][1], f, zsum[n][1][k]);
       }
     };
 
-    // acc += (P s) c over tokens 32 h .. 32 h + 31 of a page, the warp's columns.
+    // acc += c^T (P s) over tokens 32 h .. 32 h + 31 of a page, the warp's columns.
     auto gather = [&](int st_at, int pb, int h) {
       const uint32_t st = stages + st_at * C::STAGE + add_off, ps = pbufs + pb * C::PBUF + p_off;
-      uint32_t pa[2][4], x[CH][4];
-#pragma unroll
-      for (int i = 0; i < 2; ++i) ldsm_x4(ps ^ ((2 * h + i) << 5), pa[i]);
+      uint32_t pb_[NH][4], x[CH][4];
 #pragma unroll
       for (int c = 0; c < CH; ++c) ldsm_x4_t((st + h * 4096) ^ (c << 4), x[c]);
+#pragma unroll
+      for (int n = 0; n < NH; ++n) ldsm_x4_t(ps + n * C::PTILE + h * 512, pb_[n]);
 #pragma unroll
       for (int i = 0; i < 2; ++i)
 #pragma unroll
         for (int c = 0; c < CH; ++c) {
-          // of four elements e: e0, e0 + 16 e1, e2, e2 + 16 e3
+          // of four elements e: e0 over e0 + 16 e1, e2 over e2 + 16 e3
           const uint32_t u = x[c][2 * i], v = x[c][2 * i + 1], u8 = odd_bytes(u), v8 = odd_bytes(v);
-          mma_f16(acc[4 * c], pa[i], u & 0x000F000Fu, v & 0x000F000Fu);
-          mma_f16(acc[4 * c + 1], pa[i], u & 0x00FF00FFu, v & 0x00FF00FFu);
-          mma_f16(acc[4 * c + 2], pa[i], u8 & 0x000F000Fu, v8 & 0x000F000Fu);
-          mma_f16(acc[4 * c + 3], pa[i], u8, v8);
+          const uint32_t even[4] = {u & 0x000F000Fu, u & 0x00FF00FFu, v & 0x000F000Fu, v & 0x00FF00FFu};
+          const uint32_t odd[4] = {u8 & 0x000F000Fu, u8, v8 & 0x000F000Fu, v8};
+#pragma unroll
+          for (int n = 0; n < NH; ++n) mma_f16(acc[2 * c][n], even, pb_[n][2 * i], pb_[n][2 * i + 1]);
+#pragma unroll
+          for (int n = 0; n < NH; ++n) mma_f16(acc[2 * c + 1][n], odd, pb_[n][2 * i], pb_[n][2 * i + 1]);
         }
     };
 
     // ---- the pages: tick t scores page t, weighs page t - 1 and adds page t - 2 up ----
     auto after = [](int s, int n) { return s + n >= STAGES ? s + n - STAGES : s + n; };
+    float own_s[NH][2];
+    auto hand_over = [&]() {
+#pragma unroll
+      for (int n = 0; n < NH; ++n) own_s[n][0] = mine_s[n][0], own_s[n][1] = mine_s[n][1];
+    };
     score(stage, 0);
     tick(false);
     {
-      const float own_s[4] = {mine_s[0], mine_s[1], mine_s[2], mine_s[3]};
+      hand_over();
       if (count > 1) score(after(stage, 1), 1);
       join(stage, 0, seg_p, own_s);
       if (tick(weigh(0))) move_references(0);
       add_weights();
     }
     for (int t = 2; t < count; ++t) {
-      const float own_s[4] = {mine_s[0], mine_s[1], mine_s[2], mine_s[3]};
       const int pb = t & 1;
+      hand_over();
       score(after(stage, 2), pb);
       gather(stage, pb, 0);
       join(after(stage, 1), pb ^ 1, seg_p + t - 1, own_s);
@@ -581,15 +647,17 @@ __global__ void __launch_bounds__(kThreads, 1)
     done += count;
     // ---- the rows' results ----
 #pragma unroll
-    for (int r = 0; r < 2; ++r) {
-      l_sum[r] = quad_sum(l_sum[r]);
-      if (j == 0) sh.red_l[warp][g + 8 * r] = l_sum[r];
+    for (int n = 0; n < NH; ++n)
 #pragma unroll
-      for (int k = 0; k < NG; ++k) {
-        const float z = quad_sum(zsum[r][k]);
-        if (j == 0) sh.red_z[warp][g + 8 * r][k] = z;
+      for (int x = 0; x < 2; ++x) {
+        const float l = oct_sum(l_sum[n][x]);
+        if (g == 0) sh.red_l[warp][8 * n + 2 * j + x] = l;
+#pragma unroll
+        for (int k = 0; k < NG; ++k) {
+          const float z = oct_sum(zsum[n][x][k]);
+          if (g == 0) sh.red_z[warp][k][8 * n + 2 * j + x] = z;
+        }
       }
-    }
     tick(false);
     const bool whole = seg_p == 0 && count == seg_pages;
     float u = unit[0];
@@ -597,41 +665,38 @@ __global__ void __launch_bounds__(kThreads, 1)
     for (int k = 1; k < NG; ++k) u = own == k ? unit[k] : u;
     const float inv_u = 1.f / u;
     // a cut request's partial: slot 0 where the run begins in (or with) this request, else 1
-    const int64_t slot = (static_cast<int64_t>(2 * group + (first ? 0 : 1)) * blocks + block) * kRows;
+    const int64_t slot = (static_cast<int64_t>(2 * group + (first ? 0 : 1)) * blocks + block) * ROWS;
 #pragma unroll
-    for (int r = 0; r < 2; ++r) {
-      const int row = block * kRows + g + 8 * r;
-      float l = 0.f, z = 0.f;
-      for (int w = 0; w < kWarps; ++w) l += sh.red_l[w][g + 8 * r], z += sh.red_z[w][g + 8 * r][own];
-      const float inv = l == 0.f ? 0.f : inv_u / l;
-      const float lse = l == 0.f ? -INFINITY : (m_ref[r] + log2f(l)) * kLn2;
-      const bool live = row < a.q_len * a.heads;
-      const int t = live ? row / a.heads : 0, h = live ? row % a.heads : 0;
-      uint16_t* out = a.out + seg_b * a.o_sb + t * a.o_st + h * a.o_sh;
-      float* out_part = part.o + (slot + g + 8 * r) * D;
+    for (int n = 0; n < NH; ++n)
 #pragma unroll
-      for (int c = 0; c < CH; ++c) {
-        const int col = 32 * (warp * CH + c) + 8 * j;
-        float v[8];
+      for (int x = 0; x < 2; ++x) {
+        const int at = 8 * n + 2 * j + x, row = row0 + at;
+        float l = 0.f, z = 0.f;
+        for (int w = 0; w < kWarps; ++w) l += sh.red_l[w][at], z += sh.red_z[w][own][at];
+        const float inv = l == 0.f ? 0.f : inv_u / l;
+        const float lse = l == 0.f ? -INFINITY : (m_use[n][x] + log2f(l)) * kLn2;
+        const bool live = row < rows;
+        const int t = live ? row / a.heads : 0, h = live ? row % a.heads : 0;
+        uint16_t* out = a.out + seg_b * a.o_sb + t * a.o_st + h * a.o_sh;
+        float* out_part = part.o + (slot + at) * D;
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
+        for (int c = 0; c < CH; ++c) {
+          const int col = 32 * (warp * CH + c) + 4 * g;
+          float v[4];
 #pragma unroll
-          for (int k = 0; k < 2; ++k)
-            v[4 * k + i] = fmaf(i & 1 ? acc[4 * c + i][2 * r + k] - acc[4 * c + i - 1][2 * r + k] : acc[4 * c + i][2 * r + k],
-                                i & 1 ? 1048576.f : 16777216.f, -z) * inv;
-        if (!whole) {
-          reinterpret_cast<float4*>(out_part + col)[0] = make_float4(v[0], v[1], v[2], v[3]);
-          reinterpret_cast<float4*>(out_part + col)[1] = make_float4(v[4], v[5], v[6], v[7]);
-        } else if (live) {
-          *reinterpret_cast<uint4*>(out + col) = make_uint4(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]),
-                                                            pack_bf16x2(v[4], v[5]), pack_bf16x2(v[6], v[7]));
+          for (int i = 0; i < 2; ++i) {
+            const float even = acc[2 * c + i][n][x], both = acc[2 * c + i][n][x + 2];
+            v[2 * i] = fmaf(even, 16777216.f, -z) * inv;
+            v[2 * i + 1] = fmaf(both - even, 1048576.f, -z) * inv;
+          }
+          if (!whole) *reinterpret_cast<float4*>(out_part + col) = make_float4(v[0], v[1], v[2], v[3]);
+          else if (live) *reinterpret_cast<uint2*>(out + col) = make_uint2(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]));
+        }
+        if (warp == 0 && g == 0) {
+          if (!whole) part.lse[slot + at] = lse;
+          else if (live && a.lse) a.lse[(static_cast<int64_t>(seg_b) * a.q_len + t) * a.heads + h] = lse;
         }
       }
-      if (warp == 0 && j == 0) {
-        if (!whole) part.lse[slot + g + 8 * r] = lse;
-        else if (live && a.lse) a.lse[(static_cast<int64_t>(seg_b) * a.q_len + t) * a.heads + h] = lse;
-      }
-    }
     ++seg_b;
     seg_p = 0;
   }
@@ -674,7 +739,7 @@ __global__ void __launch_bounds__(kMergeThreads) merge_kernel(const DecodeArgs a
   // partial i is run r0 + i's: its first piece, but for a first run that begins in an earlier request
   const bool late = n > 0 && total * r0 / runs < first;
   auto slot = [&](int i) {
-    return (static_cast<int64_t>(2 * (r0 + i) + (i == 0 && late ? 1 : 0)) * blocks + row / kRows) * kRows + row % kRows;
+    return (static_cast<int64_t>(2 * (r0 + i) + (i == 0 && late ? 1 : 0)) * blocks + row / part.rows) * part.rows + row % part.rows;
   };
   grid_dependency_wait();
   float top = -INFINITY, den = 0.f;
@@ -718,10 +783,15 @@ __global__ void __launch_bounds__(kMergeThreads) merge_kernel(const DecodeArgs a
     a.lse[(static_cast<int64_t>(b) * a.q_len + t) * a.heads + h] = den == 0.f ? -INFINITY : top + logf(den);
 }
 
-int row_blocks(int q_len, int heads) { return (q_len * heads + kRows - 1) / kRows; }
-
-// Runs of pages per row block: one CTA a multiprocessor.
-int run_groups(int blocks) { return std::max(1, sm_count() / blocks); }
+// A CTA's tiles of 8 query rows: as few CTAs as hold them all, evenly filled.
+struct Shape {
+  int tiles, blocks, groups;  // tiles of a CTA, CTAs for all rows, runs of pages (a CTA each and row block)
+};
+Shape shape_of(int d, int q_len, int heads) {
+  const int tiles = (q_len * heads + 7) / 8, most = d == 512 ? 2 : 5;
+  const int blocks = (tiles + most - 1) / most;
+  return {(tiles + blocks - 1) / blocks, blocks, std::max(1, sm_count() / blocks)};
+}
 
 bool encode(CUtensorMap* map, const void* base, CUtensorMapDataType type, uint64_t width, uint64_t rows,
             uint64_t row_bytes, uint32_t box_width, CUtensorMapSwizzle swizzle) {
@@ -733,22 +803,23 @@ bool encode(CUtensorMap* map, const void* base, CUtensorMapDataType type, uint64
                              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-template <int D, int DR>
-int launch(const DecodeArgs& a, cudaStream_t s) {
-  using C = Cfg<D, DR>;
+template <int D, int DR, int NH>
+int launch(const DecodeArgs& a, const Shape& shape, cudaStream_t s) {
+  using C = Cfg<D, DR, NH>;
   CUtensorMap codes, rope;
   if (!encode(&codes, a.cache.codes, CU_TENSOR_MAP_DATA_TYPE_UINT8, D / 2, a.cache.num_slots, D / 2, 128,
               CU_TENSOR_MAP_SWIZZLE_128B) ||
       !encode(&rope, a.cache.rope, CU_TENSOR_MAP_DATA_TYPE_UINT16, DR, a.cache.num_slots, DR * 2, DR,
               DR == 64 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B))
     return ROLAQ_ECUDA;
-  const int blocks = row_blocks(a.q_len, a.heads), groups = run_groups(blocks);
+  const int blocks = shape.blocks, groups = shape.groups;
   Partials part;
   part.o = reinterpret_cast<float*>(static_cast<char*>(a.workspace) + kHeaderBytes);
-  part.lse = part.o + int64_t(2) * groups * blocks * kRows * D;
-  if (cudaFuncSetAttribute(decode_kernel<D, DR>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM) != cudaSuccess)
+  part.lse = part.o + int64_t(2) * groups * blocks * C::ROWS * D;
+  part.rows = C::ROWS;
+  if (cudaFuncSetAttribute(decode_kernel<D, DR, NH>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM) != cudaSuccess)
     return ROLAQ_ECUDA;
-  decode_kernel<D, DR><<<groups * blocks, kThreads, C::SMEM, s>>>(codes, rope, a, part, groups, blocks);
+  decode_kernel<D, DR, NH><<<groups * blocks, kThreads, C::SMEM, s>>>(codes, rope, a, part, groups, blocks);
   if (cudaGetLastError() != cudaSuccess) return ROLAQ_ECUDA;
 
   // Few requests are cut into many partials: all warps of a CTA share a row's then.
@@ -767,16 +838,29 @@ int launch(const DecodeArgs& a, cudaStream_t s) {
   return cudaLaunchKernelEx(&cfg, kernel, a, part, groups, blocks) == cudaSuccess ? ROLAQ_OK : ROLAQ_ECUDA;
 }
 
+template <int D, int DR>
+int launch_tiles(const DecodeArgs& a, cudaStream_t s) {
+  const Shape shape = shape_of(D, a.q_len, a.heads);
+  if (shape.tiles == 1) return launch<D, DR, 1>(a, shape, s);
+  if (shape.tiles == 2) return launch<D, DR, 2>(a, shape, s);
+  if constexpr (D == 256) {
+    if (shape.tiles == 3) return launch<D, DR, 3>(a, shape, s);
+    if (shape.tiles == 4) return launch<D, DR, 4>(a, shape, s);
+    return launch<D, DR, 5>(a, shape, s);
+  }
+  return ROLAQ_EUNSUPPORTED;
+}
+
 }  // namespace
 
 int64_t decode_workspace(int batch, int q_len, int heads, int d) {
-  const int blocks = row_blocks(q_len, heads);
-  return kHeaderBytes + int64_t(2) * run_groups(blocks) * blocks * kRows * (d + 1) * 4;
+  const Shape s = shape_of(d, q_len, heads);
+  return kHeaderBytes + int64_t(2) * s.groups * s.blocks * s.tiles * 8 * (d + 1) * 4;
 }
 
 int launch_decode(const DecodeArgs& a, cudaStream_t s) {
-  if (a.cache.latent_dim == 512) return a.cache.rope_dim == 64 ? launch<512, 64>(a, s) : launch<512, 32>(a, s);
-  return a.cache.rope_dim == 64 ? launch<256, 64>(a, s) : launch<256, 32>(a, s);
+  if (a.cache.latent_dim == 512) return a.cache.rope_dim == 64 ? launch_tiles<512, 64>(a, s) : launch_tiles<512, 32>(a, s);
+  return a.cache.rope_dim == 64 ? launch_tiles<256, 64>(a, s) : launch_tiles<256, 32>(a, s);
 }
 
 }  // namespace i4
