@@ -36,7 +36,7 @@ namespace {
 // Eight working warps and a warpgroup of which two warps load.  Of the 168 registers a thread that a block of
 // 384 is launched with, the loaders hand most to the workers: 2 * 224 + 56 = 2 * 232 + 40 = 3 * 168.
 constexpr int kWarps = 8, kWorkers = kWarps * 32, kThreads = kWorkers + 128;
-constexpr int kMinPages = 2;     // least run of pages worth a CTA of its own
+constexpr int kMinPages = 2;  // least run of pages worth a CTA of its own
 constexpr float kSlack = 1024.f, kScaleSlack = 32.f;  // how far weights and scales may pass their references (P s <= 2^15)
 constexpr float kNoMax = -1e30f, kNoUnit = 1.329227995784916e36f;  // references not yet set: the first token passes them
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
@@ -46,10 +46,11 @@ struct Cfg {
   static constexpr int NG = D / kGroup;             // groups of a token
   static constexpr int CODES = kPage * D / 2, ROPE = kPage * DR * 2, PARAMS = kPage * NG * 8;
   static constexpr int STAGE = CODES + ROPE + PARAMS;
-  static constexpr int STAGES = D == 512 ? 7 : DR == 64 ? 10 : 12;
+  static constexpr int QROW = (D + DR) * 2 + 16;    // bytes of a query row in shared memory (16: no bank conflicts)
+  static constexpr int STAGES = D == 512 ? 6 : DR == 64 ? 8 : 10;
   static constexpr int PTILE = kPage * 16;          // P s of a page, a group and 8 rows: [token][row] FP16
   static constexpr int PBUF = NG * NH * PTILE;
-  static constexpr int SMEM = 1024 + STAGES * STAGE + 2 * PBUF;
+  static constexpr int SMEM = 1024 + STAGES * STAGE + 2 * PBUF + 8 * NH * QROW;
   static constexpr int HG = NG / 2;                 // groups that a warp scores
   static constexpr int CH = D / kWarps / 32;        // 32-column chunks that a warp adds up
   static constexpr int ROWS = 8 * NH;
@@ -60,7 +61,8 @@ template <int NG, int NH>
 struct Shared {
   float2 swap[2][kWarps][NH][32];
   float red_m[kWarps][8 * NH], red_s[kWarps][NG], red_l[kWarps][8 * NH], red_z[kWarps][NG][8 * NH];
-  float q_sum[NG][8 * NH], row_scale[8 * NH];
+  float q_top[2][8 * NH], q_sum[NG][8 * NH], row_scale[8 * NH];
+  float l_all[8 * NH], z_all[NG][8 * NH], max[8 * NH];
 };
 
 // Named barriers: the end of a tick (working and loading warps), and the working warps'.
@@ -82,9 +84,22 @@ __device__ __forceinline__ int pages_of(const DecodeArgs& a, int b) {
 }
 
 // Runs are equal shares of the `total` pages: run r of n begins at page total * r / n.
-__device__ __forceinline__ int runs_of(int64_t total, int groups) {
-  return static_cast<int>(min(static_cast<int64_t>(groups), max(int64_t(1), (total + kMinPages - 1) / kMinPages)));
-}
+struct Runs {
+  int64_t total;
+  int n;
+  __device__ Runs(int64_t total_, int groups)
+      : total(total_), n(static_cast<int>(min(static_cast<int64_t>(groups), max(int64_t(1), (total_ + kMinPages - 1) / kMinPages)))) {}
+  __device__ int64_t begin(int r) const {
+    const uint64_t x = static_cast<uint64_t>(total) * r;
+    return x >> 32 ? static_cast<int64_t>(x / n) : static_cast<uint32_t>(x) / static_cast<uint32_t>(n);  // 32 bits where they do
+  }
+  __device__ int holding(int64_t page) const {  // the run that holds a page
+    const uint64_t x = static_cast<uint64_t>(page) * n;
+    int r = static_cast<int>(x >> 32 || total >> 32 ? x / total : static_cast<uint32_t>(x) / static_cast<uint32_t>(total));
+    while (begin(r + 1) <= page) ++r;
+    return r;
+  }
+};
 
 __device__ __forceinline__ void ldsm_x4(uint32_t addr, uint32_t (&r)[4]) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
@@ -165,6 +180,7 @@ __device__ __forceinline__ int64_t block_scan(int64_t v, int64_t& total, int64_t
 struct Partials {
   float* o;    // [2 * groups * row blocks][rows of a CTA][D], normalised
   float* lse;  // [2 * groups * row blocks][rows of a CTA], natural log
+  int4* cut;   // [batch]: a request's first run, its runs, whether the first begins in an earlier request
   int rows;    // of a CTA
 };
 
@@ -174,18 +190,22 @@ __global__ void __launch_bounds__(kThreads, 1)
                   const DecodeArgs a, const Partials part, const int groups, const int blocks) {
   using C = Cfg<D, DR, NH>;
   constexpr int NG = C::NG, HG = C::HG, CH = C::CH, STAGES = C::STAGES, ROWS = C::ROWS;
+  constexpr bool HELD_MAX = NH < 4;  // references in registers
   constexpr int KR = DR / 32;  // 16-column steps of the rotary part that a warp scores
   extern __shared__ char raw[];
   char* smem = reinterpret_cast<char*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
   char* pbuf = smem + STAGES * C::STAGE;
-  __shared__ uint64_t full[STAGES];
+  char* qbuf = pbuf + 2 * C::PBUF;
+  __shared__ uint64_t full[STAGES], q_full;
   __shared__ int bad_page[STAGES];
   __shared__ int64_t scan[kThreads / 32];
   __shared__ int start[2];
+  __shared__ int64_t run_total, run_begin;  // read again where a request ends (registers are short in between)
   __shared__ Shared<NG, NH> sh;
 
   const int tid = threadIdx.x, warp = tid / 32, lane = tid & 31, g = lane >> 2, j = lane & 3;
   const int block = blockIdx.x % blocks, group = blockIdx.x / blocks;
+  const int rows = a.q_len * a.heads, row0 = block * ROWS;
   grid_launch_dependents();
 
   // ---- this CTA's run of pages ----
@@ -194,13 +214,24 @@ __global__ void __launch_bounds__(kThreads, 1)
   for (int b = tid * per; b < min(a.batch, (tid + 1) * per); ++b) mine += pages_of(a, b);
   if (tid == 0) {
     for (int s = 0; s < STAGES; ++s) mbar_init(&full[s], 1);
+    mbar_init(&q_full, 1);
     fence_mbar_init();
   }
   int64_t before = block_scan<kThreads / 32>(mine, total, scan);
-  const int runs = runs_of(total, groups);
-  if (group >= runs || total == 0) return;
-  const int64_t u0 = total * group / runs;
-  const int n_units = static_cast<int>(total * (group + 1) / runs - u0);
+  for (int b = group; b < a.batch; b += groups) {  // requests without a token
+    if (pages_of(a, b) != 0) continue;
+    if (tid == 0 && block == 0) part.cut[b] = make_int4(0, 0, 0, 0);
+    for (int i = tid; i < min(ROWS, rows - row0) * (D / 8); i += kThreads) {
+      const int row = row0 + i / (D / 8), t = row / a.heads, h = row % a.heads;
+      *reinterpret_cast<uint4*>(a.out + b * a.o_sb + t * a.o_st + h * a.o_sh + 8 * (i % (D / 8))) = make_uint4(0, 0, 0, 0);
+      if (a.lse && i % (D / 8) == 0) a.lse[static_cast<int64_t>(b) * rows + row] = -INFINITY;
+    }
+  }
+  const Runs runs(total, groups);
+  if (group >= runs.n || total == 0) return;
+  const int64_t u0 = runs.begin(group);
+  const int n_units = static_cast<int>(runs.begin(group + 1) - u0);
+  if (tid == 0) run_total = total, run_begin = u0;
   if (before <= u0 && u0 < before + mine) {
     int b = tid * per;
     for (int n; before + (n = pages_of(a, b)) <= u0; ++b) before += n;
@@ -251,8 +282,17 @@ __global__ void __launch_bounds__(kThreads, 1)
       __syncwarp();
       if (++load_stage == STAGES) load_stage = 0;
     };
+    auto load_query = [&](int b) {
+      const int live = min(ROWS, rows - row0);
+      if (lane == 0) mbar_expect_tx(&q_full, live * ((D + DR) * 2));
+      __syncwarp();
+      for (int r = lane; r < live; r += 32) {
+        const int t = (row0 + r) / a.heads, h = (row0 + r) % a.heads;
+        bulk_load(qbuf + r * C::QROW, a.q + b * a.q_sb + t * a.q_st + h * a.q_sh, (D + DR) * 2, &q_full);
+      }
+    };
     // ================= the awaiting warp =================
-    int stage = 0, lap = 0, arrived = 0;
+    int stage = 0, lap = 0, arrived = 0, queries = 0;
     bool healthy = true;
     auto await = [&]() {  // the next page of the run; after one that did not come in time the rest is not awaited
       if (arrived == n_units) return;
@@ -261,22 +301,36 @@ __global__ void __launch_bounds__(kThreads, 1)
       ++arrived;
       if (++stage == STAGES) stage = 0, ++lap;
     };
+    auto await_query = [&]() {
+      if (healthy) healthy = mbar_wait(&q_full, queries & 1, a.err);
+      __syncwarp();
+      ++queries;
+    };
     if (loader) {
       next_ids = fetch_ids(0);
+      load_query(seg_b);
       for (int i = 0; i < STAGES; ++i) load();
     } else {
+      await_query();
       await();
     }
     tick(false);
-    for (int done = 0; done < n_units; ++seg_b, seg_p = 0) {
+    for (int done = 0; done < n_units;) {
       const int count = min(pages_of(a, seg_b) - seg_p, n_units - done);
-      if (count <= 0) continue;
-      for (int t = 0; t < count + 2; ++t) {
-        if (!loader && (t + 1 < count || t == count + 1)) await();  // the page that the next tick scores
-        tick(false);
-        if (loader && t >= 2) load();  // page t - 2 has been added up
-      }
       done += count;
+      do ++seg_b;  // the request after this one, where the run has one
+      while (done < n_units && pages_of(a, seg_b) == 0);
+      seg_p = 0;
+      for (int t = 0; t < count + 2; ++t) {
+        if (!loader && t + 1 < count) await();  // the page that the next tick scores
+        if (!loader && t == count + 1 && done < n_units) {
+          await_query();
+          await();
+        }
+        tick(false);
+        if (loader && t == 0 && done < n_units) load_query(seg_b);  // this request's query has been taken
+        if (loader && t >= 2) load();                               // page t - 2 has been added up
+      }
     }
     return;
   }
@@ -294,9 +348,8 @@ __global__ void __launch_bounds__(kThreads, 1)
   const uint32_t p_off = own * (NH * C::PTILE) + lane * 16;
   const uint32_t p_dst = (8 * warp + g) * 16 + 4 * j;
   const float qk_scale = a.sm_scale * kLog2e;
-  const int rows = a.q_len * a.heads, row0 = block * ROWS;
   int done = 0, stage = 0;  // pages of the run; the stage of the page scored next
-  tick(false);              // the first page is there
+  tick(false);              // the first query and page are there
 
   while (done < n_units) {
     const int seg_pages = pages_of(a, seg_b);
@@ -310,65 +363,74 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (tid == 0 && len != a.seq_lens[seg_b]) report(a.err, ROLAQ_DEV_BAD_REQ);
     const int lim_min = len - a.q_len + 1;
 
-    // ---- the query: row g of each tile, this warp's columns ----
-    uint32_t q[NH][8 * HG][2], q_pe[NH][KR][2];
-#pragma unroll
-    for (int n = 0; n < NH; ++n) {
-      const int row = row0 + 8 * n + g;
-      const bool live = row < rows;
-      const int t = live ? row / a.heads : 0, h = live ? row % a.heads : 0;
-      const uint16_t* src = a.q + seg_b * a.q_sb + t * a.q_st + h * a.q_sh;
+    // ---- the query: brought to operand form in place, 8 elements at a time, then row g of each tile to registers ----
+    constexpr int QC = D / 8;  // 16-byte pieces of a row's latent part
+    const int live = min(ROWS, rows - row0);
+#pragma unroll 1
+    for (int i = tid; i < ROWS * QC; i += kWorkers) {
+      const int r = i / QC;
       float top = 0.f, odd = 0.f;
-      uint4 raw_q[D / 32];  // the whole row: both halves scale it alike
-#pragma unroll
-      for (int c = 0; c < D / 32; ++c) {
-        raw_q[c] = live ? *reinterpret_cast<const uint4*>(src + 32 * c + 8 * j) : make_uint4(0, 0, 0, 0);
-        const uint32_t v[4] = {raw_q[c].x, raw_q[c].y, raw_q[c].z, raw_q[c].w};
+      if (r < live) {
+        const uint4 w = *reinterpret_cast<const uint4*>(qbuf + r * C::QROW + 16 * (i % QC));
+        const uint32_t v[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
           top = fmaxf(top, fmaxf(fabsf(bf16_lo(v[k])), fabsf(bf16_hi(v[k]))));
-          odd += bf16_lo(v[k]) * 0.f + bf16_hi(v[k]) * 0.f;  // NaN where an element is no finite number
+          odd = fmaf(bf16_lo(v[k]), 0.f, fmaf(bf16_hi(v[k]), 0.f, odd));  // NaN where an element is no finite number
         }
       }
-      top = quad_max(top);
-      odd = quad_sum(odd);
-      // 2^k with top 2^k in [2^13, 2^14)
-      const int k = min(max(13 - (static_cast<int>(__float_as_uint(top) >> 23) - 127), -100), 100);
-      const float up = top > 0.f ? pow2(k) : 1.f;
-      if (warp == 0 && j == 0)
-        sh.row_scale[8 * n + g] = odd != 0.f ? __int_as_float(0x7FC00000) : qk_scale * (16777216.f / up);
-      float sum[HG];
+      top = warp_max_f32(odd != 0.f ? INFINITY : top);
+      if (lane == 0) sh.q_top[D == 512 ? (i / 32) & 1 : 0][r] = top;
+    }
+    work_sync();
+    auto row_top = [&](int r) { return D == 512 ? fmaxf(sh.q_top[0][r], sh.q_top[1][r]) : sh.q_top[0][r]; };
+    auto row_unit = [&](float top) {  // 2^k with top 2^k in [2^13, 2^14)
+      return top > 0.f ? pow2(min(max(13 - (static_cast<int>(__float_as_uint(top) >> 23) - 127), -100), 100)) : 1.f;
+    };
+#pragma unroll 1
+    for (int i = tid; i < ROWS * QC; i += kWorkers) {
+      const int r = i / QC, c = i % QC;
+      const float top = row_top(r), up = row_unit(top);
+      uint4* at = reinterpret_cast<uint4*>(qbuf + r * C::QROW + 16 * c);
+      const uint4 w = r < live ? *at : make_uint4(0, 0, 0, 0);
+      const uint32_t v[4] = {w.x, w.y, w.z, w.w};
+      float x[8], sum = 0.f;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        x[2 * e] = bf16_lo(v[e]) * up, x[2 * e + 1] = bf16_hi(v[e]) * up;
+        sum += x[2 * e] + x[2 * e + 1];
+      }
+      // a word of codes gives elements (0, 4), 16 (1, 5), (2, 6) and 16 (3, 7)
+      *at = make_uint4(pack_half2(x[0], x[4]), pack_half2(x[1] * 0.0625f, x[5] * 0.0625f), pack_half2(x[2], x[6]),
+                       pack_half2(x[3] * 0.0625f, x[7] * 0.0625f));
+#pragma unroll
+      for (int o = 1; o < 16; o *= 2) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, o);
+      if (c % 16 == 0) sh.q_sum[c / 16][r] = sum * (1.f / 16777216.f);
+      if (c == 0) sh.row_scale[r] = top == INFINITY ? __int_as_float(0x7FC00000) : qk_scale * (16777216.f / up);
+    }
+    // the rotary part under the same power of two (exact), so that both parts add up
+#pragma unroll 1
+    for (int i = tid; i < ROWS * (DR / 2); i += kWorkers) {
+      const int r = i / (DR / 2);
+      const float down = row_unit(row_top(r)) * (1.f / 16777216.f);
+      uint32_t* at = reinterpret_cast<uint32_t*>(qbuf + r * C::QROW + 2 * D) + i % (DR / 2);
+      *at = r < live ? pack_bf16x2(bf16_lo(*at) * down, bf16_hi(*at) * down) : 0u;
+    }
+    work_sync();
+    uint32_t q[NH][8 * HG][2], q_pe[NH][KR][2];
+#pragma unroll
+    for (int n = 0; n < NH; ++n) {
+      const char* src = qbuf + (8 * n + g) * C::QROW;
 #pragma unroll
       for (int c = 0; c < 4 * HG; ++c) {
-        const uint4 pick = half ? raw_q[4 * HG + c] : raw_q[c];
-        const uint32_t v[4] = {pick.x, pick.y, pick.z, pick.w};
-        float x[8];
-        if (c % 4 == 0) sum[c / 4] = 0.f;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          x[2 * e] = bf16_lo(v[e]) * up, x[2 * e + 1] = bf16_hi(v[e]) * up;
-          sum[c / 4] += x[2 * e] + x[2 * e + 1];
-        }
-        // a word of codes gives elements (0, 4), 16 (1, 5), (2, 6) and 16 (3, 7)
-        q[n][2 * c][0] = pack_half2(x[0], x[4]), q[n][2 * c][1] = pack_half2(x[1] * 0.0625f, x[5] * 0.0625f);
-        q[n][2 * c + 1][0] = pack_half2(x[2], x[6]), q[n][2 * c + 1][1] = pack_half2(x[3] * 0.0625f, x[7] * 0.0625f);
+        const uint4 w = *reinterpret_cast<const uint4*>(src + half * D + 64 * c + 16 * j);
+        q[n][2 * c][0] = w.x, q[n][2 * c][1] = w.y, q[n][2 * c + 1][0] = w.z, q[n][2 * c + 1][1] = w.w;
       }
-#pragma unroll
-      for (int i = 0; i < HG; ++i) {
-        sum[i] = quad_sum(sum[i]) * (1.f / 16777216.f);
-        if (quarter == 0 && j == 0) sh.q_sum[half * HG + i][8 * n + g] = sum[i];
-      }
-      // the rotary part under the same power of two (exact), so that both parts add up
-      const float down = up * (1.f / 16777216.f);
 #pragma unroll
       for (int c = 0; c < KR; ++c)
 #pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const uint32_t v = live ? *reinterpret_cast<const uint32_t*>(src + D + 16 * (half * KR + c) + 8 * e + 2 * j) : 0;
-          q_pe[n][c][e] = pack_bf16x2(bf16_lo(v) * down, bf16_hi(v) * down);
-        }
+        for (int e = 0; e < 2; ++e) q_pe[n][c][e] = *reinterpret_cast<const uint32_t*>(src + 2 * (D + 16 * (half * KR + c) + 8 * e + 2 * j));
     }
-    work_sync();
     // the rows' factors: held where few, read again each page where many
     float2 held_sum[NH <= 2 ? HG : 1][NH <= 2 ? NH : 1], held_scale[NH <= 2 ? NH : 1];
     auto q_sum_of = [&](int k, int n) { return *reinterpret_cast<const float2*>(&sh.q_sum[half * HG + k][8 * n + 2 * j]); };
@@ -383,23 +445,34 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
 
     // accumulators: tile 2 c + h of chunk c holds columns 4 g + 2 h (and that + 16 times the next one) x rows 2 j, + 1
-    float acc[2 * CH][NH][4], zsum[NH][2][NG], unit[NG], l_sum[NH][2], m_use[NH][2];
+    float acc[2 * CH][NH][4], zsum[NH][2][NG], unit[NG], l_sum[NH][2];
+    float2 held_max[HELD_MAX ? NH : 1];  // references: the largest scores so far, kNoMax before the first
 #pragma unroll
     for (int n = 0; n < NH; ++n) {
 #pragma unroll
       for (int c = 0; c < 2 * CH; ++c) acc[c][n][0] = acc[c][n][1] = acc[c][n][2] = acc[c][n][3] = 0.f;
 #pragma unroll
       for (int x = 0; x < 2; ++x) {
-        l_sum[n][x] = 0.f, m_use[n][x] = kNoMax;
+        l_sum[n][x] = 0.f;
 #pragma unroll
         for (int k = 0; k < NG; ++k) zsum[n][x][k] = 0.f;
       }
     }
 #pragma unroll
     for (int k = 0; k < NG; ++k) unit[k] = kNoUnit;
+    auto max_of = [&](int n) {
+      if constexpr (HELD_MAX) return held_max[n];
+      else return *reinterpret_cast<const float2*>(&sh.max[8 * n + 2 * j]);
+    };
+    auto set_max = [&](int n, float2 m) {
+      if constexpr (HELD_MAX) held_max[n] = m;
+      else if (warp == 0 && g == 0) *reinterpret_cast<float2*>(&sh.max[8 * n + 2 * j]) = m;
+    };
+#pragma unroll
+    for (int n = 0; n < NH; ++n) set_max(n, make_float2(kNoMax, kNoMax));
 
     // Partial scores of the pair's 16 tokens: the warp's own eight in mine_s, the partner's to the swap.
-    float mine_s[NH][2];
+    float mine_s[NH][2] = {};
     auto score = [&](int st_at, int pb) {
       const uint32_t st = stages + st_at * C::STAGE;
       float c_acc[HG][NH][4], r_acc[NH][4];
@@ -505,8 +578,9 @@ __global__ void __launch_bounds__(kThreads, 1)
       float weights = 0.f, sizes = 0.f;
 #pragma unroll
       for (int n = 0; n < NH; ++n) {
-        p_val[n][0] = ex2_approx(s_val[n][0] - m_use[n][0]);
-        p_val[n][1] = ex2_approx(s_val[n][1] - m_use[n][1]);
+        const float2 m = max_of(n);
+        p_val[n][0] = ex2_approx(s_val[n][0] - m.x);
+        p_val[n][1] = ex2_approx(s_val[n][1] - m.y);
         weights += p_val[n][0] + p_val[n][1];
       }
       char* dst = pbuf + pb * C::PBUF + p_dst;
@@ -550,19 +624,26 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (k == own) keep_own = keep_unit[k];
       }
 #pragma unroll
-      for (int n = 0; n < NH; ++n)
+      for (int n = 0; n < NH; ++n) {
+        const float2 old = max_of(n);
+        float2 m = old;
+        for (int w = 0; w < kWarps; ++w) {
+          const float2 v = *reinterpret_cast<const float2*>(&sh.red_m[w][8 * n + 2 * j]);
+          m.x = fmaxf(m.x, v.x), m.y = fmaxf(m.y, v.y);
+        }
+        if constexpr (!HELD_MAX) work_sync();  // all have read the old ones
+        set_max(n, m);
 #pragma unroll
         for (int x = 0; x < 2; ++x) {
-          float m = m_use[n][x];
-          for (int w = 0; w < kWarps; ++w) m = fmaxf(m, sh.red_m[w][8 * n + 2 * j + x]);
-          const float keep = ex2_approx(m_use[n][x] - m);
-          m_use[n][x] = m;
+          const float keep = ex2_approx(x ? old.y - m.y : old.x - m.x);
           l_sum[n][x] *= keep;
 #pragma unroll
           for (int k = 0; k < NG; ++k) zsum[n][x][k] *= keep * keep_unit[k];
 #pragma unroll
           for (int c = 0; c < 2 * CH; ++c) acc[c][n][x] *= keep * keep_own, acc[c][n][x + 2] *= keep * keep_own;
         }
+      }
+      if constexpr (!HELD_MAX) work_sync();
       weigh(pb);
       work_sync();
     };
@@ -605,45 +686,53 @@ __global__ void __launch_bounds__(kThreads, 1)
 
     // ---- the pages: tick t scores page t, weighs page t - 1 and adds page t - 2 up ----
     auto after = [](int s, int n) { return s + n >= STAGES ? s + n - STAGES : s + n; };
-    float own_s[NH][2];
-    auto hand_over = [&]() {
+    int st_score = stage, st_weigh = stage, st_add = stage;
+    // A tick of whatever parts it has: the first two and the last.
+    auto any_tick = [&](int t) {
+      const int pb = t & 1;
+      float own_s[NH][2];
 #pragma unroll
       for (int n = 0; n < NH; ++n) own_s[n][0] = mine_s[n][0], own_s[n][1] = mine_s[n][1];
+      if (t < count) {
+        score(st_score, pb);
+        st_score = after(st_score, 1);
+      }
+      if (t >= 2) {
+        gather(st_add, pb, 0);
+        gather(st_add, pb, 1);
+        st_add = after(st_add, 1);
+      }
+      bool vote = false;
+      if (t >= 1) {
+        join(st_weigh, pb ^ 1, seg_p + t - 1, own_s);
+        st_weigh = after(st_weigh, 1);
+        vote = weigh(pb ^ 1);
+      }
+      if (tick(vote)) move_references(pb ^ 1);
+      if (t >= 1) add_weights();
     };
-    score(stage, 0);
-    tick(false);
-    {
-      hand_over();
-      if (count > 1) score(after(stage, 1), 1);
-      join(stage, 0, seg_p, own_s);
-      if (tick(weigh(0))) move_references(0);
-      add_weights();
-    }
-    for (int t = 2; t < count; ++t) {
+#pragma unroll 1
+    for (int t = 0; t <= count; ++t) {
+      if (t < 2 || t == count) {
+        any_tick(t);
+        continue;
+      }
       const int pb = t & 1;
-      hand_over();
-      score(after(stage, 2), pb);
-      gather(stage, pb, 0);
-      join(after(stage, 1), pb ^ 1, seg_p + t - 1, own_s);
-      gather(stage, pb, 1);
-      const bool move = tick(weigh(pb ^ 1));
-      if (move) move_references(pb ^ 1);
+      float own_s[NH][2];
+#pragma unroll
+      for (int n = 0; n < NH; ++n) own_s[n][0] = mine_s[n][0], own_s[n][1] = mine_s[n][1];
+      score(st_score, pb);
+      gather(st_add, pb, 0);
+      gather(st_add, pb, 1);
+      join(st_weigh, pb ^ 1, seg_p + t - 1, own_s);
+      const bool vote = weigh(pb ^ 1);
+      st_score = after(st_score, 1), st_weigh = after(st_weigh, 1), st_add = after(st_add, 1);
+      if (tick(vote)) move_references(pb ^ 1);
       add_weights();
-      stage = after(stage, 1);
     }
-    if (count > 1) {
-      const int pb = count & 1;
-      gather(stage, pb, 0);
-      join(after(stage, 1), pb ^ 1, seg_p + count - 1, mine_s);
-      gather(stage, pb, 1);
-      const bool move = tick(weigh(pb ^ 1));
-      if (move) move_references(pb ^ 1);
-      add_weights();
-      stage = after(stage, 1);
-    }
-    gather(stage, (count - 1) & 1, 0);
-    gather(stage, (count - 1) & 1, 1);
-    stage = after(stage, 1);
+    gather(st_add, (count - 1) & 1, 0);
+    gather(st_add, (count - 1) & 1, 1);
+    stage = st_score;
     done += count;
     // ---- the rows' results ----
 #pragma unroll
@@ -659,7 +748,22 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
       }
     tick(false);
+    for (int i = tid; i < ROWS * (NG + 1); i += kWorkers) {
+      const int at = i % ROWS, k = i / ROWS - 1;
+      float s = 0.f;
+#pragma unroll
+      for (int w = 0; w < kWarps; ++w) s += k < 0 ? sh.red_l[w][at] : sh.red_z[w][max(k, 0)][at];
+      if (k < 0) sh.l_all[at] = s;
+      else sh.z_all[k][at] = s;
+    }
+    work_sync();
     const bool whole = seg_p == 0 && count == seg_pages;
+    if (tid == 0 && block == 0 && seg_p == 0) {  // the run that begins a request says how it is cut
+      const Runs again(run_total, groups);
+      const int64_t page0 = run_begin + (done - count);
+      part.cut[seg_b] = whole ? make_int4(0, 0, 0, 0)
+                              : make_int4(group, again.holding(page0 + seg_pages - 1) - group + 1, run_begin < page0, 0);
+    }
     float u = unit[0];
 #pragma unroll
     for (int k = 1; k < NG; ++k) u = own == k ? unit[k] : u;
@@ -671,10 +775,9 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
       for (int x = 0; x < 2; ++x) {
         const int at = 8 * n + 2 * j + x, row = row0 + at;
-        float l = 0.f, z = 0.f;
-        for (int w = 0; w < kWarps; ++w) l += sh.red_l[w][at], z += sh.red_z[w][own][at];
+        const float l = sh.l_all[at], z = sh.z_all[own][at];
         const float inv = l == 0.f ? 0.f : inv_u / l;
-        const float lse = l == 0.f ? -INFINITY : (m_use[n][x] + log2f(l)) * kLn2;
+        const float lse = l == 0.f ? -INFINITY : ((x ? max_of(n).y : max_of(n).x) + log2f(l)) * kLn2;
         const bool live = row < rows;
         const int t = live ? row / a.heads : 0, h = live ? row % a.heads : 0;
         uint16_t* out = a.out + seg_b * a.o_sb + t * a.o_st + h * a.o_sh;
@@ -694,9 +797,10 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         if (warp == 0 && g == 0) {
           if (!whole) part.lse[slot + at] = lse;
-          else if (live && a.lse) a.lse[(static_cast<int64_t>(seg_b) * a.q_len + t) * a.heads + h] = lse;
+          else if (live && a.lse) a.lse[static_cast<int64_t>(seg_b) * rows + row] = lse;
         }
       }
+
     ++seg_b;
     seg_p = 0;
   }
@@ -704,44 +808,22 @@ __global__ void __launch_bounds__(kThreads, 1)
 
 constexpr int kMergeWarps = 8, kMergeThreads = kMergeWarps * 32;
 
-// Joins the partials of the requests that more than one run holds, and writes the rows of requests
-// without a token.  WARPS warps share the partials of 128 columns of one row.
+// Joins the partials of the requests that more than one run holds, in the runs' order.  WARPS warps share the
+// partials of 128 columns of one row.
 template <int D, int WARPS>
-__global__ void __launch_bounds__(kMergeThreads) merge_kernel(const DecodeArgs a, const Partials part, const int groups,
-                                                         const int blocks) {
+__global__ void __launch_bounds__(kMergeThreads) merge_kernel(const DecodeArgs a, const Partials part, const int blocks) {
   constexpr int CHUNKS = D / 128, TASKS = kMergeWarps / WARPS;
-  __shared__ int64_t scan[kMergeWarps], scan2[kMergeWarps];
-  __shared__ float4 red[kMergeWarps][32];
-  const int tid = threadIdx.x, warp = tid / 32, lane = tid & 31, b = blockIdx.y;
-  int64_t sum = 0, below = 0, total, first;
-  for (int i = tid; i < a.batch; i += kMergeThreads) {
-    const int n = pages_of(a, i);
-    sum += n;
-    if (i < b) below += n;
-  }
-  block_scan<kMergeWarps>(sum, total, scan);
-  block_scan<kMergeWarps>(below, first, scan2);
-  const int pages = pages_of(a, b);
-  const int runs = runs_of(total, groups);
-  // the runs that hold the request's first and last page
-  int64_t r0 = 0, r1 = 0;
-  if (pages > 0) {
-    r0 = first * runs / total;
-    while (total * (r0 + 1) / runs <= first) ++r0;
-    r1 = (first + pages - 1) * runs / total;
-    while (total * (r1 + 1) / runs <= first + pages - 1) ++r1;
-  }
-  const int n = pages == 0 ? 0 : static_cast<int>(r1 - r0 + 1);
-  if (n == 1) return;
-  const int task = blockIdx.x * TASKS + warp / WARPS, row = task / CHUNKS, col = (task % CHUNKS) * 128 + 4 * lane;
+  const int warp = threadIdx.x / 32, lane = threadIdx.x & 31, b = blockIdx.y;
+  const int task = blockIdx.x * TASKS + warp / WARPS, share = warp % WARPS;
+  const int row = task / CHUNKS, col = (task % CHUNKS) * 128 + 4 * lane;
   const bool live = row < a.q_len * a.heads;
-  const int share = warp % WARPS;
-  // partial i is run r0 + i's: its first piece, but for a first run that begins in an earlier request
-  const bool late = n > 0 && total * r0 / runs < first;
-  auto slot = [&](int i) {
-    return (static_cast<int64_t>(2 * (r0 + i) + (i == 0 && late ? 1 : 0)) * blocks + row / part.rows) * part.rows + row % part.rows;
-  };
   grid_dependency_wait();
+  const int4 cut = part.cut[b];
+  const int n = cut.y;
+  if (n == 0) return;
+  auto slot = [&](int i) {
+    return (static_cast<int64_t>(2 * (cut.x + i) + (i == 0 ? cut.z : 0)) * blocks + row / part.rows) * part.rows + row % part.rows;
+  };
   float top = -INFINITY, den = 0.f;
   float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
   if (live) {
@@ -753,16 +835,17 @@ __global__ void __launch_bounds__(kMergeThreads) merge_kernel(const DecodeArgs a
     }
     top = warp_max_f32(top);
     if (__any_sync(0xFFFFFFFFu, odd)) top = __int_as_float(0x7FC00000);
+#pragma unroll 8
     for (int i = share; i < n; i += WARPS) {
       const float l = part.lse[slot(i)];
-      if (l == -INFINITY) continue;
-      const float w = ex2_approx((l - top) * kLog2e);
       const float4 v = *reinterpret_cast<const float4*>(part.o + slot(i) * D + col);
+      const float w = l == -INFINITY ? 0.f : ex2_approx((l - top) * kLog2e);
       den += w;
       acc.x = fmaf(w, v.x, acc.x), acc.y = fmaf(w, v.y, acc.y), acc.z = fmaf(w, v.z, acc.z), acc.w = fmaf(w, v.w, acc.w);
     }
   }
   if constexpr (WARPS > 1) {
+    __shared__ float4 red[kMergeWarps][32];
     __shared__ float dens[kMergeWarps];
     red[warp][lane] = acc;
     if (lane == 0) dens[warp] = den;
@@ -814,7 +897,8 @@ int launch(const DecodeArgs& a, const Shape& shape, cudaStream_t s) {
     return ROLAQ_ECUDA;
   const int blocks = shape.blocks, groups = shape.groups;
   Partials part;
-  part.o = reinterpret_cast<float*>(static_cast<char*>(a.workspace) + kHeaderBytes);
+  part.cut = reinterpret_cast<int4*>(static_cast<char*>(a.workspace) + kHeaderBytes);
+  part.o = reinterpret_cast<float*>(part.cut + a.batch);
   part.lse = part.o + int64_t(2) * groups * blocks * C::ROWS * D;
   part.rows = C::ROWS;
   if (cudaFuncSetAttribute(decode_kernel<D, DR, NH>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM) != cudaSuccess)
@@ -835,7 +919,7 @@ int launch(const DecodeArgs& a, const Shape& shape, cudaStream_t s) {
   cfg.attrs = attr;
   cfg.numAttrs = 1;
   const auto kernel = wide ? merge_kernel<D, kMergeWarps> : merge_kernel<D, 1>;
-  return cudaLaunchKernelEx(&cfg, kernel, a, part, groups, blocks) == cudaSuccess ? ROLAQ_OK : ROLAQ_ECUDA;
+  return cudaLaunchKernelEx(&cfg, kernel, a, part, blocks) == cudaSuccess ? ROLAQ_OK : ROLAQ_ECUDA;
 }
 
 template <int D, int DR>
@@ -855,7 +939,7 @@ int launch_tiles(const DecodeArgs& a, cudaStream_t s) {
 
 int64_t decode_workspace(int batch, int q_len, int heads, int d) {
   const Shape s = shape_of(d, q_len, heads);
-  return kHeaderBytes + int64_t(2) * s.groups * s.blocks * s.tiles * 8 * (d + 1) * 4;
+  return kHeaderBytes + int64_t(16) * batch + int64_t(2) * s.groups * s.blocks * s.tiles * 8 * (d + 1) * 4;
 }
 
 int launch_decode(const DecodeArgs& a, cudaStream_t s) {

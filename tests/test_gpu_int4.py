@@ -163,6 +163,24 @@ def test_attention_over_one_long_request_and_over_many_short_ones(batch, ctx, q_
     assert torch.equal(out, again) and torch.equal(lse, lse2)
 
 
+@pytest.mark.parametrize("lens", [[64 * 13 * 2, 64 * 300], [64 * 161, 64 * 160, 1, 0, 64 * 163 + 5], [64 * 97, 64 * 400, 64 * 30, 64 * 222], [30000] + [70] * 40])
+@pytest.mark.parametrize("heads", [16, 40])
+def test_requests_cut_into_few_and_many_partials(lens, heads):
+    """Long requests next to one another and to short ones: partials joined in one and in two steps."""
+    table, pages = _requests(lens, seed=sum(lens))
+    cache = ref.random_cache(pages * 64, 256, 32, seed=len(lens))
+    q = torch.randn(len(lens), 1, heads, 288, generator=torch.Generator().manual_seed(2)).bfloat16().cuda()
+    view = int4.Int4View(*cache)
+    ws = int4.Workspace(view, len(lens), 1, heads, table.shape[1])
+    out = torch.empty(len(lens), 1, heads, 256, dtype=torch.bfloat16, device="cuda")
+    lse = torch.empty(len(lens), 1, heads, device="cuda")
+    sl = torch.tensor(lens, dtype=torch.int32, device="cuda")
+    for _ in range(2):
+        out.fill_(math.nan)
+        int4.decode(q, view, table, sl, SM, out, lse, ws)
+        _check(q, cache, table, lens, out, lse)
+
+
 def test_attention_where_the_maximum_keeps_rising_and_where_it_falls():
     """Logits that grow by hundreds along the request (every reference maximum is left behind), and the reverse."""
     n = 1500
