@@ -25,6 +25,7 @@
 // The pages of all requests are dealt to the CTAs in one equal run each (a run may begin or end inside
 // a request); what is cut is joined by merge_kernel by log-sum-exp.
 #include <algorithm>
+#include <atomic>
 
 #include "int4.cuh"
 #include "kernels.cuh"
@@ -206,17 +207,20 @@ __global__ void __launch_bounds__(kThreads, 1)
   const int tid = threadIdx.x, warp = tid / 32, lane = tid & 31, g = lane >> 2, j = lane & 3;
   const int block = blockIdx.x % blocks, group = blockIdx.x / blocks;
   const int rows = a.q_len * a.heads, row0 = block * ROWS;
+  if (tid == 0) {
+    for (int s = 0; s < STAGES; ++s) mbar_init(&full[s], 1);
+    mbar_init(&q_full, 1);
+    fence_mbar_init();
+    prefetch_tensormap(&map_codes);
+    prefetch_tensormap(&map_rope);
+  }
   grid_launch_dependents();
+  grid_dependency_wait();
 
   // ---- this CTA's run of pages ----
   const int per = (a.batch + kThreads - 1) / kThreads;
   int64_t mine = 0, total;
   for (int b = tid * per; b < min(a.batch, (tid + 1) * per); ++b) mine += pages_of(a, b);
-  if (tid == 0) {
-    for (int s = 0; s < STAGES; ++s) mbar_init(&full[s], 1);
-    mbar_init(&q_full, 1);
-    fence_mbar_init();
-  }
   int64_t before = block_scan<kThreads / 32>(mine, total, scan);
   for (int b = group; b < a.batch; b += groups) {  // requests without a token
     if (pages_of(a, b) != 0) continue;
@@ -901,23 +905,34 @@ int launch(const DecodeArgs& a, const Shape& shape, cudaStream_t s) {
   part.o = reinterpret_cast<float*>(part.cut + a.batch);
   part.lse = part.o + int64_t(2) * groups * blocks * C::ROWS * D;
   part.rows = C::ROWS;
-  if (cudaFuncSetAttribute(decode_kernel<D, DR, NH>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM) != cudaSuccess)
-    return ROLAQ_ECUDA;
-  decode_kernel<D, DR, NH><<<groups * blocks, kThreads, C::SMEM, s>>>(codes, rope, a, part, groups, blocks);
-  if (cudaGetLastError() != cudaSuccess) return ROLAQ_ECUDA;
+  static std::atomic<uint64_t> prepared{0};  // devices whose shared-memory limit is raised
+  int device = 0;
+  if (cudaGetDevice(&device) != cudaSuccess) return ROLAQ_ECUDA;
+  if (!(prepared.load() >> (device & 63) & 1)) {
+    if (cudaFuncSetAttribute(decode_kernel<D, DR, NH>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM) != cudaSuccess)
+      return ROLAQ_ECUDA;
+    prepared |= uint64_t(1) << (device & 63);
+  }
+  // Both kernels may start before the one ahead of them in the stream has ended; they wait for it where they
+  // first read or write what it may have to do with.
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(groups * blocks);
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = C::SMEM;
+  cfg.stream = s;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  if (cudaLaunchKernelEx(&cfg, decode_kernel<D, DR, NH>, codes, rope, a, part, groups, blocks) != cudaSuccess) return ROLAQ_ECUDA;
 
   // Few requests are cut into many partials: all warps of a CTA share a row's then.
   const bool wide = groups >= 8 * a.batch;
   const int tasks = a.q_len * a.heads * (D / 128), per_cta = wide ? 1 : kMergeWarps;
-  cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((tasks + per_cta - 1) / per_cta, a.batch);
   cfg.blockDim = dim3(kMergeThreads);
-  cfg.stream = s;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
+  cfg.dynamicSmemBytes = 0;
   const auto kernel = wide ? merge_kernel<D, kMergeWarps> : merge_kernel<D, 1>;
   return cudaLaunchKernelEx(&cfg, kernel, a, part, blocks) == cudaSuccess ? ROLAQ_OK : ROLAQ_ECUDA;
 }
@@ -938,8 +953,8 @@ int launch_tiles(const DecodeArgs& a, cudaStream_t s) {
 }  // namespace
 
 int64_t decode_workspace(int batch, int q_len, int heads, int d) {
-  const Shape s = shape_of(d, q_len, heads);
-  return kHeaderBytes + int64_t(16) * batch + int64_t(2) * s.groups * s.blocks * s.tiles * 8 * (d + 1) * 4;
+  const Shape s = shape_of(d, q_len, heads);  // groups * blocks <= sm_count() + blocks; that does not shrink as calls grow
+  return kHeaderBytes + int64_t(16) * batch + int64_t(2) * (sm_count() + s.blocks) * s.tiles * 8 * (d + 1) * 4;
 }
 
 int launch_decode(const DecodeArgs& a, cudaStream_t s) {

@@ -3,6 +3,8 @@
 //
 // Codec (the uniform min/max codec of mla_quant/oscar.py:91-101 with 16 levels): per 128 elements
 // scale = (hi - lo) / 15, code = round((x - lo) / scale), zero = -lo / scale, value = (code - zero) scale.
+#include <algorithm>
+
 #include "int4.cuh"
 
 namespace rolaq {
@@ -27,23 +29,25 @@ __device__ __forceinline__ void load16(const uint16_t* p, float (&x)[16]) {
   }
 }
 
-// Eight threads per unit: a unit is one 128-element group of a row (16 elements a thread, min and max
-// over the eight by shuffles) or the row's k_pe.
-template <typename T>
-__global__ void write_kernel(const T* __restrict__ c, int64_t ld_c, const uint16_t* __restrict__ k_pe, int64_t ld_pe,
-                             const void* slots, int slots64, int64_t n, rolaq_int4_cache cache, int32_t* err) {
-  const int ng = cache.latent_dim / kGroup;
-  const int64_t unit = (static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x) / 8;
+// Eight threads per unit: a unit is one 128-element group of a row (16 elements a thread, min and max over the
+// eight by shuffles) or the row's k_pe.  Bound by memory as long as the 16 divisions of a thread are not: the
+// quotient's rounding is decided by a product with the reciprocal, which is within 2^-20 of the quotient, unless that
+// lies within 1e-4 of a half; then the thread divides.
+template <typename T, int NG>
+__global__ void __launch_bounds__(256) write_kernel(const T* __restrict__ c, int64_t ld_c,
+                                                    const uint16_t* __restrict__ k_pe, int64_t ld_pe, const void* slots,
+                                                    int slots64, int64_t n, rolaq_int4_cache cache, int32_t* err) {
+  const uint32_t unit = (blockIdx.x * 256u + threadIdx.x) / 8;
   const int part = threadIdx.x & 7;
-  const int64_t row = unit / (ng + 1);
-  const int g = static_cast<int>(unit % (ng + 1));
+  const int64_t row = unit / (NG + 1);
+  const int g = unit % (NG + 1);
   if (row >= n) return;  // whole groups of eight threads leave together
   const int64_t slot = load_index(slots, slots64, row);
   if (slot < 0 || slot >= cache.num_slots) {
     if (part == 0) report(err, ROLAQ_DEV_BAD_SLOT);
     return;
   }
-  if (g == ng) {
+  if (g == NG) {
     if (part * 8 < cache.rope_dim)
       *reinterpret_cast<uint4*>(cache.rope + slot * cache.rope_dim + part * 8) =
           *reinterpret_cast<const uint4*>(k_pe + row * ld_pe + part * 8);
@@ -56,7 +60,7 @@ __global__ void write_kernel(const T* __restrict__ c, int64_t ld_c, const uint16
   for (int i = 0; i < 16; ++i) {
     lo = fminf(lo, x[i]);
     hi = fmaxf(hi, x[i]);
-    bad += x[i] * 0.f;  // NaN as soon as one element is no finite number
+    bad = fmaf(x[i], 0.f, bad);  // NaN as soon as one element is no finite number
   }
   const uint32_t lanes = 0xFFu << (threadIdx.x & 24);
 #pragma unroll
@@ -67,15 +71,34 @@ __global__ void write_kernel(const T* __restrict__ c, int64_t ld_c, const uint16
   }
   const float range = __fsub_rn(hi, lo);
   float scale = fabsf(range) <= 1e-8f ? 1.f : __fdiv_rn(range, kTop);
-  uint32_t w[2] = {0, 0};
+  const float inv = __fdiv_rn(1.f, scale);
+  float code[16], off = 0.f;
 #pragma unroll
   for (int i = 0; i < 16; ++i) {
-    const float code = fminf(fmaxf(rintf(__fdiv_rn(__fsub_rn(x[i], lo), scale)), 0.f), kTop);
-    w[i / 8] |= static_cast<uint32_t>(code) << (4 * (i % 8));
+    const float quotient = __fmul_rn(__fsub_rn(x[i], lo), inv);
+    code[i] = __fsub_rn(__fadd_rn(quotient, 12582912.f), 12582912.f);  // the nearest whole number, halves to even
+    off = fmaxf(off, fabsf(__fsub_rn(quotient, code[i])));
+  }
+  if (!(off <= 0.4999f)) {
+#pragma unroll
+    for (int i = 0; i < 16; ++i) code[i] = rintf(__fdiv_rn(__fsub_rn(x[i], lo), scale));
+  }
+  uint32_t w[2];
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    float half[2];  // four codes as one whole number below 2^16
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      const float* v = code + 8 * h + 4 * k;
+      half[k] = 0.f;
+#pragma unroll
+      for (int i = 3; i >= 0; --i) half[k] = fmaf(half[k], 16.f, fminf(fmaxf(v[i], 0.f), kTop));
+    }
+    w[h] = static_cast<uint32_t>(half[0]) | static_cast<uint32_t>(half[1]) << 16;
   }
   if (bad != 0.f) scale = __int_as_float(0x7FC00000);
-  *reinterpret_cast<uint2*>(cache.codes + slot * (cache.latent_dim / 2) + g * 64 + part * 8) = make_uint2(w[0], w[1]);
-  if (part == 0) reinterpret_cast<float2*>(cache.params)[slot * ng + g] = make_float2(scale, __fdiv_rn(-lo, scale));
+  *reinterpret_cast<uint2*>(cache.codes + slot * (NG * 64) + g * 64 + part * 8) = make_uint2(w[0], w[1]);
+  if (part == 0) reinterpret_cast<float2*>(cache.params)[slot * NG + g] = make_float2(scale, __fdiv_rn(-lo, scale));
 }
 
 __device__ __forceinline__ void store8(float* p, const float (&v)[8]) {
@@ -87,70 +110,141 @@ __device__ __forceinline__ void store8(uint16_t* p, const float (&v)[8]) {
       make_uint4(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]), pack_bf16x2(v[4], v[5]), pack_bf16x2(v[6], v[7]));
 }
 
-// One thread per 8 elements of a row (a word of codes), and per 8 elements of its rotary part.
-template <typename T>
-__global__ void read_kernel(rolaq_int4_cache cache, const void* slots, int slots64, int64_t n, T* __restrict__ out,
-                            int64_t ld_out, uint16_t* __restrict__ out_pe, int64_t ld_pe, int32_t* err) {
-  const int words = cache.latent_dim / 8, all = words + (out_pe ? cache.rope_dim / 8 : 0);
-  const int64_t unit = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x;
-  const int64_t row = unit / all;
-  const int k = static_cast<int>(unit % all);
+// Eight threads per unit, a unit as in write_kernel: a thread reads the words of 8 elements at 8 part and at 64 + 8 part
+// of its group, so that a warp's stores are whole lines.
+template <typename T, int NG>
+__global__ void __launch_bounds__(256) read_kernel(rolaq_int4_cache cache, const void* slots, int slots64, int64_t n,
+                                                   T* __restrict__ out, int64_t ld_out, uint16_t* __restrict__ out_pe,
+                                                   int64_t ld_pe, int32_t* err) {
+  const uint32_t unit = (blockIdx.x * 256u + threadIdx.x) / 8;
+  const int part = threadIdx.x & 7;
+  const int64_t row = unit / (NG + 1);
+  const int g = unit % (NG + 1);
   if (row >= n) return;
   const int64_t slot = load_index(slots, slots64, row);
   const bool ok = slot >= 0 && slot < cache.num_slots;
-  if (!ok && k == 0) report(err, ROLAQ_DEV_BAD_SLOT);
-  if (k >= words) {
-    const int j = 8 * (k - words);
-    *reinterpret_cast<uint4*>(out_pe + row * ld_pe + j) =
-        ok ? *reinterpret_cast<const uint4*>(cache.rope + slot * cache.rope_dim + j) : make_uint4(0, 0, 0, 0);
+  if (!ok && g == 0 && part == 0) report(err, ROLAQ_DEV_BAD_SLOT);
+  if (g == NG) {
+    if (out_pe != nullptr && part * 8 < cache.rope_dim)
+      *reinterpret_cast<uint4*>(out_pe + row * ld_pe + part * 8) =
+          ok ? *reinterpret_cast<const uint4*>(cache.rope + slot * cache.rope_dim + part * 8) : make_uint4(0, 0, 0, 0);
     return;
   }
-  float v[8] = {};
+  uint32_t w[2] = {0, 0};
+  float2 p = make_float2(0.f, 0.f);
   if (ok) {
-    const uint32_t w = reinterpret_cast<const uint32_t*>(cache.codes)[slot * words + k];
-    const float2 p = reinterpret_cast<const float2*>(cache.params)[slot * (cache.latent_dim / kGroup) + k / 16];
-#pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = value((w >> (4 * i)) & 15u, p.x, p.y);
+    const uint32_t* src = reinterpret_cast<const uint32_t*>(cache.codes + slot * (NG * 64) + g * 64) + part;
+    w[0] = src[0], w[1] = src[8];
+    p = reinterpret_cast<const float2*>(cache.params)[slot * NG + g];
   }
-  store8(out + row * ld_out + 8 * k, v);
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    float v[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = ok ? value((w[h] >> (4 * i)) & 15u, p.x, p.y) : 0.f;
+    store8(out + row * ld_out + g * kGroup + 64 * h + 8 * part, v);
+  }
 }
 
-// One CTA per page, a column at a time per thread.
-__global__ void boxes_kernel(rolaq_int4_cache cache, const int32_t* __restrict__ pages,
-                             const int32_t* __restrict__ counts, int32_t* err) {
-  __shared__ float tops[2][32];
-  const int d = cache.latent_dim, w = d + cache.rope_dim, ng = d / kGroup;
+// The minimum and maximum of a word's 8 codes' values over the tokens of a CTA's share, in 32-bit steps that are
+// value()'s: codes become floats by one OR under 2^23 (their place in the word a power of 16) and one exact FMA.
+__device__ __forceinline__ void widen(uint32_t w, float scale, float zero, float (&lo)[8], float (&hi)[8]) {
+  const uint32_t high = w >> 12;  // codes 5, 6 and 7 at places 2, 3 and 4
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const int place = i < 5 ? i : i - 3;
+    const float at = 1.f / static_cast<float>(1 << (4 * place));
+    const float code = fmaf(__uint_as_float(((i < 5 ? w : high) & (15u << (4 * place))) | 0x4B000000u), at, -8388608.f * at);
+    const float v = __fmul_rn(__fsub_rn(code, zero), scale);
+    lo[i] = fminf(lo[i], v);
+    hi[i] = fmaxf(hi[i], v);
+  }
+}
+
+// One CTA per page: a thread takes a word (8 columns) of every (512 * 8 / W)-th token, the CTA joins them through
+// shared memory.  Bound by memory for whole pages: seven operations an element, 64 KB of a page in flight on an SM.
+template <int D, int DR>
+__global__ void __launch_bounds__(256) boxes_kernel(rolaq_int4_cache cache, const int32_t* __restrict__ pages,
+                                                    const int32_t* __restrict__ counts, int32_t* err) {
+  constexpr int W = D + DR, NG = D / kGroup, WORDS = D / 8, SHARES = 256 / WORDS, EACH = kPage / SHARES;
+  constexpr int RWORDS = DR / 8, RSHARES = 256 / RWORDS, REACH = kPage / RSHARES;  // the rotary part: 8 columns of 16 bits
+  __shared__ __align__(16) float box[2][SHARES][D], rope_box[2][8][DR];  // low and high; the rotary part by warps
+  __shared__ float tops[2][8];
+  const int tid = threadIdx.x, warp = tid / 32, lane = tid & 31;
   const int64_t page = pages[blockIdx.x];
   const int count = counts[blockIdx.x];
   if (page < 0 || page >= cache.num_slots / kPage || count < 1 || count > kPage) {
-    if (threadIdx.x == 0) report(err, ROLAQ_DEV_BAD_PAGE);
+    if (tid == 0) report(err, ROLAQ_DEV_BAD_PAGE);
     return;
   }
-  float lo[3], hi[3], top[2] = {0.f, 0.f};
+  {
+    const int word = tid % WORDS, share = tid / WORDS;
+    const uint32_t* codes = reinterpret_cast<const uint32_t*>(cache.codes) + (page * kPage + share) * WORDS + word;
+    const float2* params = reinterpret_cast<const float2*>(cache.params) + (page * kPage + share) * NG + word / 16;
+    float lo[8], hi[8];
 #pragma unroll
-  for (int k = 0; k < 3; ++k) {
-    const int col = threadIdx.x + 256 * k;
+    for (int i = 0; i < 8; ++i) lo[i] = INFINITY, hi[i] = -INFINITY;
+    uint32_t w[EACH];
+    float2 p[EACH];
+#pragma unroll
+    for (int k = 0; k < EACH; ++k)
+      if (share + k * SHARES < count) w[k] = codes[k * SHARES * WORDS], p[k] = params[k * SHARES * NG];
+#pragma unroll
+    for (int k = 0; k < EACH; ++k)
+      if (share + k * SHARES < count) widen(w[k], p[k].x, p[k].y, lo, hi);
+    store8(&box[0][share][8 * word], lo);
+    store8(&box[1][share][8 * word], hi);
+  }
+  {
+    const int word = tid % RWORDS, share = tid / RWORDS;
+    float lo[8], hi[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) lo[i] = INFINITY, hi[i] = -INFINITY;
+#pragma unroll
+    for (int k = 0; k < REACH; ++k) {
+      const int t = share + k * RSHARES;
+      if (t >= count) continue;
+      const uint4 v = *reinterpret_cast<const uint4*>(cache.rope + (page * kPage + t) * DR + 8 * word);
+      const uint32_t u[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        lo[2 * i] = fminf(lo[2 * i], bf16_lo(u[i])), hi[2 * i] = fmaxf(hi[2 * i], bf16_lo(u[i]));
+        lo[2 * i + 1] = fminf(lo[2 * i + 1], bf16_hi(u[i])), hi[2 * i + 1] = fmaxf(hi[2 * i + 1], bf16_hi(u[i]));
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {  // over the warp's tokens
+#pragma unroll
+      for (int o = RWORDS; o < 32; o *= 2) {
+        lo[i] = fminf(lo[i], __shfl_xor_sync(0xFFFFFFFFu, lo[i], o));
+        hi[i] = fmaxf(hi[i], __shfl_xor_sync(0xFFFFFFFFu, hi[i], o));
+      }
+      if (lane < RWORDS) rope_box[0][warp][8 * word + i] = lo[i], rope_box[1][warp][8 * word + i] = hi[i];
+    }
+  }
+  __syncthreads();
+  constexpr int COLS = (W + 255) / 256;
+  float lo[COLS], hi[COLS], top[2] = {0.f, 0.f};
+#pragma unroll
+  for (int k = 0; k < COLS; ++k) {
+    const int col = tid + 256 * k;
     lo[k] = INFINITY;
     hi[k] = -INFINITY;
-    if (col >= w) continue;
-    for (int t = 0; t < count; ++t) {
-      const int64_t slot = page * kPage + t;
-      float v;
-      if (col < d) {
-        const float2 p = reinterpret_cast<const float2*>(cache.params)[slot * ng + col / kGroup];
-        v = value((cache.codes[slot * (d / 2) + col / 2] >> (4 * (col & 1))) & 15u, p.x, p.y);
-      } else {
-        v = bf16_lo(cache.rope[slot * cache.rope_dim + col - d]);
-      }
-      lo[k] = fminf(lo[k], v);
-      hi[k] = fmaxf(hi[k], v);
+    if (col < D) {
+#pragma unroll
+      for (int s = 0; s < SHARES; ++s) lo[k] = fminf(lo[k], box[0][s][col]), hi[k] = fmaxf(hi[k], box[1][s][col]);
+    } else if (col < W) {
+#pragma unroll
+      for (int s = 0; s < 8; ++s) lo[k] = fminf(lo[k], rope_box[0][s][col - D]), hi[k] = fmaxf(hi[k], rope_box[1][s][col - D]);
+    } else {
+      continue;
     }
-    top[col >= d] = fmaxf(top[col >= d], fmaxf(fabsf(lo[k]), fabsf(hi[k])));
+    top[col >= D] = fmaxf(top[col >= D], fmaxf(fabsf(lo[k]), fabsf(hi[k])));
   }
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
     top[i] = warp_max_f32(top[i]);
-    if ((threadIdx.x & 31) == 0) tops[i][threadIdx.x / 32] = top[i];
+    if (lane == 0) tops[i][warp] = top[i];
   }
   __syncthreads();
   int e[2];
@@ -159,17 +253,17 @@ __global__ void boxes_kernel(rolaq_int4_cache cache, const int32_t* __restrict__
     float m = 0.f;
     for (int k = 0; k < 8; ++k) m = fmaxf(m, tops[i][k]);
     e[i] = unit_exponent(m);
-    if (threadIdx.x == 0) cache.box_exps[page * 2 + i] = e[i];
+    if (tid == 0) cache.box_exps[page * 2 + i] = e[i];
   }
 #pragma unroll
-  for (int k = 0; k < 3; ++k) {
-    const int col = threadIdx.x + 256 * k;
-    if (col >= w) continue;
-    const float inv = pow2(-e[col >= d]);
+  for (int k = 0; k < COLS; ++k) {
+    const int col = tid + 256 * k;
+    if (col >= W) continue;
+    const float inv = pow2(-e[col >= D]);
     const float center = rintf(__fmul_rn(__fmul_rn(__fadd_rn(lo[k], hi[k]), 0.5f), inv));
     const float radius = ceilf(fmaxf(__fsub_rn(__fmul_rn(hi[k], inv), center), __fsub_rn(center, __fmul_rn(lo[k], inv))));
-    cache.box_center[page * w + col] = static_cast<int8_t>(static_cast<int>(fminf(fmaxf(center, -127.f), 127.f)));
-    cache.box_radius[page * w + col] = static_cast<uint8_t>(static_cast<int>(fminf(fmaxf(radius, 0.f), 255.f)));
+    cache.box_center[page * W + col] = static_cast<int8_t>(static_cast<int>(fminf(fmaxf(center, -127.f), 127.f)));
+    cache.box_radius[page * W + col] = static_cast<uint8_t>(static_cast<int>(fminf(fmaxf(radius, 0.f), 255.f)));
   }
 }
 
@@ -205,27 +299,49 @@ int status() { return cudaGetLastError() == cudaSuccess ? ROLAQ_OK : ROLAQ_ECUDA
 
 int launch_write(const void* c, bool f32, int64_t ld_c, const uint16_t* k_pe, int64_t ld_pe, const void* slots,
                  int slots64, int64_t n, const rolaq_int4_cache& cache, int32_t* err, cudaStream_t s) {
-  const unsigned grid = blocks_for(n * (cache.latent_dim / kGroup + 1) * 8, 256);
-  if (f32)
-    write_kernel<<<grid, 256, 0, s>>>(static_cast<const float*>(c), ld_c, k_pe, ld_pe, slots, slots64, n, cache, err);
-  else
-    write_kernel<<<grid, 256, 0, s>>>(static_cast<const uint16_t*>(c), ld_c, k_pe, ld_pe, slots, slots64, n, cache, err);
+  const int ng = cache.latent_dim / kGroup;
+  // 32 bits of units a launch
+  const int64_t most = (int64_t(1) << 31) / (8 * (ng + 1)) / 256 * 256;
+  for (int64_t at = 0; at < n; at += most) {
+    const int64_t rows = std::min(n - at, most);
+    const unsigned grid = blocks_for(rows * (ng + 1) * 8, 256);
+    const void* sl = static_cast<const char*>(slots) + at * (slots64 ? 8 : 4);
+    auto go = [&](auto kernel, auto* src) {
+      kernel<<<grid, 256, 0, s>>>(src + at * ld_c, ld_c, k_pe + at * ld_pe, ld_pe, sl, slots64, rows, cache, err);
+    };
+    if (f32 && ng == 4) go(write_kernel<float, 4>, static_cast<const float*>(c));
+    else if (f32) go(write_kernel<float, 2>, static_cast<const float*>(c));
+    else if (ng == 4) go(write_kernel<uint16_t, 4>, static_cast<const uint16_t*>(c));
+    else go(write_kernel<uint16_t, 2>, static_cast<const uint16_t*>(c));
+  }
   return status();
 }
 
 int launch_read(const rolaq_int4_cache& cache, const void* slots, int slots64, int64_t n, void* out, bool f32,
                 int64_t ld_out, uint16_t* out_pe, int64_t ld_pe, int32_t* err, cudaStream_t s) {
-  const unsigned grid = blocks_for(n * (cache.latent_dim / 8 + (out_pe ? cache.rope_dim / 8 : 0)), 256);
-  if (f32)
-    read_kernel<<<grid, 256, 0, s>>>(cache, slots, slots64, n, static_cast<float*>(out), ld_out, out_pe, ld_pe, err);
-  else
-    read_kernel<<<grid, 256, 0, s>>>(cache, slots, slots64, n, static_cast<uint16_t*>(out), ld_out, out_pe, ld_pe, err);
+  const int ng = cache.latent_dim / kGroup;
+  const int64_t most = (int64_t(1) << 31) / (8 * (ng + 1)) / 256 * 256;
+  for (int64_t at = 0; at < n; at += most) {
+    const int64_t rows = std::min(n - at, most);
+    const unsigned grid = blocks_for(rows * (ng + 1) * 8, 256);
+    const void* sl = static_cast<const char*>(slots) + at * (slots64 ? 8 : 4);
+    uint16_t* pe = out_pe ? out_pe + at * ld_pe : nullptr;
+    auto go = [&](auto kernel, auto* dst) {
+      kernel<<<grid, 256, 0, s>>>(cache, sl, slots64, rows, dst + at * ld_out, ld_out, pe, ld_pe, err);
+    };
+    if (f32 && ng == 4) go(read_kernel<float, 4>, static_cast<float*>(out));
+    else if (f32) go(read_kernel<float, 2>, static_cast<float*>(out));
+    else if (ng == 4) go(read_kernel<uint16_t, 4>, static_cast<uint16_t*>(out));
+    else go(read_kernel<uint16_t, 2>, static_cast<uint16_t*>(out));
+  }
   return status();
 }
 
 int launch_update_boxes(const rolaq_int4_cache& cache, const int32_t* pages, const int32_t* counts, int64_t n,
                         int32_t* err, cudaStream_t s) {
-  boxes_kernel<<<static_cast<unsigned>(n), 256, 0, s>>>(cache, pages, counts, err);
+  const auto kernel = cache.latent_dim == 512 ? (cache.rope_dim == 64 ? boxes_kernel<512, 64> : boxes_kernel<512, 32>)
+                                              : (cache.rope_dim == 64 ? boxes_kernel<256, 64> : boxes_kernel<256, 32>);
+  kernel<<<static_cast<unsigned>(n), 256, 0, s>>>(cache, pages, counts, err);
   return status();
 }
 

@@ -66,7 +66,7 @@ class Int4View:
         _lib.require_device(codes)
         self.codes, self.params, self.rope, self.boxes = codes, params, rope, boxes
         self.latent_dim, self.rope_dim, self.num_slots = d, rope.shape[1], slots
-        self.device = codes.device
+        self.device, self.index = codes.device, codes.get_device()
         ptrs = [t.data_ptr() for t in tensors] + [None] * (6 - len(tensors))
         self._c = _lib.Int4Cache(*ptrs, slots, d, rope.shape[1])
         self._ref = ctypes.addressof(self._c)
@@ -87,17 +87,18 @@ class Workspace:
         self.sel_lens = torch.zeros(batch, dtype=_I32, device=view.device)
 
 
-def _stream(t: torch.Tensor, *others) -> int:
-    """The current stream of the tensors' device, which has to be the current device."""
-    dev = t.device
-    for o in others:
-        if o is not None and o.device != dev:
-            raise ValueError(f"tensors on {dev} and {o.device}: one device is needed")
-    if dev.type != "cuda":
-        raise ValueError("the 4-bit cache kernels run on CUDA tensors only (no CPU fallback)")
-    if dev.index != torch.cuda.current_device():
-        raise ValueError(f"tensors are on {dev}, the current device is cuda:{torch.cuda.current_device()}")
-    return torch.cuda.current_stream(dev).cuda_stream
+_raw_stream = torch._C._cuda_getCurrentRawStream  # torch.cuda.current_stream(d).cuda_stream without its object
+_current_device = torch.cuda.current_device
+
+
+def _stream(index: int, *tensors) -> int:
+    """The current stream of device ``index``, on which all of ``tensors`` and which the current device have to be."""
+    for t in tensors:
+        if t is not None and t.get_device() != index:
+            raise ValueError(f"tensors on cuda:{index} and {t.device}: one device is needed")
+    if index != _current_device():
+        raise ValueError(f"the cache is on cuda:{index}, the current device is cuda:{_current_device()}")
+    return _raw_stream(index)
 
 
 def _need(t: torch.Tensor, name: str, dtype, ndim: int) -> None:
@@ -108,7 +109,7 @@ def _need(t: torch.Tensor, name: str, dtype, ndim: int) -> None:
 
 
 def _rows(t: torch.Tensor, name: str, n: int, width: int) -> None:
-    if t.dim() != 2 or t.shape[0] != n or t.shape[1] != width:
+    if t.shape != (n, width):
         raise ValueError(f"{name} must be [{n}, {width}], got {tuple(t.shape)}")
     if t.stride(1) != 1:
         raise ValueError(f"{name} rows must be contiguous")
@@ -142,7 +143,7 @@ def write(view: Int4View, c: torch.Tensor, k_pe: torch.Tensor, slots: torch.Tens
     _rows(c, "c", n, view.latent_dim)
     _rows(k_pe, "k_pe", n, view.rope_dim)
     _lib.call("rolaq_int4_write", c.data_ptr(), c.dtype == _F32, c.stride(0), k_pe.data_ptr(), k_pe.stride(0),
-              slots.data_ptr(), is64, n, view._ref, _err(err), _stream(c, k_pe, slots, view, err))
+              slots.data_ptr(), is64, n, view._ref, _err(err), _stream(view.index, c, k_pe, slots, err))
 
 
 def read(view: Int4View, slots: torch.Tensor, out: torch.Tensor, out_pe: torch.Tensor | None = None,
@@ -159,7 +160,7 @@ def read(view: Int4View, slots: torch.Tensor, out: torch.Tensor, out_pe: torch.T
         _rows(out_pe, "out_pe", n, view.rope_dim)
     _lib.call("rolaq_int4_read", view._ref, slots.data_ptr(), is64, n, out.data_ptr(), out.dtype == _F32, out.stride(0),
               None if out_pe is None else out_pe.data_ptr(), 0 if out_pe is None else out_pe.stride(0), _err(err),
-              _stream(out, out_pe, slots, view, err))
+              _stream(view.index, out, out_pe, slots, err))
 
 
 def _pages(t: torch.Tensor, name: str, n: int | None = None) -> int:
@@ -174,7 +175,7 @@ def update_boxes(view: Int4View, pages: torch.Tensor, counts: torch.Tensor, err:
     n = _pages(pages, "pages")
     _pages(counts, "counts", n)
     _lib.call("rolaq_int4_update_boxes", view._ref, pages.data_ptr(), counts.data_ptr(), n, _err(err),
-              _stream(pages, counts, view, err))
+              _stream(view.index, pages, counts, err))
 
 
 def read_boxes(view: Int4View, pages: torch.Tensor, lo: torch.Tensor, hi: torch.Tensor,
@@ -188,18 +189,22 @@ def read_boxes(view: Int4View, pages: torch.Tensor, lo: torch.Tensor, hi: torch.
     if lo.stride(0) != hi.stride(0):
         raise ValueError("lo and hi must share the row stride")
     _lib.call("rolaq_int4_read_boxes", view._ref, pages.data_ptr(), n, lo.data_ptr(), hi.data_ptr(), lo.stride(0),
-              _err(err), _stream(pages, lo, hi, view, err))
+              _err(err), _stream(view.index, pages, lo, hi, err))
 
 
-def _requests(q, view, page_table, seq_lens, b):
-    if q.dtype != _BF16 or q.shape[-1] != view.latent_dim + view.rope_dim or q.stride(-1) != 1:
+def _requests(shape, q, view, page_table, seq_lens) -> tuple[int, int]:
+    """Checks what the attention and the selection share; the page table's row stride and width."""
+    b = shape[0]
+    if q.dtype != _BF16 or shape[-1] != view.latent_dim + view.rope_dim or q.stride(-1) != 1:
         raise ValueError("q must be bfloat16 [B, T, H, D + Dr] or [B, H, D + Dr] with contiguous rows")
     if page_table.dtype != _I32 or seq_lens.dtype != _I32:
         raise TypeError("page_table and seq_lens must be int32")
-    if page_table.dim() != 2 or page_table.shape[0] != b or (page_table.shape[1] > 1 and page_table.stride(1) != 1):
+    table = page_table.shape
+    if len(table) != 2 or table[0] != b or (table[1] > 1 and page_table.stride(1) != 1):
         raise ValueError("page_table must be [B, max_pages] with contiguous rows")
-    if seq_lens.dim() != 1 or seq_lens.shape[0] != b or not seq_lens.is_contiguous():
+    if seq_lens.shape != (b,) or not seq_lens.is_contiguous():
         raise ValueError("seq_lens must be contiguous [B]")
+    return page_table.stride(0), table[1]
 
 
 def decode(q: torch.Tensor, view: Int4View, page_table: torch.Tensor, seq_lens: torch.Tensor, sm_scale: float,
@@ -207,24 +212,27 @@ def decode(q: torch.Tensor, view: Int4View, page_table: torch.Tensor, seq_lens: 
     """Attention of ``q`` (bf16 ``[B, H, D + Dr]``, or ``[B, T, H, D + Dr]`` for the last T tokens of each request,
     causal among themselves) over the requests' tokens: ``out`` bf16 ``[B, (T,) H, D]``, ``lse`` f32 ``[B, (T,) H]``
     (natural log, or None).  Rows that see no token get 0 and -inf."""
-    if q.dim() == 3:
-        b, h, _ = q.shape
-        t, q_st, o_st = 1, 0, 0
-    elif q.dim() == 4:
-        b, t, h, _ = q.shape
-        q_st = q.stride(1)
-        o_st = out.stride(1) if out.dim() == 4 else 0
+    shape = q.shape
+    if len(shape) == 4:
+        b, t, h, _ = shape
+        q_sb, q_st, q_sh, _ = q.stride()
+    elif len(shape) == 3:
+        b, h, _ = shape
+        q_sb, q_sh, _ = q.stride()
+        t, q_st = 1, 0
     else:
         raise ValueError("q must be [B, H, D + Dr] or [B, T, H, D + Dr]")
-    _requests(q, view, page_table, seq_lens, b)
-    if out.dtype != _BF16 or out.shape[:-1] != q.shape[:-1] or out.shape[-1] != view.latent_dim or out.stride(-1) != 1:
+    pt_stride, max_pages = _requests(shape, q, view, page_table, seq_lens)
+    if out.dtype != _BF16 or out.shape != (*shape[:-1], view.latent_dim) or out.stride(-1) != 1:
         raise ValueError("out must be bfloat16, q's shape with D columns, with contiguous rows")
-    if lse is not None and (lse.dtype != _F32 or lse.shape != q.shape[:-1] or not lse.is_contiguous()):
+    o_stride = out.stride()
+    if lse is not None and (lse.dtype != _F32 or lse.shape != shape[:-1] or not lse.is_contiguous()):
         raise ValueError("lse must be contiguous float32 of q's shape without the last axis")
-    _lib.call("rolaq_int4_decode", q.data_ptr(), q.stride(0), q_st, q.stride(-2), b, t, h, view._ref,
-              page_table.data_ptr(), page_table.stride(0), page_table.shape[1], seq_lens.data_ptr(), sm_scale, ws._ptr,
-              ws.nbytes, out.data_ptr(), out.stride(0), o_st, out.stride(-2), None if lse is None else lse.data_ptr(),
-              _err(err), _stream(q, view, page_table, seq_lens, out, lse, ws.scratch, err))
+    _lib.call("rolaq_int4_decode", q.data_ptr(), q_sb, q_st, q_sh, b, t, h, view._ref, page_table.data_ptr(), pt_stride,
+              max_pages, seq_lens.data_ptr(), sm_scale, ws._ptr, ws.nbytes, out.data_ptr(), o_stride[0],
+              o_stride[1] if t > 1 or len(shape) == 4 else 0, o_stride[-2], None if lse is None else lse.data_ptr(),
+              None if err is None else _err(err),
+              _stream(view.index, q, page_table, seq_lens, out, lse, ws.scratch, err))
 
 
 def select_pages(q: torch.Tensor, view: Int4View, page_table: torch.Tensor, seq_lens: torch.Tensor, budget: int,
@@ -234,18 +242,19 @@ def select_pages(q: torch.Tensor, view: Int4View, page_table: torch.Tensor, seq_
     as a page table: the first ``keep_first``, the last ``keep_last``, and those whose boxes score highest."""
     if view.boxes is None:
         raise ValueError("the cache has no page boxes")
-    if q.dim() == 4 and q.shape[1] != 1 or q.dim() not in (3, 4):
+    if q.dim() not in (3, 4) or q.dim() == 4 and q.shape[1] != 1:
         raise ValueError("pages are selected for one query token per request: q must be [B, H, D + Dr] or [B, 1, H, D + Dr]")
-    b, h = q.shape[0], q.shape[-2]
-    _requests(q, view, page_table, seq_lens, b)
-    if sel_table.dtype != _I32 or sel_table.dim() != 2 or sel_table.shape[0] != b or sel_table.shape[1] != budget or not sel_table.is_contiguous():
+    shape = q.shape
+    b, h = shape[0], shape[-2]
+    pt_stride, max_pages = _requests(shape, q, view, page_table, seq_lens)
+    if sel_table.dtype != _I32 or sel_table.shape != (b, budget) or not sel_table.is_contiguous():
         raise ValueError("sel_table must be contiguous int32 [B, budget]")
-    if sel_lens.dtype != _I32 or sel_lens.dim() != 1 or sel_lens.shape[0] != b or not sel_lens.is_contiguous():
+    if sel_lens.dtype != _I32 or sel_lens.shape != (b,) or not sel_lens.is_contiguous():
         raise ValueError("sel_lens must be contiguous int32 [B]")
     _lib.call("rolaq_int4_select_pages", q.data_ptr(), q.stride(0), q.stride(-2), b, h, view._ref,
-              page_table.data_ptr(), page_table.stride(0), page_table.shape[1], seq_lens.data_ptr(), budget, keep_first,
+              page_table.data_ptr(), pt_stride, max_pages, seq_lens.data_ptr(), budget, keep_first,
               keep_last, ws._ptr, ws.nbytes, sel_table.data_ptr(), budget, sel_lens.data_ptr(), _err(err),
-              _stream(q, view, page_table, seq_lens, sel_table, sel_lens, ws.scratch, err))
+              _stream(view.index, q, page_table, seq_lens, sel_table, sel_lens, ws.scratch, err))
 
 
 def sparse_decode(q: torch.Tensor, view: Int4View, page_table: torch.Tensor, seq_lens: torch.Tensor, sm_scale: float,
