@@ -139,6 +139,32 @@ __global__ void __launch_bounds__(kThreads) select_kernel(const SelectArgs a, co
   const int p_begin = blockIdx.x * chunk_pages, p_end = min(held, p_begin + chunk_pages);
   if (held <= a.budget || p_begin >= p_end) return;
 
+  // The boxes of the warp's next 8 pages, the lane's part as operands.  The first are on their way while the query
+  // is quantised.
+  const int pool_pages = static_cast<int>(a.cache.num_slots / kPage);
+  uint4 c[STEPS / 2], r[STEPS / 2];
+  uint2 c_end, r_end;
+  int2 e_page;
+  bool ok;
+  auto load_boxes = [&](int p0) {
+    const int id = p0 + g < p_end ? table[p0 + g] : 0;
+    ok = id >= 0 && id < pool_pages;
+    if (!ok && j == 0) report(a.err, ROLAQ_DEV_BAD_PAGE);
+    const int64_t page = ok ? id : 0, at = page * W;
+#pragma unroll
+    for (int s = 0; s < STEPS / 2; ++s) {
+      c[s] = *reinterpret_cast<const uint4*>(a.cache.box_center + at + 64 * s + 16 * j);
+      r[s] = *reinterpret_cast<const uint4*>(a.cache.box_radius + at + 64 * s + 16 * j);
+    }
+    if (DR == 32) {
+      c_end = *reinterpret_cast<const uint2*>(a.cache.box_center + at + D + 8 * j);
+      r_end = *reinterpret_cast<const uint2*>(a.cache.box_radius + at + D + 8 * j);
+    }
+    e_page = *reinterpret_cast<const int2*>(a.cache.box_exps + 2 * page);
+  };
+  const int first = p_begin + warp * kTile;
+  if (first < p_end) load_boxes(first);
+
   // ---- the query in 8 bits, in operand order ----
   const uint16_t* q = a.q + b * a.q_sb;
   float top[2] = {0.f, 0.f};
@@ -193,25 +219,8 @@ __global__ void __launch_bounds__(kThreads) select_kernel(const SelectArgs a, co
 
   // ---- the scores ----
   float* scores = a.scores + static_cast<int64_t>(b) * a.max_pages;
-  const int pool_pages = static_cast<int>(a.cache.num_slots / kPage);
-  for (int p0 = p_begin + warp * kTile; p0 < p_end; p0 += kTile * kWarps) {
-    const int p = p0 + g;  // the lane's page as an operand
-    const int id = p < p_end ? table[p] : 0;
-    const bool ok = id >= 0 && id < pool_pages;
-    if (!ok && j == 0) report(a.err, ROLAQ_DEV_BAD_PAGE);
-    const int64_t at = static_cast<int64_t>(ok ? id : 0) * W;
-    uint4 c[STEPS / 2], r[STEPS / 2];
-    uint2 c_end, r_end;
-#pragma unroll
-    for (int s = 0; s < STEPS / 2; ++s) {
-      c[s] = *reinterpret_cast<const uint4*>(a.cache.box_center + at + 64 * s + 16 * j);
-      r[s] = *reinterpret_cast<const uint4*>(a.cache.box_radius + at + 64 * s + 16 * j);
-    }
-    if (DR == 32) {
-      c_end = *reinterpret_cast<const uint2*>(a.cache.box_center + at + D + 8 * j);
-      r_end = *reinterpret_cast<const uint2*>(a.cache.box_radius + at + D + 8 * j);
-    }
-    const int2 e_page = *reinterpret_cast<const int2*>(a.cache.box_exps + 2 * static_cast<int64_t>(ok ? id : 0));
+  for (int p0 = first; p0 < p_end; p0 += kTile * kWarps) {
+    if (p0 != first) load_boxes(p0);
     // pages 2 j and 2 j + 1 of the tile are the lane's as results
     float unit[2][2];
     bool there[2];

@@ -11,17 +11,17 @@ namespace rolaq {
 namespace i4 {
 namespace {
 
-// 16 consecutive elements of a row as FP32.
-__device__ __forceinline__ void load16(const float* p, float (&x)[16]) {
+// 32 consecutive elements of a row as FP32.
+__device__ __forceinline__ void load32(const float* p, float (&x)[32]) {
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
+  for (int i = 0; i < 8; ++i) {
     const float4 v = reinterpret_cast<const float4*>(p)[i];
     x[4 * i] = v.x, x[4 * i + 1] = v.y, x[4 * i + 2] = v.z, x[4 * i + 3] = v.w;
   }
 }
-__device__ __forceinline__ void load16(const uint16_t* p, float (&x)[16]) {
+__device__ __forceinline__ void load32(const uint16_t* p, float (&x)[32]) {
 #pragma unroll
-  for (int i = 0; i < 2; ++i) {
+  for (int i = 0; i < 4; ++i) {
     const uint4 v = reinterpret_cast<const uint4*>(p)[i];
     const uint32_t w[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
@@ -29,75 +29,79 @@ __device__ __forceinline__ void load16(const uint16_t* p, float (&x)[16]) {
   }
 }
 
-// Eight threads per unit: a unit is one 128-element group of a row (16 elements a thread, min and max over the
-// eight by shuffles) or the row's k_pe.  Bound by memory as long as the 16 divisions of a thread are not: the
-// quotient's rounding is decided by a product with the reciprocal, which is within 2^-20 of the quotient, unless that
-// lies within 1e-4 of a half; then the thread divides.
+// Four threads per unit: a unit is one 128-element group of a row (32 elements a thread, min and max over the four by
+// shuffles) or the row's k_pe.  Bound by memory as long as 32 divisions of a thread are not: the quotient's rounding is
+// decided by a product with the reciprocal, which is within 2^-18 of the quotient, unless that lies within 1e-5 of a
+// half; then the thread divides.
 template <typename T, int NG>
 __global__ void __launch_bounds__(256) write_kernel(const T* __restrict__ c, int64_t ld_c,
                                                     const uint16_t* __restrict__ k_pe, int64_t ld_pe, const void* slots,
                                                     int slots64, int64_t n, rolaq_int4_cache cache, int32_t* err) {
-  const uint32_t unit = (blockIdx.x * 256u + threadIdx.x) / 8;
-  const int part = threadIdx.x & 7;
+  constexpr float kNear = 0.49999f;
+  const uint32_t unit = (blockIdx.x * 256u + threadIdx.x) / 4;
+  const int part = threadIdx.x & 3;
   const int64_t row = unit / (NG + 1);
   const int g = unit % (NG + 1);
-  if (row >= n) return;  // whole groups of eight threads leave together
+  if (row >= n) return;  // whole groups of four threads leave together
   const int64_t slot = load_index(slots, slots64, row);
-  if (slot < 0 || slot >= cache.num_slots) {
-    if (part == 0) report(err, ROLAQ_DEV_BAD_SLOT);
-    return;
-  }
+  const bool ok = slot >= 0 && slot < cache.num_slots;
   if (g == NG) {
-    if (part * 8 < cache.rope_dim)
-      *reinterpret_cast<uint4*>(cache.rope + slot * cache.rope_dim + part * 8) =
-          *reinterpret_cast<const uint4*>(k_pe + row * ld_pe + part * 8);
+    if (!ok) {
+      if (part == 0) report(err, ROLAQ_DEV_BAD_SLOT);
+      return;
+    }
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int col = 8 * (part + 4 * i);
+      if (col < cache.rope_dim)
+        *reinterpret_cast<uint4*>(cache.rope + slot * cache.rope_dim + col) =
+            *reinterpret_cast<const uint4*>(k_pe + row * ld_pe + col);
+    }
     return;
   }
-  float x[16];
-  load16(c + row * ld_c + g * kGroup + part * 16, x);
+  float x[32];  // on its way together with the slot
+  load32(c + row * ld_c + g * kGroup + part * 32, x);
   float lo = x[0], hi = x[0], bad = 0.f;
 #pragma unroll
-  for (int i = 0; i < 16; ++i) {
+  for (int i = 0; i < 32; ++i) {
     lo = fminf(lo, x[i]);
     hi = fmaxf(hi, x[i]);
     bad = fmaf(x[i], 0.f, bad);  // NaN as soon as one element is no finite number
   }
-  const uint32_t lanes = 0xFFu << (threadIdx.x & 24);
+  const uint32_t lanes = 0xFu << (threadIdx.x & 28);
 #pragma unroll
-  for (int o = 1; o < 8; o *= 2) {
+  for (int o = 1; o < 4; o *= 2) {
     lo = fminf(lo, __shfl_xor_sync(lanes, lo, o));
     hi = fmaxf(hi, __shfl_xor_sync(lanes, hi, o));
     bad += __shfl_xor_sync(lanes, bad, o);
   }
   const float range = __fsub_rn(hi, lo);
   float scale = fabsf(range) <= 1e-8f ? 1.f : __fdiv_rn(range, kTop);
-  const float inv = __fdiv_rn(1.f, scale);
-  float code[16], off = 0.f;
+  const float inv = __fdividef(1.f, scale);
+  uint32_t w[4];
 #pragma unroll
-  for (int i = 0; i < 16; ++i) {
-    const float quotient = __fmul_rn(__fsub_rn(x[i], lo), inv);
-    code[i] = __fsub_rn(__fadd_rn(quotient, 12582912.f), 12582912.f);  // the nearest whole number, halves to even
-    off = fmaxf(off, fabsf(__fsub_rn(quotient, code[i])));
-  }
-  if (!(off <= 0.4999f)) {
+  for (int k = 0; k < 4; ++k) {  // a word of 8 codes
+    float code[8], off = 0.f;
 #pragma unroll
-    for (int i = 0; i < 16; ++i) code[i] = rintf(__fdiv_rn(__fsub_rn(x[i], lo), scale));
-  }
-  uint32_t w[2];
-#pragma unroll
-  for (int h = 0; h < 2; ++h) {
-    float half[2];  // four codes as one whole number below 2^16
-#pragma unroll
-    for (int k = 0; k < 2; ++k) {
-      const float* v = code + 8 * h + 4 * k;
-      half[k] = 0.f;
-#pragma unroll
-      for (int i = 3; i >= 0; --i) half[k] = fmaf(half[k], 16.f, fminf(fmaxf(v[i], 0.f), kTop));
+    for (int i = 0; i < 8; ++i) {
+      const float quotient = __fmul_rn(__fsub_rn(x[8 * k + i], lo), inv);
+      code[i] = __fsub_rn(__fadd_rn(quotient, 12582912.f), 12582912.f);  // the nearest whole number, halves to even
+      off = fmaxf(off, fabsf(__fsub_rn(quotient, code[i])));
     }
-    w[h] = static_cast<uint32_t>(half[0]) | static_cast<uint32_t>(half[1]) << 16;
+    if (off > kNear) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) code[i] = rintf(__fdiv_rn(__fsub_rn(x[8 * k + i], lo), scale));
+    }
+    float half[2];  // four codes as one whole number below 2^16 (0 <= code <= 15: lo and hi are the group's own)
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+      half[h] = fmaf(fmaf(fmaf(code[4 * h + 3], 16.f, code[4 * h + 2]), 16.f, code[4 * h + 1]), 16.f, code[4 * h]);
+    // under 2^23 a whole number is the float's low bits
+    w[k] = (__float_as_uint(half[0] + 8388608.f) & 0xFFFFu) | __float_as_uint(half[1] + 8388608.f) << 16;
   }
   if (bad != 0.f) scale = __int_as_float(0x7FC00000);
-  *reinterpret_cast<uint2*>(cache.codes + slot * (NG * 64) + g * 64 + part * 8) = make_uint2(w[0], w[1]);
+  if (!ok) return;
+  *reinterpret_cast<uint4*>(cache.codes + slot * (NG * 64) + g * 64 + part * 16) = make_uint4(w[0], w[1], w[2], w[3]);
   if (part == 0) reinterpret_cast<float2*>(cache.params)[slot * NG + g] = make_float2(scale, __fdiv_rn(-lo, scale));
 }
 
@@ -110,40 +114,60 @@ __device__ __forceinline__ void store8(uint16_t* p, const float (&v)[8]) {
       make_uint4(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]), pack_bf16x2(v[4], v[5]), pack_bf16x2(v[6], v[7]));
 }
 
-// Eight threads per unit, a unit as in write_kernel: a thread reads the words of 8 elements at 8 part and at 64 + 8 part
-// of its group, so that a warp's stores are whole lines.
+// Eight threads per unit, a unit as in write_kernel, and two rows a thread, `apart` rows from each other, so that
+// twice as much is under way: a thread reads the words of 8 elements at 8 part and at 64 + 8 part of its group, so
+// that a warp's stores are whole lines.
 template <typename T, int NG>
 __global__ void __launch_bounds__(256) read_kernel(rolaq_int4_cache cache, const void* slots, int slots64, int64_t n,
-                                                   T* __restrict__ out, int64_t ld_out, uint16_t* __restrict__ out_pe,
-                                                   int64_t ld_pe, int32_t* err) {
+                                                   int64_t apart, T* __restrict__ out, int64_t ld_out,
+                                                   uint16_t* __restrict__ out_pe, int64_t ld_pe, int32_t* err) {
   const uint32_t unit = (blockIdx.x * 256u + threadIdx.x) / 8;
   const int part = threadIdx.x & 7;
-  const int64_t row = unit / (NG + 1);
   const int g = unit % (NG + 1);
-  if (row >= n) return;
-  const int64_t slot = load_index(slots, slots64, row);
-  const bool ok = slot >= 0 && slot < cache.num_slots;
-  if (!ok && g == 0 && part == 0) report(err, ROLAQ_DEV_BAD_SLOT);
+  if (unit / (NG + 1) >= apart) return;
+  int64_t row[2], slot[2];
+  bool ok[2];
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    row[i] = unit / (NG + 1) + i * apart;
+    slot[i] = row[i] < n ? load_index(slots, slots64, row[i]) : 0;
+  }
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    ok[i] = row[i] < n && slot[i] >= 0 && slot[i] < cache.num_slots;
+    if (row[i] < n && !ok[i] && g == 0 && part == 0) report(err, ROLAQ_DEV_BAD_SLOT);
+  }
   if (g == NG) {
-    if (out_pe != nullptr && part * 8 < cache.rope_dim)
-      *reinterpret_cast<uint4*>(out_pe + row * ld_pe + part * 8) =
-          ok ? *reinterpret_cast<const uint4*>(cache.rope + slot * cache.rope_dim + part * 8) : make_uint4(0, 0, 0, 0);
+    if (out_pe == nullptr || part * 8 >= cache.rope_dim) return;
+    uint4 v[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+      v[i] = ok[i] ? *reinterpret_cast<const uint4*>(cache.rope + slot[i] * cache.rope_dim + part * 8) : make_uint4(0, 0, 0, 0);
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+      if (row[i] < n) *reinterpret_cast<uint4*>(out_pe + row[i] * ld_pe + part * 8) = v[i];
     return;
   }
-  uint32_t w[2] = {0, 0};
-  float2 p = make_float2(0.f, 0.f);
-  if (ok) {
-    const uint32_t* src = reinterpret_cast<const uint32_t*>(cache.codes + slot * (NG * 64) + g * 64) + part;
-    w[0] = src[0], w[1] = src[8];
-    p = reinterpret_cast<const float2*>(cache.params)[slot * NG + g];
+  uint32_t w[2][2];
+  float2 p[2];
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    if (!ok[i]) continue;
+    const uint32_t* src = reinterpret_cast<const uint32_t*>(cache.codes + slot[i] * (NG * 64) + g * 64) + part;
+    w[i][0] = src[0], w[i][1] = src[8];
+    p[i] = reinterpret_cast<const float2*>(cache.params)[slot[i] * NG + g];
   }
 #pragma unroll
-  for (int h = 0; h < 2; ++h) {
-    float v[8];
+  for (int i = 0; i < 2; ++i)
+    if (row[i] < n) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = ok ? value((w[h] >> (4 * i)) & 15u, p.x, p.y) : 0.f;
-    store8(out + row * ld_out + g * kGroup + 64 * h + 8 * part, v);
-  }
+      for (int h = 0; h < 2; ++h) {
+        float v[8];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) v[k] = ok[i] ? value((w[i][h] >> (4 * k)) & 15u, p[i].x, p[i].y) : 0.f;
+        store8(out + row[i] * ld_out + g * kGroup + 64 * h + 8 * part, v);
+      }
+    }
 }
 
 // The minimum and maximum of a word's 8 codes' values over the tokens of a CTA's share, in 32-bit steps that are
@@ -164,7 +188,7 @@ __device__ __forceinline__ void widen(uint32_t w, float scale, float zero, float
 // One CTA per page: a thread takes a word (8 columns) of every (512 * 8 / W)-th token, the CTA joins them through
 // shared memory.  Bound by memory for whole pages: seven operations an element, 64 KB of a page in flight on an SM.
 template <int D, int DR>
-__global__ void __launch_bounds__(256) boxes_kernel(rolaq_int4_cache cache, const int32_t* __restrict__ pages,
+__global__ void __launch_bounds__(256, 4) boxes_kernel(rolaq_int4_cache cache, const int32_t* __restrict__ pages,
                                                     const int32_t* __restrict__ counts, int32_t* err) {
   constexpr int W = D + DR, NG = D / kGroup, WORDS = D / 8, SHARES = 256 / WORDS, EACH = kPage / SHARES;
   constexpr int RWORDS = DR / 8, RSHARES = 256 / RWORDS, REACH = kPage / RSHARES;  // the rotary part: 8 columns of 16 bits
@@ -184,14 +208,23 @@ __global__ void __launch_bounds__(256) boxes_kernel(rolaq_int4_cache cache, cons
     float lo[8], hi[8];
 #pragma unroll
     for (int i = 0; i < 8; ++i) lo[i] = INFINITY, hi[i] = -INFINITY;
-    uint32_t w[EACH];
-    float2 p[EACH];
+    constexpr int AT_ONCE = EACH < 8 ? EACH : 8;
+#pragma unroll 1
+    for (int k0 = 0; k0 < EACH; k0 += AT_ONCE) {
+      uint32_t w[AT_ONCE];
+      float2 p[AT_ONCE];
 #pragma unroll
-    for (int k = 0; k < EACH; ++k)
-      if (share + k * SHARES < count) w[k] = codes[k * SHARES * WORDS], p[k] = params[k * SHARES * NG];
+      for (int k = 0; k < AT_ONCE; ++k) {  // past the count: the share's first token again (share < count), or nothing
+        const int at = share + (k0 + k) * SHARES < count ? k0 + k : 0;
+        w[k] = codes[at * SHARES * WORDS], p[k] = params[at * SHARES * NG];
+      }
 #pragma unroll
-    for (int k = 0; k < EACH; ++k)
-      if (share + k * SHARES < count) widen(w[k], p[k].x, p[k].y, lo, hi);
+      for (int k = 0; k < AT_ONCE; ++k) widen(w[k], p[k].x, p[k].y, lo, hi);
+      if (share >= count) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) lo[i] = INFINITY, hi[i] = -INFINITY;
+      }
+    }
     store8(&box[0][share][8 * word], lo);
     store8(&box[1][share][8 * word], hi);
   }
@@ -301,10 +334,10 @@ int launch_write(const void* c, bool f32, int64_t ld_c, const uint16_t* k_pe, in
                  int slots64, int64_t n, const rolaq_int4_cache& cache, int32_t* err, cudaStream_t s) {
   const int ng = cache.latent_dim / kGroup;
   // 32 bits of units a launch
-  const int64_t most = (int64_t(1) << 31) / (8 * (ng + 1)) / 256 * 256;
+  const int64_t most = (int64_t(1) << 31) / (4 * (ng + 1)) / 256 * 256;
   for (int64_t at = 0; at < n; at += most) {
     const int64_t rows = std::min(n - at, most);
-    const unsigned grid = blocks_for(rows * (ng + 1) * 8, 256);
+    const unsigned grid = blocks_for(rows * (ng + 1) * 4, 256);
     const void* sl = static_cast<const char*>(slots) + at * (slots64 ? 8 : 4);
     auto go = [&](auto kernel, auto* src) {
       kernel<<<grid, 256, 0, s>>>(src + at * ld_c, ld_c, k_pe + at * ld_pe, ld_pe, sl, slots64, rows, cache, err);
@@ -323,11 +356,12 @@ int launch_read(const rolaq_int4_cache& cache, const void* slots, int slots64, i
   const int64_t most = (int64_t(1) << 31) / (8 * (ng + 1)) / 256 * 256;
   for (int64_t at = 0; at < n; at += most) {
     const int64_t rows = std::min(n - at, most);
-    const unsigned grid = blocks_for(rows * (ng + 1) * 8, 256);
+    const int64_t apart = (rows + 1) / 2;
+    const unsigned grid = blocks_for(apart * (ng + 1) * 8, 256);
     const void* sl = static_cast<const char*>(slots) + at * (slots64 ? 8 : 4);
     uint16_t* pe = out_pe ? out_pe + at * ld_pe : nullptr;
     auto go = [&](auto kernel, auto* dst) {
-      kernel<<<grid, 256, 0, s>>>(cache, sl, slots64, rows, dst + at * ld_out, ld_out, pe, ld_pe, err);
+      kernel<<<grid, 256, 0, s>>>(cache, sl, slots64, rows, apart, dst + at * ld_out, ld_out, pe, ld_pe, err);
     };
     if (f32 && ng == 4) go(read_kernel<float, 4>, static_cast<float*>(out));
     else if (f32) go(read_kernel<float, 2>, static_cast<float*>(out));
