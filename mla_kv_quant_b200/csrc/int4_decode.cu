@@ -3,24 +3,23 @@
 // With value (c - z) s of a 4-bit code c, per 128-element group g of a token t:
 //   q . k_t = sum_g s_gt (q_g . c_gt - z_gt sum q_g) + q_pe . k_pe_t
 //   sum_t P_t v_t = sum_t (P_t s_gt) c_gt - sum_t (P_t s_gt) z_gt
-// so both contractions run on the raw codes, which tensor cores take after one AND per register:
-// the FP16 patterns 0..15 and 16 * (0..15) are c 2^-24 and 16 c 2^-24 exactly.  The factor 16 of odd
-// elements is taken out of the query before and out of the result after.  The query is FP16 under a
-// power of two of its row (exact for BF16 within 2^26 of the row's largest element), P s is FP16 (11
-// bits), the rotary part stays BF16; all are m16n8k16 products with FP32 sums.
+// so both contractions run on the raw codes, which become operands by ANDs:
+//   - scores: the E4M3 patterns 0..15 are c 2^-9 exactly.  tcgen05.mma of 128 tokens (codes in TMEM) by the query rows
+//     in two E4M3 terms each (hi + lo: exact for BF16 within 2^10 of the row's largest element, 2^-18 of it below),
+//     one FP32 sum a group; the rotary part BF16 by BF16.  Asynchronous: no warp's issue slots go into it.
+//   - sums: the FP16 patterns 0..255 are that many 2^-24 exactly.  mma.sync m16n8k16 with the codes as rows (c of an
+//     even element, and c + 16 c' of it and the next: c' comes out at the end) and P s in FP16 as columns.
+// All sums are FP32.  mma.sync blocks a scheduler's other warps while it runs (8 cycles each, measured), so only what
+// tcgen05 could not do with fewer shared-memory bytes - the product that needs the codes transposed - is left to it.
 //
-// Codes are the 16-high side of the products, the query rows (query tokens x heads) the 8-wide side: a CTA holds
-// NH tiles of 8 rows (one or two for D = 512, up to five for D = 256, where 40 heads then are one pass) and
-// walks the pages of one or more requests; a page (64 tokens) is one pipeline stage (TMA, 128-byte swizzle,
-// so that ldmatrix reads without conflicts).
-// The 8 working warps form pairs: a pair scores 16 of a page's tokens, each warp of it over half of the
-// latent columns (the query's operand registers would not fit otherwise), and swaps partial scores, so
-// that a tick later each warp weighs 8 tokens: against a reference maximum that moves only when weights
-// pass it by 2^10, P s of each group going to shared memory.  Another tick later each warp adds D/8
-// latent columns of the page up.  So three pages are under way in a tick, with nothing to wait for between
-// their parts, and one barrier ends it: it publishes the swap and the weights, carries the vote on
-// moving the references, and joins two helping warps: one waits for the next page's arrival before it,
-// one refills the stage that became free after it (either would cost a working warp hundreds of cycles).
+// A CTA holds NH tiles of 8 query rows (query tokens x heads; up to two for D = 512, five for D = 256) and walks the
+// pages of one or more requests, two (a tile of 128 tokens) at a time:
+//   - a loading warp brings pages by TMA (128-byte swizzle); one thread issues the tcgen05 products;
+//   - eight token warps, two threads a token: codes to TMEM, scores from TMEM, the softmax against references that
+//     move only when weights pass them by 2^10, P s of each group to shared memory.  A vote a tile moves the
+//     references; a move leaves the factors for the sums beside the weights;
+//   - eight adding warps hold D/8 latent columns of the result each.
+// The roles meet in mbarriers only, each a tile ahead of the next.
 //
 // The pages of all requests are dealt to the CTAs in one equal run each (a run may begin or end inside
 // a request); what is cut is joined by merge_kernel by log-sum-exp.
@@ -34,9 +33,12 @@ namespace rolaq {
 namespace i4 {
 namespace {
 
-// Eight working warps and a warpgroup of which two warps load.  Of the 168 registers a thread that a block of
-// 384 is launched with, the loaders hand most to the workers: 2 * 224 + 56 = 2 * 232 + 40 = 3 * 168.
-constexpr int kWarps = 8, kWorkers = kWarps * 32, kThreads = kWorkers + 128;
+// Warps 0..7 are the token warps, 8..15 the adding ones, 16 and 17 load, 18 issues.  Of the 96 registers a thread that a
+// block of 640 is launched with, the others hand some to the token warps.
+constexpr int kTokenWarps = 8, kAddWarps = 8;
+constexpr int kTokens = kTokenWarps * 32, kAdders = kAddWarps * 32, kThreads = kTokens + kAdders + 128;
+constexpr int kTile = 2 * kPage;  // tokens of a tile
+constexpr int kAhead = 12;    // pages ahead of their loads that they are called to L2
 constexpr int kMinPages = 2;  // least run of pages worth a CTA of its own
 constexpr float kSlack = 1024.f, kScaleSlack = 32.f;  // how far weights and scales may pass their references (P s <= 2^15)
 constexpr float kNoMax = -1e30f, kNoUnit = 1.329227995784916e36f;  // references not yet set: the first token passes them
@@ -45,38 +47,80 @@ constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 template <int D, int DR, int NH>
 struct Cfg {
   static constexpr int NG = D / kGroup;             // groups of a token
-  static constexpr int CODES = kPage * D / 2, ROPE = kPage * DR * 2, PARAMS = kPage * NG * 8;
-  static constexpr int STAGE = CODES + ROPE + PARAMS;
-  static constexpr int QROW = (D + DR) * 2 + 16;    // bytes of a query row in shared memory (16: no bank conflicts)
-  static constexpr int STAGES = D == 512 ? 6 : DR == 64 ? 8 : 10;
+  static constexpr int CODES = kPage * D / 2, ROPE = kPage * DR * 2, PARAMS = kPage * NG * 8;  // of a page
+  static constexpr int PAGES = D == 512 ? 8 : 12;   // a ring of pages' codes and params
+  static constexpr int TILES = 2;                   // one of tiles' rotary parts, which only the scores need
+  static constexpr int WEIGHTS = 3;                 // and one of pages' P s: a tile's first is written while the last one's second is in use
+  static constexpr int ROWS = 8 * NH;
+  static constexpr int NQ = (ROWS + 15) / 16 * 16;  // columns of the scores' products
+  static constexpr int QB_GROUP = NQ * 128, QB = 2 * NG * QB_GROUP, QPE = NQ * DR * 2;  // hi of all groups, lo of all groups
   static constexpr int PTILE = kPage * 16;          // P s of a page, a group and 8 rows: [token][row] FP16
   static constexpr int PBUF = NG * NH * PTILE;
-  static constexpr int SMEM = 1024 + STAGES * STAGE + 2 * PBUF + 8 * NH * QROW;
-  static constexpr int HG = NG / 2;                 // groups that a warp scores
-  static constexpr int CH = D / kWarps / 32;        // 32-column chunks that a warp adds up
-  static constexpr int ROWS = 8 * NH;
-  static constexpr int WORKER_REGS = NH < 4 ? 224 : 232, LOADER_REGS = NH < 4 ? 56 : 40;
+  // swizzled tiles first, on 1024-byte boundaries; the pages' params apart
+  static constexpr int OFF_ROPE = PAGES * CODES, OFF_QB = OFF_ROPE + TILES * 2 * ROPE, OFF_QPE = OFF_QB + QB;
+  static constexpr int OFF_P = OFF_QPE + QPE, OFF_PARAMS = OFF_P + WEIGHTS * PBUF;
+  static constexpr int SMEM = 1024 + OFF_PARAMS + PAGES * PARAMS;
+  static constexpr int CH = D / kAddWarps / 32;     // 32-column chunks that an adding warp holds
+  static constexpr int HT = (NH + 1) / 2;           // tiles of 8 rows of a token thread
+  // TMEM columns: two tiles' codes; two tiles' scores (the groups' sums, the rotary part's)
+  static constexpr int T_CODES = D / 4, T_SUM = 2 * T_CODES, T_ROPE = NG * NQ, T_TILE = (NG + 1) * NQ;
+  static constexpr int TOKEN_REGS = 136, ADD_REGS = 80, LOAD_REGS = 48;
+  static_assert(T_SUM + 2 * T_TILE <= 512 && 2 * TOKEN_REGS + 2 * ADD_REGS + LOAD_REGS <= 5 * 96, "TMEM, registers");
 };
 
 template <int NG, int NH>
-struct Shared {
-  float2 swap[2][kWarps][NH][32];
-  float red_m[kWarps][8 * NH], red_s[kWarps][NG], red_l[kWarps][8 * NH], red_z[kWarps][NG][8 * NH];
-  float q_top[2][8 * NH], q_sum[NG][8 * NH], row_scale[8 * NH];
-  float l_all[8 * NH], z_all[NG][8 * NH], max[8 * NH];
+struct alignas(16) Shared {  // rows are read two at a time
+  float red_m[4][8 * NH], red_s[4][NG];                   // by quarters of the tile's tokens
+  float keep[3][8 * NH], keep_unit[3][NG];                // factors for the sums before tile i (at i % 3), where moved[i % 3]
+  float max[8 * NH], q_sum[NG][8 * NH], row_scale[8 * NH];
+  float l[4][8 * NH], z[4][NG][8 * NH], max_out[8 * NH], unit_out[NG];  // of a finished request
+  int moved[3];
 };
 
-// Named barriers: the end of a tick (working and loading warps), and the working warps'.
-constexpr int kBarTick = 1, kBarWork = 2;
-__device__ __forceinline__ void work_sync() { named_bar_sync(kBarWork, kWorkers); }
-__device__ __forceinline__ bool tick(bool vote) {
+// Named barriers: the token warps; a request's sums are written / have been taken.
+constexpr int kBarToken = 1, kBarSums = 2, kBarTaken = 3;
+__device__ __forceinline__ void token_sync() { named_bar_sync(kBarToken, kTokens); }
+__device__ __forceinline__ bool token_any(bool vote) {
   int any;
   asm volatile(
       "{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %3, 0;\n\tbar.red.or.pred q, %1, %2, p;\n\tselp.b32 %0, 1, 0, q;\n\t}"
       : "=r"(any)
-      : "n"(kBarTick), "n"(kWorkers + 64), "r"(static_cast<int>(vote))
+      : "n"(kBarToken), "n"(kTokens), "r"(static_cast<int>(vote))
       : "memory");
   return any != 0;
+}
+__device__ __forceinline__ bool elect_one() {
+  uint32_t one;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xFFFFFFFF;\n\tselp.b32 %0, 1, 0, p;\n\t}" : "=r"(one));
+  return one != 0;
+}
+__device__ __forceinline__ void bar_arrive(int id, int threads) {
+  asm volatile("bar.arrive %0, %1;" ::"r"(id), "r"(threads) : "memory");
+}
+
+// Two FP32 operations an instruction, each rounded like the plain one.
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  uint64_t d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;"
+      : "=l"(d)
+      : "l"(*reinterpret_cast<uint64_t*>(&a)), "l"(*reinterpret_cast<uint64_t*>(&b)), "l"(*reinterpret_cast<uint64_t*>(&c)));
+  return *reinterpret_cast<float2*>(&d);
+}
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+  uint64_t d;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(*reinterpret_cast<uint64_t*>(&a)), "l"(*reinterpret_cast<uint64_t*>(&b)));
+  return *reinterpret_cast<float2*>(&d);
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+  uint64_t d;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(*reinterpret_cast<uint64_t*>(&a)), "l"(*reinterpret_cast<uint64_t*>(&b)));
+  return *reinterpret_cast<float2*>(&d);
+}
+__device__ __forceinline__ float2 both(float x) { return make_float2(x, x); }
+__device__ __forceinline__ float warp_sum(float v) {
+#pragma unroll
+  for (int o = 16; o >= 1; o /= 2) v += __shfl_xor_sync(0xFFFFFFFFu, v, o);
+  return v;
 }
 
 __device__ __forceinline__ int pages_of(const DecodeArgs& a, int b) {
@@ -102,11 +146,6 @@ struct Runs {
   }
 };
 
-__device__ __forceinline__ void ldsm_x4(uint32_t addr, uint32_t (&r)[4]) {
-  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
-               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
-               : "r"(addr));
-}
 __device__ __forceinline__ void ldsm_x4_t(uint32_t addr, uint32_t (&r)[4]) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
                : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
@@ -115,12 +154,6 @@ __device__ __forceinline__ void ldsm_x4_t(uint32_t addr, uint32_t (&r)[4]) {
 // D (16 x 8, FP32) += A (16 x 16) B (16 x 8).  Not volatile: the compiler may interleave them.
 __device__ __forceinline__ void mma_f16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
   asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
-      "{%0, %1, %2, %3};"
-      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-}
-__device__ __forceinline__ void mma_bf16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-  asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
       "{%0, %1, %2, %3};"
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
@@ -134,27 +167,6 @@ __device__ __forceinline__ uint32_t pack_half2(float lo, float hi) {
 // The shared-memory offset of 16-byte chunk `chunk` of row `row` under TMA's swizzles.
 __device__ __forceinline__ uint32_t sw128(int row, int chunk) { return row * 128 + ((chunk ^ (row & 7)) << 4); }
 __device__ __forceinline__ uint32_t sw64(int row, int chunk) { return row * 64 + ((chunk ^ ((row >> 1) & 3)) << 4); }
-
-// Sum over a quad's four lanes / maximum over them, and over the eight lanes of the same place in their quads.
-__device__ __forceinline__ float quad_sum(float v) {
-  v += __shfl_xor_sync(0xFFFFFFFFu, v, 1);
-  return v + __shfl_xor_sync(0xFFFFFFFFu, v, 2);
-}
-__device__ __forceinline__ float quad_max(float v) {
-  v = fmaxf(v, __shfl_xor_sync(0xFFFFFFFFu, v, 1));
-  return fmaxf(v, __shfl_xor_sync(0xFFFFFFFFu, v, 2));
-}
-
-__device__ __forceinline__ float oct_sum(float v) {
-#pragma unroll
-  for (int o = 4; o < 32; o *= 2) v += __shfl_xor_sync(0xFFFFFFFFu, v, o);
-  return v;
-}
-__device__ __forceinline__ float oct_max(float v) {
-#pragma unroll
-  for (int o = 4; o < 32; o *= 2) v = fmaxf(v, __shfl_xor_sync(0xFFFFFFFFu, v, o));
-  return v;
-}
 
 // Exclusive prefix over the CTA's threads of v; the total in `total`.
 template <int WARPS>
@@ -190,26 +202,27 @@ __global__ void __launch_bounds__(kThreads, 1)
     decode_kernel(const __grid_constant__ CUtensorMap map_codes, const __grid_constant__ CUtensorMap map_rope,
                   const DecodeArgs a, const Partials part, const int groups, const int blocks) {
   using C = Cfg<D, DR, NH>;
-  constexpr int NG = C::NG, HG = C::HG, CH = C::CH, STAGES = C::STAGES, ROWS = C::ROWS;
-  constexpr bool HELD_MAX = NH < 4;  // references in registers
-  constexpr int KR = DR / 32;  // 16-column steps of the rotary part that a warp scores
+  constexpr int NG = C::NG, CH = C::CH, PAGES = C::PAGES, TILES = C::TILES, ROWS = C::ROWS, HT = C::HT;
   extern __shared__ char raw[];
   char* smem = reinterpret_cast<char*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
-  char* pbuf = smem + STAGES * C::STAGE;
-  char* qbuf = pbuf + 2 * C::PBUF;
-  __shared__ uint64_t full[STAGES], q_full;
-  __shared__ int bad_page[STAGES];
+  // a page's codes loaded / added; a tile's rotary part loaded / used; its codes in TMEM, its scores there, they are taken,
+  // its weights in shared memory; the request's query there
+  __shared__ uint64_t full[PAGES], page_free[PAGES], rope_full[TILES], rope_free[TILES], coded[2], scored[2], taken[2], weighed[3], q_ready;
+  __shared__ int bad_page[PAGES];
   __shared__ int64_t scan[kThreads / 32];
   __shared__ int start[2];
-  __shared__ int64_t run_total, run_begin;  // read again where a request ends (registers are short in between)
+  __shared__ uint32_t tmem_slot;
   __shared__ Shared<NG, NH> sh;
 
-  const int tid = threadIdx.x, warp = tid / 32, lane = tid & 31, g = lane >> 2, j = lane & 3;
+  const int tid = threadIdx.x, warp = __shfl_sync(0xFFFFFFFFu, tid / 32, 0), lane = tid & 31;
   const int block = blockIdx.x % blocks, group = blockIdx.x / blocks;
   const int rows = a.q_len * a.heads, row0 = block * ROWS;
   if (tid == 0) {
-    for (int s = 0; s < STAGES; ++s) mbar_init(&full[s], 1);
-    mbar_init(&q_full, 1);
+    for (int s = 0; s < PAGES; ++s) mbar_init(&full[s], 1), mbar_init(&page_free[s], kAddWarps);
+    for (int s = 0; s < TILES; ++s) mbar_init(&rope_full[s], 1), mbar_init(&rope_free[s], 1);
+    for (int s = 0; s < 2; ++s) mbar_init(&coded[s], kTokenWarps), mbar_init(&scored[s], 1), mbar_init(&taken[s], kTokenWarps);
+    for (int s = 0; s < 3; ++s) mbar_init(&weighed[s], 1);
+    mbar_init(&q_ready, 1);
     fence_mbar_init();
     prefetch_tensormap(&map_codes);
     prefetch_tensormap(&map_rope);
@@ -235,579 +248,595 @@ __global__ void __launch_bounds__(kThreads, 1)
   if (group >= runs.n || total == 0) return;
   const int64_t u0 = runs.begin(group);
   const int n_units = static_cast<int>(runs.begin(group + 1) - u0);
-  if (tid == 0) run_total = total, run_begin = u0;
   if (before <= u0 && u0 < before + mine) {
     int b = tid * per;
     for (int n; before + (n = pages_of(a, b)) <= u0; ++b) before += n;
     start[0] = b;
     start[1] = static_cast<int>(u0 - before);
   }
-  __syncthreads();
-  int seg_b = start[0], seg_p = start[1];
-
-  if (warp >= kWarps) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(C::LOADER_REGS));
-    if (warp > kWarps + 1) return;
-    const bool loader = warp == kWarps;
-    // ================= the loading warp: stage k holds page k of the run =================
-    // Lane l holds the id of page `base` + l of the run; the next 32 are requested 32 pages ahead of their use.
-    const int pool_pages = static_cast<int>(a.cache.num_slots / kPage);
-    int id_b = seg_b, id_p = seg_p + lane, ids = -1, next_ids = -1, loaded = 0, load_stage = 0;
-    auto fetch_ids = [&](int first) {
-      int id = -1;
-      if (first + lane < n_units) {
-        for (int n; id_p >= (n = pages_of(a, id_b)); ++id_b) id_p -= n;
-        id = a.page_table[id_b * a.pt_stride + id_p];
-      }
-      id_p += 32;
-      return id;
-    };
-    auto load = [&]() {
-      if (loaded == n_units) return;
-      if ((loaded & 31) == 0) {
-        ids = next_ids;
-        next_ids = fetch_ids(loaded + 32);
-      }
-      const int id = __shfl_sync(0xFFFFFFFFu, ids, loaded & 31);
-      ++loaded;
-      const bool ok = id >= 0 && id < pool_pages;
-      const int page = ok ? id : 0;
-      if (lane == 0) {
-        char* dst = smem + load_stage * C::STAGE;
-        uint64_t* bar = &full[load_stage];
-        bad_page[load_stage] = !ok;
-        mbar_expect_tx(bar, C::STAGE);
-#pragma unroll
-        for (int k = 0; k < D / 256; ++k) tma_load_2d(dst + k * 8192, &map_codes, bar, k * 128, page * kPage);
-        tma_load_2d(dst + C::CODES, &map_rope, bar, 0, page * kPage);
-        bulk_load(dst + C::CODES + C::ROPE, a.cache.params + static_cast<int64_t>(page) * (kPage * NG * 2), C::PARAMS, bar);
-        if (!ok) report(a.err, ROLAQ_DEV_BAD_PAGE);
-      }
-      __syncwarp();
-      if (++load_stage == STAGES) load_stage = 0;
-    };
-    auto load_query = [&](int b) {
-      const int live = min(ROWS, rows - row0);
-      if (lane == 0) mbar_expect_tx(&q_full, live * ((D + DR) * 2));
-      __syncwarp();
-      for (int r = lane; r < live; r += 32) {
-        const int t = (row0 + r) / a.heads, h = (row0 + r) % a.heads;
-        bulk_load(qbuf + r * C::QROW, a.q + b * a.q_sb + t * a.q_st + h * a.q_sh, (D + DR) * 2, &q_full);
-      }
-    };
-    // ================= the awaiting warp =================
-    int stage = 0, lap = 0, arrived = 0, queries = 0;
-    bool healthy = true;
-    auto await = [&]() {  // the next page of the run; after one that did not come in time the rest is not awaited
-      if (arrived == n_units) return;
-      if (healthy) healthy = mbar_wait(&full[stage], lap & 1, a.err);
-      __syncwarp();
-      ++arrived;
-      if (++stage == STAGES) stage = 0, ++lap;
-    };
-    auto await_query = [&]() {
-      if (healthy) healthy = mbar_wait(&q_full, queries & 1, a.err);
-      __syncwarp();
-      ++queries;
-    };
-    if (loader) {
-      next_ids = fetch_ids(0);
-      load_query(seg_b);
-      for (int i = 0; i < STAGES; ++i) load();
-    } else {
-      await_query();
-      await();
-    }
-    tick(false);
-    for (int done = 0; done < n_units;) {
-      const int count = min(pages_of(a, seg_b) - seg_p, n_units - done);
-      done += count;
-      do ++seg_b;  // the request after this one, where the run has one
-      while (done < n_units && pages_of(a, seg_b) == 0);
-      seg_p = 0;
-      for (int t = 0; t < count + 2; ++t) {
-        if (!loader && t + 1 < count) await();  // the page that the next tick scores
-        if (!loader && t == count + 1 && done < n_units) {
-          await_query();
-          await();
-        }
-        tick(false);
-        if (loader && t == 0 && done < n_units) load_query(seg_b);  // this request's query has been taken
-        if (loader && t >= 2) load();                               // page t - 2 has been added up
-      }
-    }
-    return;
+  if (warp == 0) {
+    tmem_alloc(&tmem_slot, 512);
+    tmem_relinquish();
   }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = __shfl_sync(0xFFFFFFFFu, tmem_slot, 0);
+  int seg_b = start[0], seg_p = start[1];
+  // A wait that ran out of time is reported; the role goes on without waiting, so that all barriers are met.
+  bool healthy = true;
+  auto wait_for = [&](uint64_t* bar, int phase) {
+    if (healthy) healthy = mbar_wait(bar, phase & 1, a.err);
+  };
 
-  asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(C::WORKER_REGS));
-  const int half = warp & 1, quarter = warp >> 1;  // half of the latent columns, 16 of the page's tokens
-  const int own = warp * NG / kWarps;              // the group of the columns that the warp adds up
-  // Offsets of the lane's ldmatrix rows from a 1024-byte boundary.  Chunk c of a row lies at c ^ row % 8, so
-  // chunk c ^ x is at the address ^ 16 x.  Of the pair's 16 tokens the warp's own eight come first.
-  const uint32_t stages = smem_u32(smem), pbufs = smem_u32(pbuf);
-  const int tok_row = 16 * quarter + ((8 * half + (lane & 15)) & 15);
-  const uint32_t code_off = D == 512 ? half * 8192 + sw128(tok_row, lane >> 4) : sw128(tok_row, 4 * half + (lane >> 4));
-  const uint32_t rope_off = C::CODES + (DR == 64 ? sw128(tok_row, 4 * half + (lane >> 4)) : sw64(tok_row, 2 * half + (lane >> 4)));
-  const uint32_t add_off = (warp * CH / 8) * 8192 + sw128(lane, (warp * CH) & 7);
-  const uint32_t p_off = own * (NH * C::PTILE) + lane * 16;
-  const uint32_t p_dst = (8 * warp + g) * 16 + 4 * j;
-  const float qk_scale = a.sm_scale * kLog2e;
-  int done = 0, stage = 0;  // pages of the run; the stage of the page scored next
-  tick(false);              // the first query and page are there
-
-  while (done < n_units) {
-    const int seg_pages = pages_of(a, seg_b);
-    if (seg_pages == 0) {
-      ++seg_b;
-      continue;
-    }
-    const bool first = done == 0;
-    const int count = min(seg_pages - seg_p, n_units - done);
-    const int len = min(static_cast<int64_t>(a.seq_lens[seg_b]), static_cast<int64_t>(a.max_pages) * kPage);
-    if (tid == 0 && len != a.seq_lens[seg_b]) report(a.err, ROLAQ_DEV_BAD_REQ);
-    const int lim_min = len - a.q_len + 1;
-
-    // ---- the query: brought to operand form in place, 8 elements at a time, then row g of each tile to registers ----
-    constexpr int QC = D / 8;  // 16-byte pieces of a row's latent part
-    const int live = min(ROWS, rows - row0);
-#pragma unroll 1
-    for (int i = tid; i < ROWS * QC; i += kWorkers) {
-      const int r = i / QC;
-      float top = 0.f, odd = 0.f;
-      if (r < live) {
-        const uint4 w = *reinterpret_cast<const uint4*>(qbuf + r * C::QROW + 16 * (i % QC));
-        const uint32_t v[4] = {w.x, w.y, w.z, w.w};
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          top = fmaxf(top, fmaxf(fabsf(bf16_lo(v[k])), fabsf(bf16_hi(v[k]))));
-          odd = fmaf(bf16_lo(v[k]), 0.f, fmaf(bf16_hi(v[k]), 0.f, odd));  // NaN where an element is no finite number
+  if (tid >= kTokens + kAdders) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(C::LOAD_REGS));
+    constexpr int first_warp = kTokenWarps + kAddWarps;
+    if (warp <= first_warp + 1) {
+      // ================= the loading warps: codes and params by pages; rotary parts by tiles =================
+      // Lane l holds the id of page `base` + l of the run; the next 32 are requested 32 pages ahead of their use.
+      const bool codes = warp == first_warp;
+      const int pool_pages = static_cast<int>(a.cache.num_slots / kPage);
+      int id_b = seg_b, id_p = seg_p + lane, ids = -1, next_ids = -1, id_q = 0;
+      auto fetch_ids = [&](int first) {
+        int id = -1;
+        if (first + lane < n_units) {
+          for (int n; id_p >= (n = pages_of(a, id_b)); ++id_b) id_p -= n;
+          id = a.page_table[id_b * a.pt_stride + id_p];
         }
-      }
-      top = warp_max_f32(odd != 0.f ? INFINITY : top);
-      if (lane == 0) sh.q_top[D == 512 ? (i / 32) & 1 : 0][r] = top;
-    }
-    work_sync();
-    auto row_top = [&](int r) { return D == 512 ? fmaxf(sh.q_top[0][r], sh.q_top[1][r]) : sh.q_top[0][r]; };
-    auto row_unit = [&](float top) {  // 2^k with top 2^k in [2^13, 2^14)
-      return top > 0.f ? pow2(min(max(13 - (static_cast<int>(__float_as_uint(top) >> 23) - 127), -100), 100)) : 1.f;
-    };
-#pragma unroll 1
-    for (int i = tid; i < ROWS * QC; i += kWorkers) {
-      const int r = i / QC, c = i % QC;
-      const float top = row_top(r), up = row_unit(top);
-      uint4* at = reinterpret_cast<uint4*>(qbuf + r * C::QROW + 16 * c);
-      const uint4 w = r < live ? *at : make_uint4(0, 0, 0, 0);
-      const uint32_t v[4] = {w.x, w.y, w.z, w.w};
-      float x[8], sum = 0.f;
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        x[2 * e] = bf16_lo(v[e]) * up, x[2 * e + 1] = bf16_hi(v[e]) * up;
-        sum += x[2 * e] + x[2 * e + 1];
-      }
-      // a word of codes gives elements (0, 4), 16 (1, 5), (2, 6) and 16 (3, 7)
-      *at = make_uint4(pack_half2(x[0], x[4]), pack_half2(x[1] * 0.0625f, x[5] * 0.0625f), pack_half2(x[2], x[6]),
-                       pack_half2(x[3] * 0.0625f, x[7] * 0.0625f));
-#pragma unroll
-      for (int o = 1; o < 16; o *= 2) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, o);
-      if (c % 16 == 0) sh.q_sum[c / 16][r] = sum * (1.f / 16777216.f);
-      if (c == 0) sh.row_scale[r] = top == INFINITY ? __int_as_float(0x7FC00000) : qk_scale * (16777216.f / up);
-    }
-    // the rotary part under the same power of two (exact), so that both parts add up
-#pragma unroll 1
-    for (int i = tid; i < ROWS * (DR / 2); i += kWorkers) {
-      const int r = i / (DR / 2);
-      const float down = row_unit(row_top(r)) * (1.f / 16777216.f);
-      uint32_t* at = reinterpret_cast<uint32_t*>(qbuf + r * C::QROW + 2 * D) + i % (DR / 2);
-      *at = r < live ? pack_bf16x2(bf16_lo(*at) * down, bf16_hi(*at) * down) : 0u;
-    }
-    work_sync();
-    uint32_t q[NH][8 * HG][2], q_pe[NH][KR][2];
-#pragma unroll
-    for (int n = 0; n < NH; ++n) {
-      const char* src = qbuf + (8 * n + g) * C::QROW;
-#pragma unroll
-      for (int c = 0; c < 4 * HG; ++c) {
-        const uint4 w = *reinterpret_cast<const uint4*>(src + half * D + 64 * c + 16 * j);
-        q[n][2 * c][0] = w.x, q[n][2 * c][1] = w.y, q[n][2 * c + 1][0] = w.z, q[n][2 * c + 1][1] = w.w;
-      }
-#pragma unroll
-      for (int c = 0; c < KR; ++c)
-#pragma unroll
-        for (int e = 0; e < 2; ++e) q_pe[n][c][e] = *reinterpret_cast<const uint32_t*>(src + 2 * (D + 16 * (half * KR + c) + 8 * e + 2 * j));
-    }
-    // the rows' factors: held where few, read again each page where many
-    float2 held_sum[NH <= 2 ? HG : 1][NH <= 2 ? NH : 1], held_scale[NH <= 2 ? NH : 1];
-    auto q_sum_of = [&](int k, int n) { return *reinterpret_cast<const float2*>(&sh.q_sum[half * HG + k][8 * n + 2 * j]); };
-    auto scale_of = [&](int n) { return *reinterpret_cast<const float2*>(&sh.row_scale[8 * n + 2 * j]); };
-    if constexpr (NH <= 2) {
-#pragma unroll
-      for (int n = 0; n < NH; ++n) {
-        held_scale[n] = scale_of(n);
-#pragma unroll
-        for (int k = 0; k < HG; ++k) held_sum[k][n] = q_sum_of(k, n);
-      }
-    }
-
-    // accumulators: tile 2 c + h of chunk c holds columns 4 g + 2 h (and that + 16 times the next one) x rows 2 j, + 1
-    float acc[2 * CH][NH][4], zsum[NH][2][NG], unit[NG], l_sum[NH][2];
-    float2 held_max[HELD_MAX ? NH : 1];  // references: the largest scores so far, kNoMax before the first
-#pragma unroll
-    for (int n = 0; n < NH; ++n) {
-#pragma unroll
-      for (int c = 0; c < 2 * CH; ++c) acc[c][n][0] = acc[c][n][1] = acc[c][n][2] = acc[c][n][3] = 0.f;
-#pragma unroll
-      for (int x = 0; x < 2; ++x) {
-        l_sum[n][x] = 0.f;
-#pragma unroll
-        for (int k = 0; k < NG; ++k) zsum[n][x][k] = 0.f;
-      }
-    }
-#pragma unroll
-    for (int k = 0; k < NG; ++k) unit[k] = kNoUnit;
-    auto max_of = [&](int n) {
-      if constexpr (HELD_MAX) return held_max[n];
-      else return *reinterpret_cast<const float2*>(&sh.max[8 * n + 2 * j]);
-    };
-    auto set_max = [&](int n, float2 m) {
-      if constexpr (HELD_MAX) held_max[n] = m;
-      else if (warp == 0 && g == 0) *reinterpret_cast<float2*>(&sh.max[8 * n + 2 * j]) = m;
-    };
-#pragma unroll
-    for (int n = 0; n < NH; ++n) set_max(n, make_float2(kNoMax, kNoMax));
-
-    // Partial scores of the pair's 16 tokens: the warp's own eight in mine_s, the partner's to the swap.
-    float mine_s[NH][2] = {};
-    auto score = [&](int st_at, int pb) {
-      const uint32_t st = stages + st_at * C::STAGE;
-      float c_acc[HG][NH][4], r_acc[NH][4];
-      uint32_t w[HG][2][4], w_pe[KR][4];
-#pragma unroll
-      for (int k = 0; k < HG; ++k)
-#pragma unroll
-        for (int i = 0; i < 2; ++i) ldsm_x4((st + code_off) ^ (k << 6) ^ (i << 5), w[k][i]);
-#pragma unroll
-      for (int c = 0; c < KR; ++c) ldsm_x4((st + rope_off) ^ (c << 5), w_pe[c]);
-#pragma unroll
-      for (int n = 0; n < NH; ++n)
-#pragma unroll
-        for (int x = 0; x < 4; ++x) {
-          r_acc[n][x] = 0.f;
-#pragma unroll
-          for (int k = 0; k < HG; ++k) c_acc[k][n][x] = 0.f;
+        id_p += 32;
+        return id;
+      };
+      next_ids = fetch_ids(0);
+      int slot = 0, lap = 0, left = 0;  // left: pages of the present request
+      for (int i = 0; i < n_units; ++i) {
+        if ((i & 31) == 0) {
+          ids = next_ids;
+          next_ids = fetch_ids(i + 32);
         }
-      // the accumulators in turn, so that no product waits for the one before it
+        const int id = __shfl_sync(0xFFFFFFFFu, ids, i & 31);
+        const bool ok = id >= 0 && id < pool_pages;
+        const int page = ok ? id : 0;
+        // The rings are a few pages short of covering the way from memory: pages come to L2 ahead of them.
+        const int ahead_id = __shfl_sync(0xFFFFFFFFu, (i & 31) + kAhead < 32 ? ids : next_ids, (i + kAhead) & 31);
+        if (lane == 1 && i + kAhead < n_units && ahead_id >= 0 && ahead_id < pool_pages) {
+          const int64_t token = static_cast<int64_t>(ahead_id) * kPage;
+          if (codes) {
+            prefetch_l2(a.cache.codes + token * (D / 2), C::CODES);
+            prefetch_l2(a.cache.params + token * (NG * 2), C::PARAMS);
+          } else {
+            prefetch_l2(a.cache.rope + token * DR, C::ROPE);
+          }
+        }
+        if (codes) {
+          if (lap > 0) wait_for(&page_free[slot], lap - 1);
+          if (lane == 0) {
+            uint64_t* bar = &full[slot];
+            bad_page[slot] = !ok;
+            if (!ok) report(a.err, ROLAQ_DEV_BAD_PAGE);
+            mbar_expect_tx(bar, C::CODES + C::PARAMS);
 #pragma unroll
-      for (int i = 0; i < 2; ++i)
-#pragma unroll
-        for (int c = 0; c < 2; ++c)
-#pragma unroll
-          for (int e = 0; e < 2; ++e)
-#pragma unroll
-            for (int k = 0; k < HG; ++k) {
-              const uint32_t lo = e ? odd_bytes(w[k][i][2 * c]) : w[k][i][2 * c], hi = e ? odd_bytes(w[k][i][2 * c + 1]) : w[k][i][2 * c + 1];
-              const uint32_t lo0 = lo & 0x000F000Fu, hi0 = hi & 0x000F000Fu;
-              const uint32_t codes[4] = {lo0, hi0, e ? lo - lo0 : lo & 0x00F000F0u, e ? hi - hi0 : hi & 0x00F000F0u};
-#pragma unroll
-              for (int n = 0; n < NH; ++n) mma_f16(c_acc[k][n], codes, q[n][8 * k + 4 * i + 2 * c + e][0], q[n][8 * k + 4 * i + 2 * c + e][1]);
-            }
-#pragma unroll
-      for (int c = 0; c < KR; ++c)
-#pragma unroll
-        for (int n = 0; n < NH; ++n) mma_bf16(r_acc[n], w_pe[c], q_pe[n][c][0], q_pe[n][c][1]);
-      // tokens g (own) and g + 8 (the partner's)
-      float s[2][HG], z[2][HG];
-#pragma unroll
-      for (int t = 0; t < 2; ++t) {
-        const char* par = smem + st_at * C::STAGE + C::CODES + C::ROPE + ((8 * (warp ^ t)) + g) * (NG * 8) + half * (HG * 8);
-        if constexpr (HG == 2) {
-          const float4 v = *reinterpret_cast<const float4*>(par);
-          s[t][0] = v.x, z[t][0] = v.y, s[t][1] = v.z, z[t][1] = v.w;
+            for (int k = 0; k < D / 256; ++k)
+              tma_load_2d(smem + slot * C::CODES + k * 8192, &map_codes, bar, k * 128, page * kPage);
+            bulk_load(smem + C::OFF_PARAMS + slot * C::PARAMS, a.cache.params + static_cast<int64_t>(page) * (kPage * NG * 2),
+                      C::PARAMS, bar);
+          }
+          if (++slot == PAGES) slot = 0, ++lap;
         } else {
-          const float2 v = *reinterpret_cast<const float2*>(par);
-          s[t][0] = v.x, z[t][0] = v.y;
+          if (left == 0) {  // a tile's first page is an even one of its request's share
+            for (; pages_of(a, seg_b) - seg_p <= 0; seg_p = 0) ++seg_b;
+            left = min(pages_of(a, seg_b) - seg_p, n_units - i);
+            ++seg_b;
+            seg_p = 0;
+            id_q = 0;
+          }
+          if ((id_q & 1) == 0) {
+            if (lap > 0) wait_for(&rope_free[slot], lap - 1);
+            if (lane == 0) mbar_expect_tx(&rope_full[slot], (left > 1 ? 2 : 1) * C::ROPE);
+          }
+          if (lane == 0) tma_load_2d(smem + C::OFF_ROPE + (2 * slot + (id_q & 1)) * C::ROPE, &map_rope, &rope_full[slot], 0, page * kPage);
+          ++id_q, --left;
+          if ((id_q & 1) == 0 || left == 0)
+            if (++slot == TILES) slot = 0, ++lap;
         }
       }
+    } else if (warp == first_warp + 2) {
+      // ================= the issuing warp: scores of tile i = codes (TMEM) x query, rope x query =================
+      // One lane issues; the others go along, so that all its operands are known to be the same in all lanes.
+      constexpr uint32_t id_qk = idesc_e4m3(128, C::NQ, 0, 0), id_pe = idesc_bf16(128, C::NQ);
+      const uint64_t d_q = sw128_kmajor_desc(smem_u32(smem + C::OFF_QB));
+      const uint64_t d_qp = DR == 64 ? sw128_kmajor_desc(smem_u32(smem + C::OFF_QPE)) : sw64_kmajor_desc(smem_u32(smem + C::OFF_QPE));
+      int tile = 0, queries = 0;
+      for (int done = 0; done < n_units; ++seg_b, seg_p = 0) {
+        const int count = min(pages_of(a, seg_b) - seg_p, n_units - done);
+        if (count <= 0) continue;
+        wait_for(&q_ready, queries++);
+        for (int p = 0; p < count; p += 2, ++tile) {
+          wait_for(&rope_full[tile & 1], tile >> 1);
+          wait_for(&coded[tile & 1], tile >> 1);
+          if (tile >= 2) wait_for(&taken[tile & 1], (tile >> 1) - 1);
+          __syncwarp();
+          tc_fence_after();
+          const uint32_t codes = tmem + (tile & 1) * C::T_CODES, sums = tmem + C::T_SUM + (tile & 1) * C::T_TILE;
+          const uint32_t rope = smem_u32(smem + C::OFF_ROPE + (tile & 1) * 2 * C::ROPE);
+          const uint64_t d_k = DR == 64 ? sw128_kmajor_desc(rope) : sw64_kmajor_desc(rope);
+          if (elect_one()) {
 #pragma unroll
-      for (int n = 0; n < NH; ++n) {
-        float sum[4] = {r_acc[n][0], r_acc[n][1], r_acc[n][2], r_acc[n][3]};
+            for (int k = 0; k < NG; ++k)
 #pragma unroll
-        for (int k = 0; k < HG; ++k) {
-          float2 qs;
-          if constexpr (NH <= 2) qs = held_sum[k][n];
-          else qs = q_sum_of(k, n);
+              for (int m = 0; m < 8; ++m)  // hi, then lo
+                umma_f8_ts(sums + k * C::NQ, codes + 32 * k + 8 * (m & 3),
+                           d_q + static_cast<uint64_t>((C::QB_GROUP >> 4) * (k + (m >> 2) * NG) + 2 * (m & 3)), id_qk, m > 0);
 #pragma unroll
-          for (int x = 0; x < 4; ++x)
-            sum[x] = fmaf(s[x >> 1][k], fmaf(-z[x >> 1][k], x & 1 ? qs.y : qs.x, c_acc[k][n][x]), sum[x]);
+            for (int m = 0; m < DR / 16; ++m) umma_bf16_ss(sums + C::T_ROPE, d_k + 2 * m, d_qp + 2 * m, id_pe, m > 0);
+            umma_commit(&scored[tile & 1]);
+            umma_commit(&rope_free[tile & 1]);
+          }
+          __syncwarp();
         }
-        mine_s[n][0] = sum[0], mine_s[n][1] = sum[1];
-        sh.swap[pb][warp][n][lane] = make_float2(sum[2], sum[3]);
+        done += count;
       }
-    };
-
-    // A page's weights.  s_val: the whole scores of the warp's 8 tokens (the thread's: token g) in log2 units.
-    float s_val[NH][2], s_tok[NG], z_tok[NG], p_val[NH][2];
-    auto join = [&](int st_at, int pb, int p, const float (&own_s)[NH][2]) {
-#pragma unroll
-      for (int n = 0; n < NH; ++n) {
-        const float2 theirs = sh.swap[pb][warp ^ 1][n][lane];
-        float2 scale;
-        if constexpr (NH <= 2) scale = held_scale[n];
-        else scale = scale_of(n);
-        s_val[n][0] = (own_s[n][0] + theirs.x) * scale.x;
-        s_val[n][1] = (own_s[n][1] + theirs.y) * scale.y;
-      }
-      const float4* par = reinterpret_cast<const float4*>(smem + st_at * C::STAGE + C::CODES + C::ROPE) + (8 * warp + g) * (NG / 2);
-#pragma unroll
-      for (int k = 0; k < NG; k += 2) {
-        const float4 v = par[k / 2];
-        s_tok[k] = v.x, z_tok[k] = v.y, s_tok[k + 1] = v.z, z_tok[k + 1] = v.w;
-      }
-      const int bad = bad_page[st_at];
-      if ((p + 1) * kPage > lim_min || bad) {  // the request's end, or a page that is not there
-        const int tok = p * kPage + 8 * warp + g;
-        if (tok >= len || bad)
-#pragma unroll
-          for (int k = 0; k < NG; ++k) s_tok[k] = z_tok[k] = 0.f;
-#pragma unroll
-        for (int n = 0; n < NH; ++n)
-#pragma unroll
-          for (int x = 0; x < 2; ++x)
-            if (bad || tok >= lim_min + (row0 + 8 * n + 2 * j + x) / a.heads) s_val[n][x] = -INFINITY;
-      }
-    };
-
-    // Weights against the present references, times each group's scale, to shared memory; true where a
-    // weight or a scale has left its reference behind (their sums: moving early does no harm), or is NaN.
-    auto weigh = [&](int pb) {
-      float weights = 0.f, sizes = 0.f;
-#pragma unroll
-      for (int n = 0; n < NH; ++n) {
-        const float2 m = max_of(n);
-        p_val[n][0] = ex2_approx(s_val[n][0] - m.x);
-        p_val[n][1] = ex2_approx(s_val[n][1] - m.y);
-        weights += p_val[n][0] + p_val[n][1];
-      }
-      char* dst = pbuf + pb * C::PBUF + p_dst;
-#pragma unroll
-      for (int k = 0; k < NG; ++k) {
-        const float s = s_tok[k] * unit[k];
-        sizes += fabsf(s);
-#pragma unroll
-        for (int n = 0; n < NH; ++n)
-          *reinterpret_cast<uint32_t*>(dst + (k * NH + n) * C::PTILE) = pack_half2(p_val[n][0] * s, p_val[n][1] * s);
-      }
-      return !(weights <= kSlack) || !(sizes <= kScaleSlack);
-    };
-
-    // New references: the page's maxima; the sums so far are brought to them.
-    auto move_references = [&](int pb) {
-#pragma unroll
-      for (int n = 0; n < NH; ++n)
-#pragma unroll
-        for (int x = 0; x < 2; ++x) {
-          const float m = oct_max(s_val[n][x]);
-          if (g == 0) sh.red_m[warp][8 * n + 2 * j + x] = m;
-        }
-#pragma unroll
-      for (int k = 0; k < NG; ++k) {
-        const float s = oct_max(fabsf(s_tok[k]));
-        if (lane == 0) sh.red_s[warp][k] = s;
-      }
-      work_sync();
-      float keep_unit[NG], keep_own = 1.f;
-#pragma unroll
-      for (int k = 0; k < NG; ++k) {
-        float s = 0.f;
-        for (int w = 0; w < kWarps; ++w) s = fmaxf(s, sh.red_s[w][k]);
-        keep_unit[k] = 1.f;
-        if (s * unit[k] > 2.f) {  // bring the largest scale into [1, 2)
-          const float u = pow2(min(max(127 - static_cast<int>(__float_as_uint(s) >> 23), -100), 100));
-          keep_unit[k] = u / unit[k];
-          unit[k] = u;
-        }
-        if (k == own) keep_own = keep_unit[k];
-      }
-#pragma unroll
-      for (int n = 0; n < NH; ++n) {
-        const float2 old = max_of(n);
-        float2 m = old;
-        for (int w = 0; w < kWarps; ++w) {
-          const float2 v = *reinterpret_cast<const float2*>(&sh.red_m[w][8 * n + 2 * j]);
-          m.x = fmaxf(m.x, v.x), m.y = fmaxf(m.y, v.y);
-        }
-        if constexpr (!HELD_MAX) work_sync();  // all have read the old ones
-        set_max(n, m);
-#pragma unroll
-        for (int x = 0; x < 2; ++x) {
-          const float keep = ex2_approx(x ? old.y - m.y : old.x - m.x);
-          l_sum[n][x] *= keep;
-#pragma unroll
-          for (int k = 0; k < NG; ++k) zsum[n][x][k] *= keep * keep_unit[k];
-#pragma unroll
-          for (int c = 0; c < 2 * CH; ++c) acc[c][n][x] *= keep * keep_own, acc[c][n][x + 2] *= keep * keep_own;
-        }
-      }
-      if constexpr (!HELD_MAX) work_sync();
-      weigh(pb);
-      work_sync();
-    };
-
-    // After the references stand: the denominators and the zeros' share.
-    auto add_weights = [&]() {
-#pragma unroll
-      for (int n = 0; n < NH; ++n) l_sum[n][0] += p_val[n][0], l_sum[n][1] += p_val[n][1];
-#pragma unroll
-      for (int k = 0; k < NG; ++k) {
-        const float f = s_tok[k] * unit[k] * z_tok[k];
-#pragma unroll
-        for (int n = 0; n < NH; ++n)
-          zsum[n][0][k] = fmaf(p_val[n][0], f, zsum[n][0][k]), zsum[n][1][k] = fmaf(p_val[n][1], f, zsum[n][1][k]);
-      }
-    };
-
-    // acc += c^T (P s) over tokens 32 h .. 32 h + 31 of a page, the warp's columns.
-    auto gather = [&](int st_at, int pb, int h) {
-      const uint32_t st = stages + st_at * C::STAGE + add_off, ps = pbufs + pb * C::PBUF + p_off;
-      uint32_t pb_[NH][4], x[CH][4];
-#pragma unroll
-      for (int c = 0; c < CH; ++c) ldsm_x4_t((st + h * 4096) ^ (c << 4), x[c]);
-#pragma unroll
-      for (int n = 0; n < NH; ++n) ldsm_x4_t(ps + n * C::PTILE + h * 512, pb_[n]);
-#pragma unroll
-      for (int i = 0; i < 2; ++i)
-#pragma unroll
-        for (int c = 0; c < CH; ++c) {
-          // of four elements e: e0 over e0 + 16 e1, e2 over e2 + 16 e3
-          const uint32_t u = x[c][2 * i], v = x[c][2 * i + 1], u8 = odd_bytes(u), v8 = odd_bytes(v);
-          const uint32_t even[4] = {u & 0x000F000Fu, u & 0x00FF00FFu, v & 0x000F000Fu, v & 0x00FF00FFu};
-          const uint32_t odd[4] = {u8 & 0x000F000Fu, u8, v8 & 0x000F000Fu, v8};
-#pragma unroll
-          for (int n = 0; n < NH; ++n) mma_f16(acc[2 * c][n], even, pb_[n][2 * i], pb_[n][2 * i + 1]);
-#pragma unroll
-          for (int n = 0; n < NH; ++n) mma_f16(acc[2 * c + 1][n], odd, pb_[n][2 * i], pb_[n][2 * i + 1]);
-        }
-    };
-
-    // ---- the pages: tick t scores page t, weighs page t - 1 and adds page t - 2 up ----
-    auto after = [](int s, int n) { return s + n >= STAGES ? s + n - STAGES : s + n; };
-    int st_score = stage, st_weigh = stage, st_add = stage;
-    // A tick of whatever parts it has: the first two and the last.
-    auto any_tick = [&](int t) {
-      const int pb = t & 1;
-      float own_s[NH][2];
-#pragma unroll
-      for (int n = 0; n < NH; ++n) own_s[n][0] = mine_s[n][0], own_s[n][1] = mine_s[n][1];
-      if (t < count) {
-        score(st_score, pb);
-        st_score = after(st_score, 1);
-      }
-      if (t >= 2) {
-        gather(st_add, pb, 0);
-        gather(st_add, pb, 1);
-        st_add = after(st_add, 1);
-      }
-      bool vote = false;
-      if (t >= 1) {
-        join(st_weigh, pb ^ 1, seg_p + t - 1, own_s);
-        st_weigh = after(st_weigh, 1);
-        vote = weigh(pb ^ 1);
-      }
-      if (tick(vote)) move_references(pb ^ 1);
-      if (t >= 1) add_weights();
-    };
-#pragma unroll 1
-    for (int t = 0; t <= count; ++t) {
-      if (t < 2 || t == count) {
-        any_tick(t);
+    }
+    if (!healthy) __nanosleep(1000000);  // what is under way to shared memory arrives before the CTA's end
+    __syncwarp();
+  } else if (tid >= kTokens) {
+    // ================= adding warps: D / 8 latent columns each =================
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(C::ADD_REGS));
+    const int w = warp - kTokenWarps, g = lane >> 2, j = lane & 3;
+    const int own = w * NG / kAddWarps;  // the group of the warp's columns
+    // Offsets of the lane's ldmatrix rows from a 1024-byte boundary.  Chunk c of a row lies at c ^ row % 8, so
+    // chunk c ^ x is at the address ^ 16 x.
+    const uint32_t add_off = (w * CH / 8) * 8192 + sw128(lane, (w * CH) & 7);
+    const uint32_t base = smem_u32(smem), p_base = base + C::OFF_P + own * (NH * C::PTILE) + lane * 16;
+    int done = 0, turn = 0, lap = 0, slot = 0, p_slot = 0;  // tiles % 3, / 3; pages % PAGES, % 3
+    while (done < n_units) {
+      const int seg_pages = pages_of(a, seg_b);
+      if (seg_pages == 0) {
+        ++seg_b;
         continue;
       }
-      const int pb = t & 1;
-      float own_s[NH][2];
+      const bool first = done == 0;
+      const int count = min(seg_pages - seg_p, n_units - done);
+      // accumulators: tile 2 c + h of chunk c holds columns 4 g + 2 h (and that + 16 times the next one) x rows 2 j, + 1
+      float acc[2 * CH][NH][4];
 #pragma unroll
-      for (int n = 0; n < NH; ++n) own_s[n][0] = mine_s[n][0], own_s[n][1] = mine_s[n][1];
-      score(st_score, pb);
-      gather(st_add, pb, 0);
-      gather(st_add, pb, 1);
-      join(st_weigh, pb ^ 1, seg_p + t - 1, own_s);
-      const bool vote = weigh(pb ^ 1);
-      st_score = after(st_score, 1), st_weigh = after(st_weigh, 1), st_add = after(st_add, 1);
-      if (tick(vote)) move_references(pb ^ 1);
-      add_weights();
-    }
-    gather(st_add, (count - 1) & 1, 0);
-    gather(st_add, (count - 1) & 1, 1);
-    stage = st_score;
-    done += count;
-    // ---- the rows' results ----
+      for (int c = 0; c < 2 * CH; ++c)
 #pragma unroll
-    for (int n = 0; n < NH; ++n)
+        for (int n = 0; n < NH; ++n) acc[c][n][0] = acc[c][n][1] = acc[c][n][2] = acc[c][n][3] = 0.f;
+      for (int p = 0; p < count; p += 2) {
+        wait_for(&weighed[turn], lap);
+        __syncwarp();
+        if (sh.moved[turn]) {
+          const float ku = sh.keep_unit[turn][own];
 #pragma unroll
-      for (int x = 0; x < 2; ++x) {
-        const float l = oct_sum(l_sum[n][x]);
-        if (g == 0) sh.red_l[warp][8 * n + 2 * j + x] = l;
+          for (int n = 0; n < NH; ++n) {
+            const float2 k = *reinterpret_cast<const float2*>(&sh.keep[turn][8 * n + 2 * j]);
 #pragma unroll
-        for (int k = 0; k < NG; ++k) {
-          const float z = oct_sum(zsum[n][x][k]);
-          if (g == 0) sh.red_z[warp][k][8 * n + 2 * j + x] = z;
-        }
-      }
-    tick(false);
-    for (int i = tid; i < ROWS * (NG + 1); i += kWorkers) {
-      const int at = i % ROWS, k = i / ROWS - 1;
-      float s = 0.f;
-#pragma unroll
-      for (int w = 0; w < kWarps; ++w) s += k < 0 ? sh.red_l[w][at] : sh.red_z[w][max(k, 0)][at];
-      if (k < 0) sh.l_all[at] = s;
-      else sh.z_all[k][at] = s;
-    }
-    work_sync();
-    const bool whole = seg_p == 0 && count == seg_pages;
-    if (tid == 0 && block == 0 && seg_p == 0) {  // the run that begins a request says how it is cut
-      const Runs again(run_total, groups);
-      const int64_t page0 = run_begin + (done - count);
-      part.cut[seg_b] = whole ? make_int4(0, 0, 0, 0)
-                              : make_int4(group, again.holding(page0 + seg_pages - 1) - group + 1, run_begin < page0, 0);
-    }
-    float u = unit[0];
-#pragma unroll
-    for (int k = 1; k < NG; ++k) u = own == k ? unit[k] : u;
-    const float inv_u = 1.f / u;
-    // a cut request's partial: slot 0 where the run begins in (or with) this request, else 1
-    const int64_t slot = (static_cast<int64_t>(2 * group + (first ? 0 : 1)) * blocks + block) * ROWS;
-#pragma unroll
-    for (int n = 0; n < NH; ++n)
-#pragma unroll
-      for (int x = 0; x < 2; ++x) {
-        const int at = 8 * n + 2 * j + x, row = row0 + at;
-        const float l = sh.l_all[at], z = sh.z_all[own][at];
-        const float inv = l == 0.f ? 0.f : inv_u / l;
-        const float lse = l == 0.f ? -INFINITY : ((x ? max_of(n).y : max_of(n).x) + log2f(l)) * kLn2;
-        const bool live = row < rows;
-        const int t = live ? row / a.heads : 0, h = live ? row % a.heads : 0;
-        uint16_t* out = a.out + seg_b * a.o_sb + t * a.o_st + h * a.o_sh;
-        float* out_part = part.o + (slot + at) * D;
-#pragma unroll
-        for (int c = 0; c < CH; ++c) {
-          const int col = 32 * (warp * CH + c) + 4 * g;
-          float v[4];
-#pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            const float even = acc[2 * c + i][n][x], both = acc[2 * c + i][n][x + 2];
-            v[2 * i] = fmaf(even, 16777216.f, -z) * inv;
-            v[2 * i + 1] = fmaf(both - even, 1048576.f, -z) * inv;
+            for (int c = 0; c < 2 * CH; ++c) {
+              acc[c][n][0] *= k.x * ku, acc[c][n][2] *= k.x * ku;
+              acc[c][n][1] *= k.y * ku, acc[c][n][3] *= k.y * ku;
+            }
           }
-          if (!whole) *reinterpret_cast<float4*>(out_part + col) = make_float4(v[0], v[1], v[2], v[3]);
-          else if (live) *reinterpret_cast<uint2*>(out + col) = make_uint2(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]));
         }
-        if (warp == 0 && g == 0) {
-          if (!whole) part.lse[slot + at] = lse;
-          else if (live && a.lse) a.lse[static_cast<int64_t>(seg_b) * rows + row] = lse;
+#pragma unroll 1
+        for (int i = 0; i < min(2, count - p); ++i) {
+          const uint32_t st = base + slot * C::CODES + add_off, ps = p_base + p_slot * C::PBUF;
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {  // 32 tokens
+            uint32_t x[CH][4], pf[NH][4];
+#pragma unroll
+            for (int c = 0; c < CH; ++c) ldsm_x4_t((st + h * 4096) ^ (c << 4), x[c]);
+#pragma unroll
+            for (int n = 0; n < NH; ++n) ldsm_x4_t(ps + n * C::PTILE + h * 512, pf[n]);
+#pragma unroll
+            for (int k = 0; k < 2; ++k)
+#pragma unroll
+              for (int c = 0; c < CH; ++c) {
+                // of four elements e: e0 over e0 + 16 e1, e2 over e2 + 16 e3
+                const uint32_t u = x[c][2 * k], v = x[c][2 * k + 1], u8 = odd_bytes(u), v8 = odd_bytes(v);
+                const uint32_t even[4] = {u & 0x000F000Fu, u & 0x00FF00FFu, v & 0x000F000Fu, v & 0x00FF00FFu};
+                const uint32_t odd[4] = {u8 & 0x000F000Fu, u8, v8 & 0x000F000Fu, v8};
+#pragma unroll
+                for (int n = 0; n < NH; ++n) mma_f16(acc[2 * c][n], even, pf[n][2 * k], pf[n][2 * k + 1]);
+#pragma unroll
+                for (int n = 0; n < NH; ++n) mma_f16(acc[2 * c + 1][n], odd, pf[n][2 * k], pf[n][2 * k + 1]);
+              }
+          }
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&page_free[slot]);
+          if (++slot == PAGES) slot = 0;
+          if (++p_slot == C::WEIGHTS) p_slot = 0;
+        }
+        if (++turn == 3) turn = 0, ++lap;
+      }
+      done += count;
+      // ---- the rows' results ----
+      named_bar_sync(kBarSums, kTokens + kAdders);
+      const bool whole = seg_p == 0 && count == seg_pages;
+      if (tid == kTokens && block == 0 && seg_p == 0) {  // the run that begins a request says how it is cut
+        const Runs again(total, groups);
+        const int64_t page0 = u0 + (done - count);
+        part.cut[seg_b] = whole ? make_int4(0, 0, 0, 0)
+                                : make_int4(group, again.holding(page0 + seg_pages - 1) - group + 1, u0 < page0, 0);
+      }
+      const float inv_u = 1.f / sh.unit_out[own];
+      // a cut request's partial: slot 0 where the run begins in (or with) this request, else 1
+      const int64_t slot = (static_cast<int64_t>(2 * group + (first ? 0 : 1)) * blocks + block) * ROWS;
+#pragma unroll
+      for (int n = 0; n < NH; ++n)
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+          const int at = 8 * n + 2 * j + x, row = row0 + at;
+          float l = 0.f, z = 0.f;
+#pragma unroll
+          for (int k = 0; k < 4; ++k) l += sh.l[k][at], z += sh.z[k][own][at];
+          const float inv = l == 0.f ? 0.f : inv_u / l;
+          const float lse = l == 0.f ? -INFINITY : (sh.max_out[at] + log2f(l)) * kLn2;
+          const bool live = row < rows;
+          const int t = live ? row / a.heads : 0, h = live ? row % a.heads : 0;
+          uint16_t* out = a.out + seg_b * a.o_sb + t * a.o_st + h * a.o_sh;
+          float* out_part = part.o + (slot + at) * D;
+#pragma unroll
+          for (int c = 0; c < CH; ++c) {
+            const int col = 32 * (w * CH + c) + 4 * g;
+            float v[4];
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+              const float even = acc[2 * c + i][n][x], sum = acc[2 * c + i][n][x + 2];
+              v[2 * i] = fmaf(even, 16777216.f, -z) * inv;
+              v[2 * i + 1] = fmaf(sum - even, 1048576.f, -z) * inv;
+            }
+            if (!whole) *reinterpret_cast<float4*>(out_part + col) = make_float4(v[0], v[1], v[2], v[3]);
+            else if (live) *reinterpret_cast<uint2*>(out + col) = make_uint2(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]));
+          }
+          if (w == 0 && g == 0) {
+            if (!whole) part.lse[slot + at] = lse;
+            else if (live && a.lse) a.lse[static_cast<int64_t>(seg_b) * rows + row] = lse;
+          }
+        }
+      bar_arrive(kBarTaken, kTokens + kAdders);
+      ++seg_b;
+      seg_p = 0;
+    }
+  } else {
+    // ================= token warps: thread (token of the tile, half of the columns and of the rows) =================
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(C::TOKEN_REGS));
+    const int quarter = warp & 3, half = warp >> 2, token = 32 * quarter + lane;
+    const int n0 = half * HT, my_tiles = half == 0 ? HT : NH - HT;  // tiles of 8 rows
+    const uint32_t lanes = static_cast<uint32_t>(32 * quarter) << 16;
+    const float qk_scale = a.sm_scale * kLog2e;
+    const char* token_params = smem + C::OFF_PARAMS + (token & 63) * (NG * 8);
+    int done = 0, tile = 0, turn = 0;  // turn: tiles % 3
+    bool begun = false;
+
+    // The codes of tile `to` as E4M3 bytes to TMEM: of each word of 8 the even elements, then the odd ones; the thread has
+    // half the columns of a token.  `page`: its page, counted over the run.
+    const char* token_codes = smem + (D == 512 ? half * 8192 : 0) + (token & 63) * 128;
+    auto bring_codes = [&](int to, int page) {
+      const int at = page % PAGES;
+      wait_for(&full[at], page / PAGES);
+      __syncwarp();
+      const uint32_t dst = tmem + lanes + (to & 1) * C::T_CODES + half * (D / 8);
+      const char* src = token_codes + at * C::CODES;
+#pragma unroll
+      for (int c0 = 0; c0 < D / 64; c0 += 4) {
+        uint4 v[4];
+#pragma unroll
+        for (int c = 0; c < 4; ++c)
+          v[c] = *reinterpret_cast<const uint4*>(src + ((((D == 512 ? 0 : 4 * half) + c0 + c) ^ (token & 7)) << 4));
+#pragma unroll
+        for (int c = 0; c < 4; c += 2) {
+          const uint32_t x[8] = {v[c].x, v[c].y, v[c].z, v[c].w, v[c + 1].x, v[c + 1].y, v[c + 1].z, v[c + 1].w};
+          uint32_t r[16];
+#pragma unroll
+          for (int k = 0; k < 8; ++k) r[2 * k] = x[k] & 0x0F0F0F0Fu, r[2 * k + 1] = (x[k] >> 4) & 0x0F0F0F0Fu;
+          tmem_st16(dst + 8 * (c0 + c), r);
         }
       }
+      tmem_wait_st();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&coded[to & 1]);
+    };
+    // The page of the thread's token of a tile that begins with `page` and has n (where there is no second, the first).
+    auto own_page = [&](int page, int n) { return page + (token >= kPage && n > 1); };
 
-    ++seg_b;
-    seg_p = 0;
+    while (done < n_units) {
+      const int seg_pages = pages_of(a, seg_b);
+      if (seg_pages == 0) {
+        ++seg_b;
+        continue;
+      }
+      const int count = min(seg_pages - seg_p, n_units - done);
+      const int len = min(static_cast<int64_t>(a.seq_lens[seg_b]), static_cast<int64_t>(a.max_pages) * kPage);
+      if (tid == 0 && len != a.seq_lens[seg_b]) report(a.err, ROLAQ_DEV_BAD_REQ);
+      const int lim_min = len - a.q_len + 1;
+
+      // ---- the query: a row a warp at a time; the last tile's products are done with the one before ----
+#pragma unroll 1
+      for (int r = warp; r < C::NQ; r += kTokenWarps) {
+        const int row = row0 + r;
+        const bool live = r < ROWS && row < rows;
+        const int t = live ? row / a.heads : 0, h = live ? row % a.heads : 0;
+        const uint16_t* src = a.q + seg_b * a.q_sb + t * a.q_st + h * a.q_sh;
+        // lane: words (8 elements) lane and, for D = 512, lane + 32
+        uint4 w[D / 256], pe = make_uint4(0, 0, 0, 0);
+#pragma unroll
+        for (int i = 0; i < D / 256; ++i) w[i] = live ? *reinterpret_cast<const uint4*>(src + 8 * (lane + 32 * i)) : pe;
+        if (live && lane < DR / 8) pe = *reinterpret_cast<const uint4*>(src + D + 8 * lane);
+        if (lane < DR / 8) {
+          const uint32_t off = DR == 64 ? (r >> 3) * 1024 + sw128(r & 7, lane) : (r >> 3) * 512 + sw64(r & 7, lane);
+          *reinterpret_cast<uint4*>(smem + C::OFF_QPE + off) = pe;
+        }
+        if (r >= ROWS) continue;
+        float top = 0.f, odd = 0.f;
+#pragma unroll
+        for (int i = 0; i < D / 256; ++i) {
+          const uint32_t v[4] = {w[i].x, w[i].y, w[i].z, w[i].w};
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            top = fmaxf(top, fmaxf(fabsf(bf16_lo(v[k])), fabsf(bf16_hi(v[k]))));
+            odd = fmaf(bf16_lo(v[k]), 0.f, fmaf(bf16_hi(v[k]), 0.f, odd));  // NaN where an element is no finite number
+          }
+        }
+        top = warp_max_f32(odd != 0.f ? INFINITY : top);
+        // 2^k with top 2^k in [2^7, 2^8)
+        const float up = top > 0.f ? pow2(min(max(7 - (static_cast<int>(__float_as_uint(top) >> 23) - 127), -100), 100)) : 1.f;
+        if (lane == 0) sh.row_scale[r] = top == INFINITY ? __int_as_float(0x7FC00000) : qk_scale * (512.f / up);
+#pragma unroll
+        for (int i = 0; i < D / 256; ++i) {
+          const uint32_t v[4] = {w[i].x, w[i].y, w[i].z, w[i].w};
+          uint32_t hi[2], lo[2];  // even elements, odd elements
+          float sum = 0.f;
+          float x[8];
+#pragma unroll
+          for (int k = 0; k < 4; ++k) x[2 * k] = bf16_lo(v[k]) * up, x[2 * k + 1] = bf16_hi(v[k]) * up;
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const uint32_t h0 = f32x2_to_e4m3x2(x[e], x[e + 2]), h1 = f32x2_to_e4m3x2(x[e + 4], x[e + 6]);
+            const float2 f0 = __half22float2(e4m3x2_to_half2(h0)), f1 = __half22float2(e4m3x2_to_half2(h1));
+            const uint32_t l0 = f32x2_to_e4m3x2(x[e] - f0.x, x[e + 2] - f0.y), l1 = f32x2_to_e4m3x2(x[e + 4] - f1.x, x[e + 6] - f1.y);
+            const float2 s0 = __half22float2(e4m3x2_to_half2(l0)), s1 = __half22float2(e4m3x2_to_half2(l1));
+            sum += ((f0.x + s0.x) + (f0.y + s0.y)) + ((f1.x + s1.x) + (f1.y + s1.y));
+            hi[e] = h0 | h1 << 16, lo[e] = l0 | l1 << 16;
+          }
+          const int word = lane + 32 * i, k = word / 16, at = word % 16;  // 8 bytes of the group's 128
+          char* dst = smem + C::OFF_QB + k * C::QB_GROUP + (r >> 3) * 1024 + sw128(r & 7, at >> 1) + 8 * (at & 1);
+          *reinterpret_cast<uint2*>(dst) = make_uint2(hi[0], hi[1]);
+          *reinterpret_cast<uint2*>(dst + NG * C::QB_GROUP) = make_uint2(lo[0], lo[1]);
+#pragma unroll
+          for (int o = 1; o < 16; o *= 2) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, o);
+          if ((lane & 15) == 0) sh.q_sum[k][r] = sum * (1.f / 512.f);
+        }
+      }
+      if (tid < ROWS) sh.max[tid] = kNoMax;
+      fence_proxy_async();
+      token_sync();
+      if (tid == 0) mbar_arrive(&q_ready);
+
+      float2 l_sum[HT][4], zsum[NG][HT][4];
+      float unit[NG];
+#pragma unroll
+      for (int n = 0; n < HT; ++n)
+#pragma unroll
+        for (int x = 0; x < 4; ++x) {
+          l_sum[n][x] = both(0.f);
+#pragma unroll
+          for (int k = 0; k < NG; ++k) zsum[k][n][x] = both(0.f);
+        }
+#pragma unroll
+      for (int k = 0; k < NG; ++k) unit[k] = kNoUnit;
+      const int tiles = (count + 1) / 2;
+      bring_codes(tile, own_page(done, count));
+      for (int i = 0; i < tiles; ++i, ++tile) {
+        const int n_pages = min(2, count - 2 * i), page = own_page(done + 2 * i, n_pages), at = page % PAGES;
+        const bool here = (token >> 6) < n_pages;
+        if (i + 1 < tiles) bring_codes(tile + 1, own_page(done + 2 * i + 2, count - 2 * i - 2));
+        float s_tok[NG], z_tok[NG];
+        {
+          const float4* par = reinterpret_cast<const float4*>(token_params + at * C::PARAMS);
+#pragma unroll
+          for (int k = 0; k < NG; k += 2) {
+            const float4 v = par[k / 2];
+            s_tok[k] = v.x, z_tok[k] = v.y, s_tok[k + 1] = v.z, z_tok[k + 1] = v.w;
+          }
+        }
+        // ---- scores of the thread's rows, in log2 units ----
+        wait_for(&scored[tile & 1], tile >> 1);
+        __syncwarp();
+        tc_fence_after();
+        float2 s_val[HT][4];
+        const uint32_t sums = tmem + lanes + C::T_SUM + (tile & 1) * C::T_TILE + 8 * n0;
+#pragma unroll
+        for (int n = 0; n < HT; ++n)
+          if (n < my_tiles) {
+            uint32_t pe[8];
+            float2 sum[4] = {both(0.f), both(0.f), both(0.f), both(0.f)};
+#pragma unroll
+            for (int k0 = 0; k0 < NG; k0 += 2) {
+              uint32_t d[2][8];
+              tmem_ld8(sums + k0 * C::NQ + 8 * n, d[0]);
+              tmem_ld8(sums + (k0 + 1) * C::NQ + 8 * n, d[1]);
+              if (k0 == 0) tmem_ld8(sums + C::T_ROPE + 8 * n, pe);
+              tmem_wait_ld();
+              reg_fence(d[0]);
+              reg_fence(d[1]);
+              if (k0 == 0) reg_fence(pe);
+#pragma unroll
+              for (int k = k0; k < k0 + 2; ++k)
+#pragma unroll
+                for (int x = 0; x < 4; ++x) {
+                  const float2 dot = make_float2(__uint_as_float(d[k - k0][2 * x]), __uint_as_float(d[k - k0][2 * x + 1]));
+                  const float2 qs = *reinterpret_cast<const float2*>(&sh.q_sum[k][8 * (n0 + n) + 2 * x]);
+                  sum[x] = fma2(both(s_tok[k]), fma2(both(-z_tok[k]), qs, dot), sum[x]);
+                }
+            }
+#pragma unroll
+            for (int x = 0; x < 4; ++x) {
+              const float2 scale = *reinterpret_cast<const float2*>(&sh.row_scale[8 * (n0 + n) + 2 * x]);
+              const float2 rope = make_float2(__uint_as_float(pe[2 * x]), __uint_as_float(pe[2 * x + 1]));
+              s_val[n][x] = fma2(rope, both(qk_scale), mul2(sum[x], scale));
+            }
+          }
+        const int pos = (seg_p + 2 * i) * kPage + token;
+        const bool bad = bad_page[at] != 0;
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&taken[tile & 1]);
+        if (__any_sync(0xFFFFFFFFu, pos >= lim_min || bad || !here)) {
+          // the request's or the run's end, or a page that is not there
+          const bool none = bad || !here || pos >= len;
+          if (none)
+#pragma unroll
+            for (int k = 0; k < NG; ++k) s_tok[k] = z_tok[k] = 0.f;
+#pragma unroll
+          for (int n = 0; n < HT; ++n)
+#pragma unroll
+            for (int x = 0; x < 4; ++x) {
+              const int row = row0 + 8 * (n0 + n) + 2 * x;
+              if (none || pos >= lim_min + row / a.heads) s_val[n][x].x = -INFINITY;
+              if (none || pos >= lim_min + (row + 1) / a.heads) s_val[n][x].y = -INFINITY;
+            }
+        }
+        if (here && page >= C::WEIGHTS) wait_for(&page_free[(page - C::WEIGHTS) % PAGES], (page - C::WEIGHTS) / PAGES);
+        __syncwarp();
+
+        // Weights against the present references, times each group's scale, to shared memory; true where a
+        // weight or a scale has left its reference behind (their sums: moving early does no harm), or is NaN.
+        float2 p_val[HT][4];
+        auto weigh = [&]() {
+          float2 weights = both(0.f);
+          float sizes = 0.f;
+#pragma unroll
+          for (int n = 0; n < HT; ++n)
+            if (n < my_tiles) {
+#pragma unroll
+              for (int x = 0; x < 4; ++x) {
+                const float2 m = *reinterpret_cast<const float2*>(&sh.max[8 * (n0 + n) + 2 * x]);
+                const float2 d = add2(s_val[n][x], make_float2(-m.x, -m.y));
+                p_val[n][x] = make_float2(ex2_approx(d.x), ex2_approx(d.y));
+                weights = add2(weights, p_val[n][x]);
+              }
+            }
+          char* dst = smem + C::OFF_P + (page % C::WEIGHTS) * C::PBUF + n0 * C::PTILE + (token & 63) * 16;
+#pragma unroll
+          for (int k = 0; k < NG; ++k) {
+            const float s = s_tok[k] * unit[k];
+            sizes += fabsf(s);
+#pragma unroll
+            for (int n = 0; n < HT; ++n)
+              if (n < my_tiles) {
+                uint32_t h[4];
+#pragma unroll
+                for (int x = 0; x < 4; ++x) {
+                  const float2 v = mul2(p_val[n][x], both(s));
+                  h[x] = pack_half2(v.x, v.y);
+                }
+                if (here) *reinterpret_cast<uint4*>(dst + (k * NH + n) * C::PTILE) = make_uint4(h[0], h[1], h[2], h[3]);
+              }
+          }
+          return !(weights.x + weights.y <= kSlack) || !(sizes <= kScaleSlack);
+        };
+        const bool move = token_any(weigh());
+        if (move) {  // new references: the tile's maxima; the sums so far are brought to them
+#pragma unroll
+          for (int n = 0; n < HT; ++n)
+            if (n < my_tiles) {
+#pragma unroll
+              for (int x = 0; x < 4; ++x) {
+                const float m0 = warp_max_f32(s_val[n][x].x), m1 = warp_max_f32(s_val[n][x].y);
+                if (lane == 0) *reinterpret_cast<float2*>(&sh.red_m[quarter][8 * (n0 + n) + 2 * x]) = make_float2(m0, m1);
+              }
+            }
+#pragma unroll
+          for (int k = 0; k < NG; ++k) {
+            const float s = warp_max_f32(fabsf(s_tok[k]));
+            if (lane == 0 && half == 0) sh.red_s[quarter][k] = s;
+          }
+          token_sync();
+          float keep_unit[NG];
+#pragma unroll
+          for (int k = 0; k < NG; ++k) {
+            const float s = fmaxf(fmaxf(sh.red_s[0][k], sh.red_s[1][k]), fmaxf(sh.red_s[2][k], sh.red_s[3][k]));
+            keep_unit[k] = 1.f;
+            if (s * unit[k] > 2.f) {  // bring the largest scale into [1, 2)
+              const float u = pow2(min(max(127 - static_cast<int>(__float_as_uint(s) >> 23), -100), 100));
+              keep_unit[k] = u / unit[k];
+              unit[k] = u;
+            }
+            if (tid == 0) sh.keep_unit[turn][k] = keep_unit[k];
+          }
+          if (tid < ROWS) {
+            const float old = sh.max[tid];
+            const float m = fmaxf(old, fmaxf(fmaxf(sh.red_m[0][tid], sh.red_m[1][tid]), fmaxf(sh.red_m[2][tid], sh.red_m[3][tid])));
+            sh.keep[turn][tid] = ex2_approx(old - m);
+            sh.max[tid] = m;
+          }
+          token_sync();
+#pragma unroll
+          for (int n = 0; n < HT; ++n)
+            if (n < my_tiles) {
+#pragma unroll
+              for (int x = 0; x < 4; ++x) {
+                const float2 keep = *reinterpret_cast<const float2*>(&sh.keep[turn][8 * (n0 + n) + 2 * x]);
+                l_sum[n][x] = mul2(l_sum[n][x], keep);
+#pragma unroll
+                for (int k = 0; k < NG; ++k) zsum[k][n][x] = mul2(zsum[k][n][x], mul2(keep, both(keep_unit[k])));
+              }
+            }
+          weigh();
+          token_sync();
+        }
+        if (tid == 0) {
+          sh.moved[turn] = move;
+          mbar_arrive(&weighed[turn]);
+        }
+        if (++turn == 3) turn = 0;
+        // ---- the denominators and the zeros' share ----
+#pragma unroll
+        for (int n = 0; n < HT; ++n)
+          if (n < my_tiles) {
+#pragma unroll
+            for (int x = 0; x < 4; ++x) {
+              l_sum[n][x] = add2(l_sum[n][x], p_val[n][x]);
+#pragma unroll
+              for (int k = 0; k < NG; ++k) zsum[k][n][x] = fma2(p_val[n][x], both(s_tok[k] * unit[k] * z_tok[k]), zsum[k][n][x]);
+            }
+          }
+      }
+      done += count;
+      // ---- the request's sums, for the adding warps ----
+      if (begun) named_bar_sync(kBarTaken, kTokens + kAdders);  // they have taken the last request's
+      begun = true;
+#pragma unroll
+      for (int n = 0; n < HT; ++n)
+        if (n < my_tiles) {
+#pragma unroll
+          for (int x = 0; x < 4; ++x) {
+            const int at = 8 * (n0 + n) + 2 * x;
+            const float2 l = make_float2(warp_sum(l_sum[n][x].x), warp_sum(l_sum[n][x].y));
+            if (lane == 0) *reinterpret_cast<float2*>(&sh.l[quarter][at]) = l;
+#pragma unroll
+            for (int k = 0; k < NG; ++k) {
+              const float2 z = make_float2(warp_sum(zsum[k][n][x].x), warp_sum(zsum[k][n][x].y));
+              if (lane == 0) *reinterpret_cast<float2*>(&sh.z[quarter][k][at]) = z;
+            }
+          }
+        }
+      if (tid < ROWS) sh.max_out[tid] = sh.max[tid];
+      if (tid == 0)
+#pragma unroll
+        for (int k = 0; k < NG; ++k) sh.unit_out[k] = unit[k];
+      bar_arrive(kBarSums, kTokens + kAdders);
+      ++seg_b;
+      seg_p = 0;
+    }
+    if (begun) named_bar_sync(kBarTaken, kTokens + kAdders);
   }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  if (warp == 0) tmem_dealloc(tmem, 512);
 }
 
 constexpr int kMergeWarps = 8, kMergeThreads = kMergeWarps * 32;
