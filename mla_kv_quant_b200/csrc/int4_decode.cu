@@ -9,20 +9,26 @@
 //     one FP32 sum a group; the rotary part BF16 by BF16.  Asynchronous: no warp's issue slots go into it.
 //   - sums: the FP16 patterns 0..255 are that many 2^-24 exactly.  mma.sync m16n8k16 with the codes as rows (c of an
 //     even element, and c + 16 c' of it and the next: c' comes out at the end) and P s in FP16 as columns.
-// All sums are FP32.  mma.sync blocks a scheduler's other warps while it runs (8 cycles each, measured), so only what
-// tcgen05 could not do with fewer shared-memory bytes - the product that needs the codes transposed - is left to it.
+// All sums are FP32.
 //
 // A CTA holds NH tiles of 8 query rows (query tokens x heads; up to two for D = 512, five for D = 256) and walks the
 // pages of one or more requests, two (a tile of 128 tokens) at a time:
-//   - a loading warp brings pages by TMA (128-byte swizzle); one thread issues the tcgen05 products;
-//   - eight token warps, two threads a token: codes to TMEM, scores from TMEM, the softmax against references that
-//     move only when weights pass them by 2^10, P s of each group to shared memory.  A vote a tile moves the
-//     references; a move leaves the factors for the sums beside the weights;
+//   - two loading warps bring codes with params, and rotary parts, by TMA (128-byte swizzle);
+//   - eight token warps, two threads a token: codes to TMEM (a tile ahead), scores from TMEM, the softmax against
+//     references that move only when weights pass them by 2^10, P s of each group to shared memory.  A vote a tile
+//     moves the references; a move leaves the factors for the sums beside the weights;
+//   - one warp issues the tcgen05 products of a tile as soon as its codes are there;
 //   - eight adding warps hold D/8 latent columns of the result each.
-// The roles meet in mbarriers only, each a tile ahead of the next.
+// The roles meet in mbarriers only.  The pages of all requests are dealt to the CTAs in one equal run each (a run may
+// begin or end inside a request); what is cut is joined by merge_kernel by log-sum-exp.
 //
-// The pages of all requests are dealt to the CTAs in one equal run each (a run may begin or end inside
-// a request); what is cut is joined by merge_kernel by log-sum-exp.
+// Measured, 16 heads of 512 + 64, 64 requests of about 16K tokens (417 MB): 135 us, 3.1 TB/s, 47% of a copy's rate.  What
+// bounds it is the schedulers: a tile costs each of them about 2000 instructions and 128 mma.sync, and an mma.sync holds
+// back all else for 8 cycles (HMMA + n logic + m FP32 instructions measured 8 + 0.9 n + 1.2 m cycles), 2900 of the 3900
+// cycles a tile takes; memory alone would take 2050.  With the scores on mma.sync too it was 160 us.  Slower, in the same
+// setting: four warps more that only bring codes (179), the adding warps bringing them (166), sharing that (152); one
+// thread of a divergent branch issuing (167: 2000 cycles for 20 products, against 300 by an elected lane of a warp whose
+// operands are the same in all lanes).
 #include <algorithm>
 #include <atomic>
 
@@ -37,9 +43,8 @@ namespace {
 // block of 640 is launched with, the others hand some to the token warps.
 constexpr int kTokenWarps = 8, kAddWarps = 8;
 constexpr int kTokens = kTokenWarps * 32, kAdders = kAddWarps * 32, kThreads = kTokens + kAdders + 128;
-constexpr int kTile = 2 * kPage;  // tokens of a tile
-constexpr int kAhead = 12;    // pages ahead of their loads that they are called to L2
-constexpr int kMinPages = 2;  // least run of pages worth a CTA of its own
+constexpr int kAhead = 4;         // pages ahead of their loads that they are called to L2 (24: 143 us against 134)
+constexpr int kMinPages = 2;      // least run of pages worth a CTA of its own
 constexpr float kSlack = 1024.f, kScaleSlack = 32.f;  // how far weights and scales may pass their references (P s <= 2^15)
 constexpr float kNoMax = -1e30f, kNoUnit = 1.329227995784916e36f;  // references not yet set: the first token passes them
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
@@ -64,7 +69,7 @@ struct Cfg {
   static constexpr int HT = (NH + 1) / 2;           // tiles of 8 rows of a token thread
   // TMEM columns: two tiles' codes; two tiles' scores (the groups' sums, the rotary part's)
   static constexpr int T_CODES = D / 4, T_SUM = 2 * T_CODES, T_ROPE = NG * NQ, T_TILE = (NG + 1) * NQ;
-  static constexpr int TOKEN_REGS = 136, ADD_REGS = 80, LOAD_REGS = 48;
+  static constexpr int TOKEN_REGS = NH < 5 ? 136 : 144, ADD_REGS = 80, LOAD_REGS = NH < 5 ? 48 : 32;
   static_assert(T_SUM + 2 * T_TILE <= 512 && 2 * TOKEN_REGS + 2 * ADD_REGS + LOAD_REGS <= 5 * 96, "TMEM, registers");
 };
 
@@ -117,10 +122,20 @@ __device__ __forceinline__ float2 add2(float2 a, float2 b) {
   return *reinterpret_cast<float2*>(&d);
 }
 __device__ __forceinline__ float2 both(float x) { return make_float2(x, x); }
-__device__ __forceinline__ float warp_sum(float v) {
+// Eight values summed over the warp: lane l gets the sum of value l % 8.
+__device__ __forceinline__ float warp_sums(const float2 (&pairs)[4]) {
+  const int lane = threadIdx.x & 31;
+  float v[8];
 #pragma unroll
-  for (int o = 16; o >= 1; o /= 2) v += __shfl_xor_sync(0xFFFFFFFFu, v, o);
-  return v;
+  for (int i = 0; i < 4; ++i) v[2 * i] = pairs[i].x, v[2 * i + 1] = pairs[i].y;
+#pragma unroll
+  for (int h = 4; h >= 1; h /= 2) {
+    const bool up = lane & h;
+#pragma unroll
+    for (int i = 0; i < h; ++i) v[i] = (up ? v[i + h] : v[i]) + __shfl_xor_sync(0xFFFFFFFFu, up ? v[i] : v[i + h], h);
+  }
+  v[0] += __shfl_xor_sync(0xFFFFFFFFu, v[0], 8);
+  return v[0] + __shfl_xor_sync(0xFFFFFFFFu, v[0], 16);
 }
 
 __device__ __forceinline__ int pages_of(const DecodeArgs& a, int b) {
@@ -227,6 +242,10 @@ __global__ void __launch_bounds__(kThreads, 1)
     prefetch_tensormap(&map_codes);
     prefetch_tensormap(&map_rope);
   }
+  if (warp == 0) {
+    tmem_alloc(&tmem_slot, 512);
+    tmem_relinquish();
+  }
   grid_launch_dependents();
   grid_dependency_wait();
 
@@ -245,7 +264,10 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
   }
   const Runs runs(total, groups);
-  if (group >= runs.n || total == 0) return;
+  if (group >= runs.n || total == 0) {
+    if (warp == 0) tmem_dealloc(tmem_slot, 512);
+    return;
+  }
   const int64_t u0 = runs.begin(group);
   const int n_units = static_cast<int>(runs.begin(group + 1) - u0);
   if (before <= u0 && u0 < before + mine) {
@@ -253,10 +275,6 @@ __global__ void __launch_bounds__(kThreads, 1)
     for (int n; before + (n = pages_of(a, b)) <= u0; ++b) before += n;
     start[0] = b;
     start[1] = static_cast<int>(u0 - before);
-  }
-  if (warp == 0) {
-    tmem_alloc(&tmem_slot, 512);
-    tmem_relinquish();
   }
   tc_fence_before();
   __syncthreads();
@@ -274,10 +292,10 @@ __global__ void __launch_bounds__(kThreads, 1)
     constexpr int first_warp = kTokenWarps + kAddWarps;
     if (warp <= first_warp + 1) {
       // ================= the loading warps: codes and params by pages; rotary parts by tiles =================
-      // Lane l holds the id of page `base` + l of the run; the next 32 are requested 32 pages ahead of their use.
+      // Lane l holds the id of page l of 32; the next 32 are requested 32 pages ahead of their use.
       const bool codes = warp == first_warp;
       const int pool_pages = static_cast<int>(a.cache.num_slots / kPage);
-      int id_b = seg_b, id_p = seg_p + lane, ids = -1, next_ids = -1, id_q = 0;
+      int id_b = seg_b, id_p = seg_p + lane, ids = -1, next_ids = -1;
       auto fetch_ids = [&](int first) {
         int id = -1;
         if (first + lane < n_units) {
@@ -288,7 +306,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         return id;
       };
       next_ids = fetch_ids(0);
-      int slot = 0, lap = 0, left = 0;  // left: pages of the present request
+      int slot = 0, lap = 0, left = 0, in_tile = 0;  // pages left of the present request, and its page modulo 2
       for (int i = 0; i < n_units; ++i) {
         if ((i & 31) == 0) {
           ids = next_ids;
@@ -297,7 +315,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         const int id = __shfl_sync(0xFFFFFFFFu, ids, i & 31);
         const bool ok = id >= 0 && id < pool_pages;
         const int page = ok ? id : 0;
-        // The rings are a few pages short of covering the way from memory: pages come to L2 ahead of them.
+        // The rings are short of covering the way from memory: pages come to L2 ahead of them.
         const int ahead_id = __shfl_sync(0xFFFFFFFFu, (i & 31) + kAhead < 32 ? ids : next_ids, (i + kAhead) & 31);
         if (lane == 1 && i + kAhead < n_units && ahead_id >= 0 && ahead_id < pool_pages) {
           const int64_t token = static_cast<int64_t>(ahead_id) * kPage;
@@ -323,20 +341,20 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
           if (++slot == PAGES) slot = 0, ++lap;
         } else {
-          if (left == 0) {  // a tile's first page is an even one of its request's share
+          if (left == 0) {
             for (; pages_of(a, seg_b) - seg_p <= 0; seg_p = 0) ++seg_b;
             left = min(pages_of(a, seg_b) - seg_p, n_units - i);
             ++seg_b;
             seg_p = 0;
-            id_q = 0;
+            in_tile = 0;
           }
-          if ((id_q & 1) == 0) {
+          if (in_tile == 0) {
             if (lap > 0) wait_for(&rope_free[slot], lap - 1);
             if (lane == 0) mbar_expect_tx(&rope_full[slot], (left > 1 ? 2 : 1) * C::ROPE);
           }
-          if (lane == 0) tma_load_2d(smem + C::OFF_ROPE + (2 * slot + (id_q & 1)) * C::ROPE, &map_rope, &rope_full[slot], 0, page * kPage);
-          ++id_q, --left;
-          if ((id_q & 1) == 0 || left == 0)
+          if (lane == 0) tma_load_2d(smem + C::OFF_ROPE + (2 * slot + in_tile) * C::ROPE, &map_rope, &rope_full[slot], 0, page * kPage);
+          in_tile ^= 1, --left;
+          if (in_tile == 0 || left == 0)
             if (++slot == TILES) slot = 0, ++lap;
         }
       }
@@ -374,6 +392,17 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
           __syncwarp();
         }
+        done += count;
+      }
+    } else if (block == 0) {
+      // ================= the run that begins a request says how it is cut =================
+      for (int done = 0; done < n_units; ++seg_b, seg_p = 0) {
+        const int pages = pages_of(a, seg_b), count = min(pages - seg_p, n_units - done);
+        if (count <= 0) continue;
+        const int64_t page0 = u0 + done;
+        if (seg_p == 0 && lane == 0)
+          part.cut[seg_b] = count == pages ? make_int4(0, 0, 0, 0)
+                                           : make_int4(group, runs.holding(page0 + pages - 1) - group + 1, u0 < page0, 0);
         done += count;
       }
     }
@@ -453,12 +482,6 @@ __global__ void __launch_bounds__(kThreads, 1)
       // ---- the rows' results ----
       named_bar_sync(kBarSums, kTokens + kAdders);
       const bool whole = seg_p == 0 && count == seg_pages;
-      if (tid == kTokens && block == 0 && seg_p == 0) {  // the run that begins a request says how it is cut
-        const Runs again(total, groups);
-        const int64_t page0 = u0 + (done - count);
-        part.cut[seg_b] = whole ? make_int4(0, 0, 0, 0)
-                                : make_int4(group, again.holding(page0 + seg_pages - 1) - group + 1, u0 < page0, 0);
-      }
       const float inv_u = 1.f / sh.unit_out[own];
       // a cut request's partial: slot 0 where the run begins in (or with) this request, else 1
       const int64_t slot = (static_cast<int64_t>(2 * group + (first ? 0 : 1)) * blocks + block) * ROWS;
@@ -737,7 +760,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
           return !(weights.x + weights.y <= kSlack) || !(sizes <= kScaleSlack);
         };
-        const bool move = token_any(weigh());
+        const bool move = token_any(weigh());  // a request's first tile brings the first references
         if (move) {  // new references: the tile's maxima; the sums so far are brought to them
 #pragma unroll
           for (int n = 0; n < HT; ++n)
@@ -811,16 +834,13 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
       for (int n = 0; n < HT; ++n)
         if (n < my_tiles) {
+          const int row = 8 * (n0 + n) + (lane & 7);
+          const float l = warp_sums(l_sum[n]);
+          if (lane < 8) sh.l[quarter][row] = l;
 #pragma unroll
-          for (int x = 0; x < 4; ++x) {
-            const int at = 8 * (n0 + n) + 2 * x;
-            const float2 l = make_float2(warp_sum(l_sum[n][x].x), warp_sum(l_sum[n][x].y));
-            if (lane == 0) *reinterpret_cast<float2*>(&sh.l[quarter][at]) = l;
-#pragma unroll
-            for (int k = 0; k < NG; ++k) {
-              const float2 z = make_float2(warp_sum(zsum[k][n][x].x), warp_sum(zsum[k][n][x].y));
-              if (lane == 0) *reinterpret_cast<float2*>(&sh.z[quarter][k][at]) = z;
-            }
+          for (int k = 0; k < NG; ++k) {
+            const float z = warp_sums(zsum[k][n]);
+            if (lane < 8) sh.z[quarter][k][row] = z;
           }
         }
       if (tid < ROWS) sh.max_out[tid] = sh.max[tid];
@@ -899,7 +919,9 @@ __global__ void __launch_bounds__(kMergeThreads) merge_kernel(const DecodeArgs a
     a.lse[(static_cast<int64_t>(b) * a.q_len + t) * a.heads + h] = den == 0.f ? -INFINITY : top + logf(den);
 }
 
-// A CTA's tiles of 8 query rows: as few CTAs as hold them all, evenly filled.
+// A CTA's tiles of 8 query rows: as few CTAs as hold them all, evenly filled.  A page is read once for each, so five
+// tiles (40 rows) in one CTA beat three in each of two even though its registers spill a little: 128 requests of 8K,
+// 40 heads of 256 + 32: 185 us against 238.
 struct Shape {
   int tiles, blocks, groups;  // tiles of a CTA, CTAs for all rows, runs of pages (a CTA each and row block)
 };
@@ -956,7 +978,8 @@ int launch(const DecodeArgs& a, const Shape& shape, cudaStream_t s) {
   cfg.numAttrs = 1;
   if (cudaLaunchKernelEx(&cfg, decode_kernel<D, DR, NH>, codes, rope, a, part, groups, blocks) != cudaSuccess) return ROLAQ_ECUDA;
 
-  // Few requests are cut into many partials: all warps of a CTA share a row's then.
+  // Few requests are cut into many partials: all warps of a CTA share 128 columns of a row then (one request of 128K: 37 us
+  // in all); with less than 8 partials a request a warp each is enough and needs no join.
   const bool wide = groups >= 8 * a.batch;
   const int tasks = a.q_len * a.heads * (D / 128), per_cta = wide ? 1 : kMergeWarps;
   cfg.gridDim = dim3((tasks + per_cta - 1) / per_cta, a.batch);
