@@ -390,6 +390,9 @@ int64_t rolaq_int4_workspace_bytes(int32_t batch, int32_t q_len, int32_t heads, 
  * and attends to the positions up to its own; a row that sees none gets out = 0, lse = -inf.  Tokens of
  * a page outside the pool take no weight (ROLAQ_DEV_BAD_PAGE); a length above 64 max_pages is cut
  * (ROLAQ_DEV_BAD_REQ); what a page holds past a request's length is never used.
+ * A query's latent part is taken in two E4M3 terms under a power of two of the row: exactly where an element
+ * is within 2^10 of the row's largest, else to 2^-18 of that; all sums are FP32; a weight times its group's scale is held
+ * in FP16 (11 bits) for the value product.  A query row that holds a NaN or an infinity gets NaN, and only that row.
  *   q    bf16 [B, q_len, H, D + Dr], strides in elements (multiples of 8), 16-byte aligned
  *   out  bf16 [B, q_len, H, D], likewise;  lse f32 [B, q_len, H] contiguous (natural log; NULL: not wanted)
  */
@@ -406,7 +409,7 @@ int rolaq_int4_decode(const uint16_t* q, int64_t q_stride_b, int64_t q_stride_t,
  * index).  score = max over the heads of the sum over both parts of
  *   2^(e_q + e_page) (sum q8 center + sum |q8| radius),  q8 = round_half_even(q / 2^e_q) in -127..127,
  * an upper bound, up to q's rounding, of any token's q k^T; the sums are whole numbers, so the choice
- * does not depend on their order.  sel_table[b] holds the chosen pages in the request's order, then
+ * does not depend on their order; an element of q that is no finite number counts as 0.  sel_table[b] holds the chosen pages in the request's order, then
  * -1; sel_lens[b] = (chosen - 1) * 64 + tokens of the last page (0 for an empty request).
  *   q  bf16 [B, H, D + Dr], strides in elements;  sel_table int32 [B, budget] (row stride sel_stride)
  *   budget >= keep_first + keep_last, keep_last >= 1

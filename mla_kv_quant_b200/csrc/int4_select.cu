@@ -9,6 +9,8 @@
 // times |q8| into the same sums - with the 16 heads of a tile as rows; q8 lies in shared memory in operand order.
 // A request's pages are shared by a few CTAs; the one that scores last keeps the pages: the budget-th largest
 // score by an 8-bit radix search, then, in the pages' order, all above it and the first of its equals.
+// Measured: 64 requests of 256 pages, 16 heads (19 MB of boxes) 18 us, of which memory needs 3: a CTA's one pass over its
+// pages and the search are chains of dependent steps.
 #include <algorithm>
 #include <atomic>
 
@@ -298,7 +300,8 @@ int launch(const SelectArgs& a, cudaStream_t s) {
       return ROLAQ_ECUDA;
     prepared |= uint64_t(1) << (device & 63);
   }
-  // CTAs of one pass over their pages each, as long as two a multiprocessor are enough for it
+  // CTAs of one pass over their pages each, as long as two a multiprocessor are enough for it: few requests are spread
+  // over the machine (one of 2048 pages), many get one CTA each, which then needs no join of the scores
   constexpr int pass = kTile * kWarps;
   const int passes = (a.max_pages + pass - 1) / pass;
   const int per_request = std::max(1, 2 * sm_count() / a.batch);
