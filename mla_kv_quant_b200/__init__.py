@@ -9,6 +9,7 @@ Host modules mirror the reference interfaces; the arithmetic runs in
 * ``mla_latent_int2``   -- ``scatter_pack_rows`` (general writer)
 * ``mla_packed_decode`` -- ``packed_mla_decode_gf_fwd``, ``prepare_gf_splits`` (reader)
 * ``pool``              -- ``PackedLatentPool`` (cache buffers and accounting)
+* ``int4``              -- ``Int4LatentPool``: the 4-bit cache, its attention, and attention over chosen pages
 * ``seqsplit``          -- sequence-split decode across ranks (NCCL all-gather + LSE merge)
 """
 
