@@ -604,8 +604,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         top = warp_max_f32(odd != 0.f ? INFINITY : top);
         // 2^k with top 2^k in [2^7, 2^8)
-        const float up = top > 0.f ? pow2(min(max(7 - (static_cast<int>(__float_as_uint(top) >> 23) - 127), -100), 100)) : 1.f;
-        if (lane == 0) sh.row_scale[r] = top == INFINITY ? __int_as_float(0x7FC00000) : qk_scale * (512.f / up);
+        const float up = top > 0.f ? pow2(min(max(7 - (static_cast<int>(__float_as_uint(top) >> 23) - 127), -120), 100)) : 1.f;
+        if (lane == 0) sh.row_scale[r] = top == INFINITY ? __int_as_float(0x7FC00000) : (qk_scale * 512.f) / up;
 #pragma unroll
         for (int i = 0; i < D / 256; ++i) {
           const uint32_t v[4] = {w[i].x, w[i].y, w[i].z, w[i].w};
@@ -783,7 +783,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             const float s = fmaxf(fmaxf(sh.red_s[0][k], sh.red_s[1][k]), fmaxf(sh.red_s[2][k], sh.red_s[3][k]));
             keep_unit[k] = 1.f;
             if (s * unit[k] > 2.f) {  // bring the largest scale into [1, 2)
-              const float u = pow2(min(max(127 - static_cast<int>(__float_as_uint(s) >> 23), -100), 100));
+              const float u = pow2(min(max(127 - static_cast<int>(__float_as_uint(s) >> 23), -126), 100));
               keep_unit[k] = u / unit[k];
               unit[k] = u;
             }
