@@ -4,6 +4,7 @@
 // Codec (the uniform min/max codec of mla_quant/oscar.py:91-101 with 16 levels): per 128 elements
 // scale = (hi - lo) / 15, code = round((x - lo) / scale), zero = -lo / scale, value = (code - zero) scale.
 #include <algorithm>
+#include <type_traits>
 
 #include "int4.cuh"
 
@@ -172,24 +173,41 @@ __global__ void __launch_bounds__(256) read_kernel(rolaq_int4_cache cache, const
     }
 }
 
-// The minimum and maximum of a word's 8 codes' values over the tokens of a CTA's share, in 32-bit steps that are
-// value()'s: codes become floats by one OR under 2^23 (their place in the word a power of 16) and one exact FMA.
-__device__ __forceinline__ void widen(uint32_t w, float scale, float zero, float (&lo)[8], float (&hi)[8]) {
-  const uint32_t high = w >> 12;  // codes 5, 6 and 7 at places 2, 3 and 4
+// The least and greatest of three; a NaN is passed over.
+__device__ __forceinline__ float min3(float a, float b, float c) {
+  float d;
+  asm("min.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float d;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
+
+// Two tokens' words of 8 codes each widen the minima and maxima of the columns, in 32-bit steps that are value()'s: codes
+// become floats by one OR under 2^23 (their place in the word a power of 16) and one exact FMA.
+__device__ __forceinline__ void widen(const uint32_t (&w)[2], const float2 (&p)[2], float (&lo)[8], float (&hi)[8]) {
+  const uint32_t high[2] = {w[0] >> 12, w[1] >> 12};  // codes 5, 6 and 7 at places 2, 3 and 4
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
     const int place = i < 5 ? i : i - 3;
     const float at = 1.f / static_cast<float>(1 << (4 * place));
-    const float code = fmaf(__uint_as_float(((i < 5 ? w : high) & (15u << (4 * place))) | 0x4B000000u), at, -8388608.f * at);
-    const float v = __fmul_rn(__fsub_rn(code, zero), scale);
-    lo[i] = fminf(lo[i], v);
-    hi[i] = fmaxf(hi[i], v);
+    float v[2];
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      const float code = fmaf(__uint_as_float(((i < 5 ? w[k] : high[k]) & (15u << (4 * place))) | 0x4B000000u), at, -8388608.f * at);
+      v[k] = __fmul_rn(__fsub_rn(code, p[k].y), p[k].x);
+    }
+    lo[i] = min3(lo[i], v[0], v[1]);
+    hi[i] = max3(hi[i], v[0], v[1]);
   }
 }
 
 // One CTA per page: a thread takes a word (8 columns) of every (512 * 8 / W)-th token, the CTA joins them through
-// shared memory.  Seven operations an element bound it, not memory: 2048 whole pages of 512 + 64 (57 MB) 38 us, 1.5 TB/s;
-// 64 KB of a page in flight on an SM.
+// shared memory.  The operations on an element bound it (the logic pipe, which the minima and maxima need, is 56% full),
+// not memory: 2048 whole pages of 512 + 64 (57 MB) 33 us, 1.7 TB/s; 38 with addresses for pages that may end early, and
+// with a token a step.
 template <int D, int DR>
 __global__ void __launch_bounds__(256, 4) boxes_kernel(rolaq_int4_cache cache, const int32_t* __restrict__ pages,
                                                     const int32_t* __restrict__ counts, int32_t* err) {
@@ -212,22 +230,23 @@ __global__ void __launch_bounds__(256, 4) boxes_kernel(rolaq_int4_cache cache, c
 #pragma unroll
     for (int i = 0; i < 8; ++i) lo[i] = INFINITY, hi[i] = -INFINITY;
     constexpr int AT_ONCE = EACH < 8 ? EACH : 8;
+    // Tokens past the count are the share's first one again (or, where that is past it too, nothing).
+    auto walk = [&](auto whole) {
 #pragma unroll 1
-    for (int k0 = 0; k0 < EACH; k0 += AT_ONCE) {
-      uint32_t w[AT_ONCE];
-      float2 p[AT_ONCE];
+      for (int k0 = 0; k0 < EACH; k0 += AT_ONCE) {
+        uint32_t w[AT_ONCE / 2][2];
+        float2 p[AT_ONCE / 2][2];
 #pragma unroll
-      for (int k = 0; k < AT_ONCE; ++k) {  // past the count: the share's first token again (share < count), or nothing
-        const int at = share + (k0 + k) * SHARES < count ? k0 + k : 0;
-        w[k] = codes[at * SHARES * WORDS], p[k] = params[at * SHARES * NG];
+        for (int k = 0; k < AT_ONCE; ++k) {
+          const int at = whole || share + (k0 + k) * SHARES < count ? k0 + k : 0;
+          w[k / 2][k % 2] = codes[at * SHARES * WORDS], p[k / 2][k % 2] = params[at * SHARES * NG];
+        }
+#pragma unroll
+        for (int k = 0; k < AT_ONCE / 2; ++k) widen(w[k], p[k], lo, hi);
       }
-#pragma unroll
-      for (int k = 0; k < AT_ONCE; ++k) widen(w[k], p[k].x, p[k].y, lo, hi);
-      if (share >= count) {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) lo[i] = INFINITY, hi[i] = -INFINITY;
-      }
-    }
+    };
+    if (count == kPage) walk(std::true_type());
+    else if (share < count) walk(std::false_type());
     store8(&box[0][share][8 * word], lo);
     store8(&box[1][share][8 * word], hi);
   }
