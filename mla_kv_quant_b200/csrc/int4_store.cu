@@ -12,88 +12,95 @@ namespace rolaq {
 namespace i4 {
 namespace {
 
-// 32 consecutive elements of a row as FP32.
+// Every fourth 8 of 128 elements of a row as FP32.
 __device__ __forceinline__ void load32(const float* p, float (&x)[32]) {
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
-    const float4 v = reinterpret_cast<const float4*>(p)[i];
+    const float4 v = reinterpret_cast<const float4*>(p)[8 * (i / 2) + i % 2];
     x[4 * i] = v.x, x[4 * i + 1] = v.y, x[4 * i + 2] = v.z, x[4 * i + 3] = v.w;
   }
 }
 __device__ __forceinline__ void load32(const uint16_t* p, float (&x)[32]) {
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    const uint4 v = reinterpret_cast<const uint4*>(p)[i];
+    const uint4 v = reinterpret_cast<const uint4*>(p)[4 * i];
     const uint32_t w[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
     for (int k = 0; k < 4; ++k) x[8 * i + 2 * k] = bf16_lo(w[k]), x[8 * i + 2 * k + 1] = bf16_hi(w[k]);
   }
 }
 
-// Four threads per unit: a unit is one 128-element group of a row (32 elements a thread, min and max over the four by
-// shuffles) or the row's k_pe.  Bound by memory as long as 32 divisions of a thread are not: the quotient's rounding is
-// decided by a product with the reciprocal, which is within 2^-18 of the quotient, unless that lies within 1e-5 of a
-// half; then the thread divides.
-// Measured: 131072 rows of 512 + 64 in BF16 (206 MB) 76 us, 2.7 TB/s: the instructions of the rounding bound it.
-// Storing them and reading them back took 148 us with 16 elements a thread here and one row a thread there, 121 now.
+// The least and greatest of three, NaN where one is.
+__device__ __forceinline__ float min3_nan(float a, float b, float c) {
+  float d;
+  asm("min.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
+__device__ __forceinline__ float max3_nan(float a, float b, float c) {
+  float d;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
+
+// Four threads per 128-element group of a row, min and max over the four by shuffles; the last blocks copy k_pe.  A thread
+// loads words of 8 elements 4 apart (whole sectors a load) and changes its words of codes with the other three, so that
+// it stores 16 bytes in a row.
+// Divisions: with y = 1 / b rounded and q within one unit of a / b's last place, the residual a - b q is exact and
+// q + (a - b q) y rounds to the rounded quotient (Markstein, IBM J. Res. Dev. 34, 1990); the first such step brings the
+// product a y, which is within 1.5 units, within one, the second to the quotient.  All is far from the ends of the range:
+// 6e-10 < scale < 3e37.  That is without branches, where a check of the product for nearness to a half and a division then
+// met the many exact halves of BF16 rows (62 us against 55).
+// Measured: 131072 rows of 512 + 64 in BF16 (206 MB) 55 us, 3.7 TB/s, bound by instructions (61% of the
+// issue slots) and their latency at 32 warps; 76 with a thread's elements side by side and k_pe among the groups.
 template <typename T, int NG>
-__global__ void __launch_bounds__(256) write_kernel(const T* __restrict__ c, int64_t ld_c,
-                                                    const uint16_t* __restrict__ k_pe, int64_t ld_pe, const void* slots,
-                                                    int slots64, int64_t n, rolaq_int4_cache cache, int32_t* err) {
-  constexpr float kNear = 0.49999f;
-  const uint32_t unit = (blockIdx.x * 256u + threadIdx.x) / 4;
-  const int part = threadIdx.x & 3;
-  const int64_t row = unit / (NG + 1);
-  const int g = unit % (NG + 1);
-  if (row >= n) return;  // whole groups of four threads leave together
-  const int64_t slot = load_index(slots, slots64, row);
-  const bool ok = slot >= 0 && slot < cache.num_slots;
-  if (g == NG) {
-    if (!ok) {
-      if (part == 0) report(err, ROLAQ_DEV_BAD_SLOT);
-      return;
-    }
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const int col = 8 * (part + 4 * i);
-      if (col < cache.rope_dim)
-        *reinterpret_cast<uint4*>(cache.rope + slot * cache.rope_dim + col) =
-            *reinterpret_cast<const uint4*>(k_pe + row * ld_pe + col);
-    }
+__global__ void __launch_bounds__(256, 4) write_kernel(const T* __restrict__ c, int64_t ld_c,
+                                                       const uint16_t* __restrict__ k_pe, int64_t ld_pe, const void* slots,
+                                                       int slots64, int64_t n, unsigned group_blocks, rolaq_int4_cache cache,
+                                                       int32_t* err) {
+  if (blockIdx.x >= group_blocks) {
+    const uint32_t unit = (blockIdx.x - group_blocks) * 256u + threadIdx.x, chunks = cache.rope_dim / 8;
+    const int64_t row = unit / chunks;
+    const int col = 8 * (unit % chunks);
+    if (row >= n) return;
+    const int64_t slot = load_index(slots, slots64, row);
+    if (slot >= 0 && slot < cache.num_slots)
+      *reinterpret_cast<uint4*>(cache.rope + slot * cache.rope_dim + col) = *reinterpret_cast<const uint4*>(k_pe + row * ld_pe + col);
+    else if (col == 0)
+      report(err, ROLAQ_DEV_BAD_SLOT);
     return;
   }
+  const uint32_t unit = (blockIdx.x * 256u + threadIdx.x) / 4;
+  const int part = threadIdx.x & 3;
+  const int64_t row = unit / NG;
+  const int g = unit % NG;
+  if (row >= n) return;  // whole groups of four threads leave together
+  const int64_t slot = load_index(slots, slots64, row);
   float x[32];  // on its way together with the slot
-  load32(c + row * ld_c + g * kGroup + part * 32, x);
-  float lo = x[0], hi = x[0], bad = 0.f;
+  load32(c + row * ld_c + g * kGroup + part * 8, x);
+  float lo = x[0], hi = x[0];
 #pragma unroll
-  for (int i = 0; i < 32; ++i) {
-    lo = fminf(lo, x[i]);
-    hi = fmaxf(hi, x[i]);
-    bad = fmaf(x[i], 0.f, bad);  // NaN as soon as one element is no finite number
-  }
+  for (int i = 0; i < 32; i += 2) lo = min3_nan(lo, x[i], x[i + 1]), hi = max3_nan(hi, x[i], x[i + 1]);
   const uint32_t lanes = 0xFu << (threadIdx.x & 28);
 #pragma unroll
   for (int o = 1; o < 4; o *= 2) {
-    lo = fminf(lo, __shfl_xor_sync(lanes, lo, o));
-    hi = fmaxf(hi, __shfl_xor_sync(lanes, hi, o));
-    bad += __shfl_xor_sync(lanes, bad, o);
+    const float l = __shfl_xor_sync(lanes, lo, o), h = __shfl_xor_sync(lanes, hi, o);
+    lo = min3_nan(lo, lo, l);
+    hi = max3_nan(hi, hi, h);
   }
   const float range = __fsub_rn(hi, lo);
   float scale = fabsf(range) <= 1e-8f ? 1.f : __fdiv_rn(range, kTop);
-  const float inv = __fdividef(1.f, scale);
+  const float inv = __frcp_rn(scale);
   uint32_t w[4];
 #pragma unroll
   for (int k = 0; k < 4; ++k) {  // a word of 8 codes
-    float code[8], off = 0.f;
+    float code[8];
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      const float quotient = __fmul_rn(__fsub_rn(x[8 * k + i], lo), inv);
-      code[i] = __fsub_rn(__fadd_rn(quotient, 12582912.f), 12582912.f);  // the nearest whole number, halves to even
-      off = fmaxf(off, fabsf(__fsub_rn(quotient, code[i])));
-    }
-    if (off > kNear) {
-#pragma unroll
-      for (int i = 0; i < 8; ++i) code[i] = rintf(__fdiv_rn(__fsub_rn(x[8 * k + i], lo), scale));
+      const float d = __fsub_rn(x[8 * k + i], lo);
+      float q = __fmul_rn(d, inv);
+      q = __fmaf_rn(__fmaf_rn(-q, scale, d), inv, q);
+      q = __fmaf_rn(__fmaf_rn(-q, scale, d), inv, q);
+      code[i] = __fsub_rn(__fadd_rn(q, 12582912.f), 12582912.f);  // the nearest whole number, halves to even
     }
     float half[2];  // four codes as one whole number below 2^16 (0 <= code <= 15: lo and hi are the group's own)
 #pragma unroll
@@ -102,8 +109,20 @@ __global__ void __launch_bounds__(256) write_kernel(const T* __restrict__ c, int
     // under 2^23 a whole number is the float's low bits
     w[k] = (__float_as_uint(half[0] + 8388608.f) & 0xFFFFu) | __float_as_uint(half[1] + 8388608.f) << 16;
   }
-  if (bad != 0.f) scale = __int_as_float(0x7FC00000);
-  if (!ok) return;
+  // words part + 4 i to words 4 part + i: a transpose among the four
+#pragma unroll
+  for (int o = 1; o < 4; o *= 2) {
+    const bool up = part & o;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if (i & o) continue;
+      const uint32_t got = __shfl_xor_sync(lanes, up ? w[i] : w[i | o], o);
+      if (up) w[i] = got;
+      else w[i | o] = got;
+    }
+  }
+  if (!(range < INFINITY)) scale = __int_as_float(0x7FC00000);  // as soon as an element is no finite number
+  if (slot < 0 || slot >= cache.num_slots) return;  // reported with its k_pe
   *reinterpret_cast<uint4*>(cache.codes + slot * (NG * 64) + g * 64 + part * 16) = make_uint4(w[0], w[1], w[2], w[3]);
   if (part == 0) reinterpret_cast<float2*>(cache.params)[slot * NG + g] = make_float2(scale, __fdiv_rn(-lo, scale));
 }
@@ -117,7 +136,7 @@ __device__ __forceinline__ void store8(uint16_t* p, const float (&v)[8]) {
       make_uint4(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]), pack_bf16x2(v[4], v[5]), pack_bf16x2(v[6], v[7]));
 }
 
-// Eight threads per unit, a unit as in write_kernel, and two rows a thread, `apart` rows from each other, so that
+// Eight threads per unit, a unit being a group of a row or its k_pe, and two rows a thread, `apart` rows from each other, so that
 // twice as much is under way: a thread reads the words of 8 elements at 8 part and at 64 + 8 part of its group, so
 // that a warp's stores are whole lines.  Bound by memory: the rows above back in BF16 43 us, 4.8 TB/s.
 template <typename T, int NG>
@@ -359,10 +378,10 @@ int launch_write(const void* c, bool f32, int64_t ld_c, const uint16_t* k_pe, in
   const int64_t most = (int64_t(1) << 31) / (4 * (ng + 1)) / 256 * 256;
   for (int64_t at = 0; at < n; at += most) {
     const int64_t rows = std::min(n - at, most);
-    const unsigned grid = blocks_for(rows * (ng + 1) * 4, 256);
+    const unsigned groups = blocks_for(rows * ng * 4, 256), grid = groups + blocks_for(rows * (cache.rope_dim / 8), 256);
     const void* sl = static_cast<const char*>(slots) + at * (slots64 ? 8 : 4);
     auto go = [&](auto kernel, auto* src) {
-      kernel<<<grid, 256, 0, s>>>(src + at * ld_c, ld_c, k_pe + at * ld_pe, ld_pe, sl, slots64, rows, cache, err);
+      kernel<<<grid, 256, 0, s>>>(src + at * ld_c, ld_c, k_pe + at * ld_pe, ld_pe, sl, slots64, rows, groups, cache, err);
     };
     if (f32 && ng == 4) go(write_kernel<float, 4>, static_cast<const float*>(c));
     else if (f32) go(write_kernel<float, 2>, static_cast<const float*>(c));
