@@ -115,7 +115,7 @@ __device__ void keep_pages(const float* __restrict__ scores, const int32_t* __re
 // chunk_pages pages of a request per CTA (a multiple of kTile * kWarps).
 template <int D, int DR>
 __global__ void __launch_bounds__(kThreads) select_kernel(const SelectArgs a, const int chunk_pages) {
-  constexpr int W = D + DR, BLOCKS = D / 64, STEPS = (D + DR) / 32;  // 64-column blocks of the latent; 32-column steps
+  constexpr int W = D + DR, STEPS = (D + DR) / 32;  // 32-column steps
   extern __shared__ __align__(16) uint8_t dynamic[];
   uint4* q8 = reinterpret_cast<uint4*>(dynamic);  // [tile][step][q8, |q8|][lane]
   __shared__ float tops[2][kWarps];
