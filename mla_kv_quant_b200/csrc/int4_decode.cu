@@ -713,9 +713,11 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (__any_sync(0xFFFFFFFFu, pos >= lim_min || bad || !here)) {
           // the request's or the run's end, or a page that is not there
           const bool none = bad || !here || pos >= len;
-          if (none)
+          // A group that is no number: rows that see the token have a weight of NaN by their score, and for those that do
+          // not a weight of 0 has to stay 0 in its products.
 #pragma unroll
-            for (int k = 0; k < NG; ++k) s_tok[k] = z_tok[k] = 0.f;
+          for (int k = 0; k < NG; ++k)
+            if (none || !(fabsf(s_tok[k]) < INFINITY && fabsf(s_tok[k] * z_tok[k]) < INFINITY)) s_tok[k] = z_tok[k] = 0.f;
 #pragma unroll
           for (int n = 0; n < HT; ++n)
 #pragma unroll
