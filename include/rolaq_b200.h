@@ -392,7 +392,8 @@ int64_t rolaq_int4_workspace_bytes(int32_t batch, int32_t q_len, int32_t heads, 
  * (ROLAQ_DEV_BAD_REQ); what a page holds past a request's length is never used.
  * A query's latent part is taken in two E4M3 terms under a power of two of the row: exactly where an element
  * is within 2^10 of the row's largest, else to 2^-18 of that; all sums are FP32; a weight times its group's scale is held
- * in FP16 (11 bits) for the value product.  A query row that holds a NaN or an infinity gets NaN, and only that row.
+ * in FP16 for the value product, to 11 bits or to 2^-26 of the largest such product that the row has met in the group,
+ * whatever other tokens and rows hold.  A query row that holds a NaN or an infinity gets NaN, and only that row.
  *   q    bf16 [B, q_len, H, D + Dr], strides in elements (multiples of 8), 16-byte aligned
  *   out  bf16 [B, q_len, H, D], likewise;  lse f32 [B, q_len, H] contiguous (natural log; NULL: not wanted)
  */

@@ -9,7 +9,14 @@
 //     one FP32 sum a group; the rotary part BF16 by BF16.  Asynchronous: no warp's issue slots go into it.
 //   - sums: the FP16 patterns 0..255 are that many 2^-24 exactly.  mma.sync m16n8k16 with the codes as rows (c of an
 //     even element, and c + 16 c' of it and the next: c' comes out at the end) and P s in FP16 as columns.
-// All sums are FP32.
+// All sums are FP32, and so is the zeros' share.
+//
+// FP16 holds P s to 11 bits from 2^-14 to 2^16 only, so it is held relative to the largest P s that a row has met in a group:
+// a group's unit follows the largest scale, which is enough while each row gives weight to tokens of about that scale.
+// Where the references move, and the scales do not already say that each row has met a P s unit of 2 in each group, the
+// rows' largest are taken too, and a row that has not met that much in a group (its tokens' scales are far below
+// others') gets a power of two of its own there; while one is in use, each tile goes that way.  Equal elements are stored with scale 1 and codes 0: they add nothing but
+// their zero's share, and their scale is not taken for a size.
 //
 // A CTA holds NH tiles of 8 query rows (query tokens x heads; up to two for D = 512, five for D = 256) and walks the
 // pages of one or more requests, two (a tile of 128 tokens) at a time:
@@ -31,6 +38,7 @@
 // operands are the same in all lanes).
 #include <algorithm>
 #include <atomic>
+#include <type_traits>
 
 #include "int4.cuh"
 #include "kernels.cuh"
@@ -47,7 +55,10 @@ constexpr int kAhead = 4;         // pages ahead of their loads that they are ca
 // The least run of pages worth a CTA of its own (a tile), unless the requests are shorter: 31 of 20 tokens, 4 query tokens of
 // 40 heads of 256: 22 us, 33 with two requests a CTA.
 constexpr int kMinPages = 2;
-constexpr float kSlack = 1024.f, kScaleSlack = 32.f;  // how far weights and scales may pass their references (P s <= 2^15)
+// Scales are brought into [2^2, 2^3); weights and scales may pass their references until P s is 2^15.
+constexpr float kSlack = 1024.f, kScaleTop = 8.f, kScaleSlack = 32.f;
+constexpr float kLeast = 2.f;       // the least of a row's largest P s unit that needs no factor of the row's own
+constexpr float kZeroShare = 9.094947017729282e-13f;  // 2^-40: a scale below this share of its value's size counts as that much
 constexpr float kNoMax = -1e30f, kNoUnit = 1.329227995784916e36f;  // references not yet set: the first token passes them
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
@@ -77,10 +88,12 @@ struct Cfg {
 
 template <int NG, int NH>
 struct alignas(16) Shared {  // rows are read two at a time
-  float red_m[4][8 * NH], red_s[4][NG];                   // by quarters of the tile's tokens
-  float keep[3][8 * NH], keep_unit[3][NG];                // factors for the sums before tile i (at i % 3), where moved[i % 3]
+  float red_m[4][8 * NH], red_s[4][NG], red_w[4][NG * 8 * NH];  // by quarters of the tile's tokens
+  float keep[3][NG][8 * NH];                              // factors for the sums before tile i (at i % 3), where moved[i % 3]
+  float keep_row[8 * NH], keep_unit[NG];                  // the parts of the last ones
   float max[8 * NH], q_sum[NG][8 * NH], row_scale[8 * NH];
-  float l[4][8 * NH], z[4][NG][8 * NH], max_out[8 * NH], unit_out[NG];  // of a finished request
+  float met[NG * 8 * NH], factor[NG][8 * NH];             // a row's largest P s unit in a group, as of the last move; its own factor
+  float l[4][8 * NH], z[4][NG][8 * NH], max_out[8 * NH], unit_out[NG], factor_out[NG * 8 * NH];  // of a finished request (1 / factor)
   int moved[3];
 };
 
@@ -440,14 +453,13 @@ __global__ void __launch_bounds__(kThreads, 1)
         wait_for(&weighed[turn], lap);
         __syncwarp();
         if (sh.moved[turn]) {
-          const float ku = sh.keep_unit[turn][own];
 #pragma unroll
           for (int n = 0; n < NH; ++n) {
-            const float2 k = *reinterpret_cast<const float2*>(&sh.keep[turn][8 * n + 2 * j]);
+            const float2 k = *reinterpret_cast<const float2*>(&sh.keep[turn][own][8 * n + 2 * j]);
 #pragma unroll
             for (int c = 0; c < 2 * CH; ++c) {
-              acc[c][n][0] *= k.x * ku, acc[c][n][2] *= k.x * ku;
-              acc[c][n][1] *= k.y * ku, acc[c][n][3] *= k.y * ku;
+              acc[c][n][0] *= k.x, acc[c][n][2] *= k.x;
+              acc[c][n][1] *= k.y, acc[c][n][3] *= k.y;
             }
           }
         }
@@ -497,7 +509,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           float l = 0.f, z = 0.f;
 #pragma unroll
           for (int k = 0; k < 4; ++k) l += sh.l[k][at], z += sh.z[k][own][at];
-          const float inv = l == 0.f ? 0.f : inv_u / l;
+          const float inv = l == 0.f ? 0.f : inv_u / l, inv_f = sh.factor_out[own * ROWS + at];
           const float lse = l == 0.f ? -INFINITY : (sh.max_out[at] + log2f(l)) * kLn2;
           const bool live = row < rows;
           const int t = live ? row / a.heads : 0, h = live ? row % a.heads : 0;
@@ -510,8 +522,8 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
               const float even = acc[2 * c + i][n][x], sum = acc[2 * c + i][n][x + 2];
-              v[2 * i] = fmaf(even, 16777216.f, -z) * inv;
-              v[2 * i + 1] = fmaf(sum - even, 1048576.f, -z) * inv;
+              v[2 * i] = fmaf(even, 16777216.f * inv_f, -z) * inv;
+              v[2 * i + 1] = fmaf(sum - even, 1048576.f * inv_f, -z) * inv;
             }
             if (!whole) *reinterpret_cast<float4*>(out_part + col) = make_float4(v[0], v[1], v[2], v[3]);
             else if (live) *reinterpret_cast<uint2*>(out + col) = make_uint2(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]));
@@ -637,6 +649,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
       }
       if (tid < ROWS) sh.max[tid] = kNoMax;
+      if (tid < NG * ROWS) sh.met[tid] = 0.f, sh.factor[0][tid] = 1.f;
       fence_proxy_async();
       token_sync();
       if (tid == 0) mbar_arrive(&q_ready);
@@ -653,6 +666,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
 #pragma unroll
       for (int k = 0; k < NG; ++k) unit[k] = kNoUnit;
+      bool factors = false;  // a row has a factor of its own, or has met nothing yet
       const int tiles = (count + 1) / 2;
       bring_codes(tile, own_page(done, count));
       for (int i = 0; i < tiles; ++i, ++tile) {
@@ -710,6 +724,9 @@ __global__ void __launch_bounds__(kThreads, 1)
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(&taken[tile & 1]);
+        // From here on z_tok is what the zero takes from each value: z s.
+#pragma unroll
+        for (int k = 0; k < NG; ++k) z_tok[k] *= s_tok[k];
         if (__any_sync(0xFFFFFFFFu, pos >= lim_min || bad || !here)) {
           // the request's or the run's end, or a page that is not there
           const bool none = bad || !here || pos >= len;
@@ -717,7 +734,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           // not a weight of 0 has to stay 0 in its products.
 #pragma unroll
           for (int k = 0; k < NG; ++k)
-            if (none || !(fabsf(s_tok[k]) < INFINITY && fabsf(s_tok[k] * z_tok[k]) < INFINITY)) s_tok[k] = z_tok[k] = 0.f;
+            if (none || !(fabsf(s_tok[k]) < INFINITY && fabsf(z_tok[k]) < INFINITY)) s_tok[k] = z_tok[k] = 0.f;
 #pragma unroll
           for (int n = 0; n < HT; ++n)
 #pragma unroll
@@ -730,10 +747,26 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (here && page >= C::WEIGHTS) wait_for(&page_free[(page - C::WEIGHTS) % PAGES], (page - C::WEIGHTS) / PAGES);
         __syncwarp();
 
+        // Equal elements, which the store gives scale 1 and codes 0: no scale.  Looked for where a scale of 1 matters.
+        auto drop_equal = [&]() {
+#pragma unroll
+          for (int k = 0; k < NG; ++k) {
+            if (s_tok[k] != 1.f) continue;
+            const char* row = smem + at * C::CODES + (D == 512 ? k / 2 * 8192 : 0) + (token & 63) * 128;
+            uint32_t any = 0;
+#pragma unroll 1
+            for (int c = 0; c < 4; ++c) {
+              const uint4 v = *reinterpret_cast<const uint4*>(row + (((D == 512 ? k % 2 : k) * 4 + c) ^ (token & 7)) * 16);
+              any |= v.x | v.y | v.z | v.w;
+            }
+            if (any == 0) s_tok[k] = 0.f;
+          }
+        };
         // Weights against the present references, times each group's scale, to shared memory; true where a
         // weight or a scale has left its reference behind (their sums: moving early does no harm), or is NaN.
         float2 p_val[HT][4];
         auto weigh = [&]() {
+          char* weights_at = smem + C::OFF_P + (page % C::WEIGHTS) * C::PBUF + n0 * C::PTILE + (token & 63) * 16;
           float2 weights = both(0.f);
           float sizes = 0.f;
 #pragma unroll
@@ -747,11 +780,10 @@ __global__ void __launch_bounds__(kThreads, 1)
                 weights = add2(weights, p_val[n][x]);
               }
             }
-          char* dst = smem + C::OFF_P + (page % C::WEIGHTS) * C::PBUF + n0 * C::PTILE + (token & 63) * 16;
 #pragma unroll
           for (int k = 0; k < NG; ++k) {
             const float s = s_tok[k] * unit[k];
-            sizes += fabsf(s);
+            sizes = fmaxf(sizes, fmaf(fabsf(z_tok[k] * unit[k]), kZeroShare, fabsf(s)));
 #pragma unroll
             for (int n = 0; n < HT; ++n)
               if (n < my_tiles) {
@@ -761,13 +793,15 @@ __global__ void __launch_bounds__(kThreads, 1)
                   const float2 v = mul2(p_val[n][x], both(s));
                   h[x] = pack_half2(v.x, v.y);
                 }
-                if (here) *reinterpret_cast<uint4*>(dst + (k * NH + n) * C::PTILE) = make_uint4(h[0], h[1], h[2], h[3]);
+                if (here) *reinterpret_cast<uint4*>(weights_at + (k * NH + n) * C::PTILE) = make_uint4(h[0], h[1], h[2], h[3]);
               }
           }
           return !(weights.x + weights.y <= kSlack) || !(sizes <= kScaleSlack);
         };
-        const bool move = token_any(weigh());  // a request's first tile brings the first references
+        // A request's first tile brings the first references; while a row has a factor of its own, each tile moves them.
+        const bool move = token_any(weigh() || factors);
         if (move) {  // new references: the tile's maxima; the sums so far are brought to them
+          drop_equal();
 #pragma unroll
           for (int n = 0; n < HT; ++n)
             if (n < my_tiles) {
@@ -779,41 +813,107 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
 #pragma unroll
           for (int k = 0; k < NG; ++k) {
-            const float s = warp_max_f32(fabsf(s_tok[k]));
+            const float s = warp_max_f32(fmaf(fabsf(z_tok[k]), kZeroShare, fabsf(s_tok[k])));
             if (lane == 0 && half == 0) sh.red_s[quarter][k] = s;
           }
           token_sync();
           float keep_unit[NG];
+          bool doubt = factors;  // that each row has met P s unit of kLeast in each group
+          float seen = -INFINITY;
+#pragma unroll
+          for (int n = 0; n < HT; ++n)
+            if (n < my_tiles)
+#pragma unroll
+              for (int x = 0; x < 4; ++x) seen = fmaxf(seen, fmaxf(s_val[n][x].x, s_val[n][x].y));
 #pragma unroll
           for (int k = 0; k < NG; ++k) {
             const float s = fmaxf(fmaxf(sh.red_s[0][k], sh.red_s[1][k]), fmaxf(sh.red_s[2][k], sh.red_s[3][k]));
             keep_unit[k] = 1.f;
-            if (s * unit[k] > 2.f) {  // bring the largest scale into [1, 2)
-              const float u = pow2(min(max(127 - static_cast<int>(__float_as_uint(s) >> 23), -126), 100));
+            if (s * unit[k] > kScaleTop) {  // bring the largest scale into [kScaleTop / 2, kScaleTop)
+              const float u = pow2(min(max(129 - static_cast<int>(__float_as_uint(s) >> 23), -126), 100));
               keep_unit[k] = u / unit[k];
               unit[k] = u;
             }
-            if (tid == 0) sh.keep_unit[turn][k] = keep_unit[k];
+            if (tid == 0) sh.keep_unit[k] = keep_unit[k];
+            doubt |= seen > -INFINITY && !(s_tok[k] * unit[k] >= kLeast);
           }
           if (tid < ROWS) {
             const float old = sh.max[tid];
-            const float m = fmaxf(old, fmaxf(fmaxf(sh.red_m[0][tid], sh.red_m[1][tid]), fmaxf(sh.red_m[2][tid], sh.red_m[3][tid])));
-            sh.keep[turn][tid] = ex2_approx(old - m);
-            sh.max[tid] = m;
+            const float m = fmaxf(fmaxf(sh.red_m[0][tid], sh.red_m[1][tid]), fmaxf(sh.red_m[2][tid], sh.red_m[3][tid]));
+            sh.keep_row[tid] = ex2_approx(old - fmaxf(old, m));
+            sh.max[tid] = fmaxf(old, m);
+            if (m < old)  // else the row's largest weight, 1, is in this tile
+#pragma unroll
+              for (int k = 0; k < NG; ++k) doubt |= !(sh.met[k * ROWS + tid] * keep_unit[k] >= kLeast);
           }
-          token_sync();
+          __syncwarp();
+          doubt = token_any(doubt);
+          weigh();
 #pragma unroll
           for (int n = 0; n < HT; ++n)
             if (n < my_tiles) {
 #pragma unroll
               for (int x = 0; x < 4; ++x) {
-                const float2 keep = *reinterpret_cast<const float2*>(&sh.keep[turn][8 * (n0 + n) + 2 * x]);
+                const float2 keep = *reinterpret_cast<const float2*>(&sh.keep_row[8 * (n0 + n) + 2 * x]);
                 l_sum[n][x] = mul2(l_sum[n][x], keep);
 #pragma unroll
                 for (int k = 0; k < NG; ++k) zsum[k][n][x] = mul2(zsum[k][n][x], mul2(keep, both(keep_unit[k])));
               }
             }
-          weigh();
+          if (!doubt) {
+            if (tid < ROWS) {
+#pragma unroll
+              for (int k = 0; k < NG; ++k) {
+                sh.keep[turn][k][tid] = sh.keep_row[tid] * keep_unit[k];
+                sh.met[k * ROWS + tid] = kLeast;
+              }
+            }
+          } else {  // each row's largest P s unit of the tile, and factors for those that have met too little
+            float su[NG];
+#pragma unroll
+            for (int k = 0; k < NG; ++k) su[k] = s_tok[k] * unit[k];
+#pragma unroll 1
+            for (int k = 0; k < NG; ++k)
+#pragma unroll
+              for (int n = 0; n < HT; ++n)
+                if (n < my_tiles) {
+#pragma unroll
+                  for (int x = 0; x < 4; ++x) {
+                    const float2 w = mul2(p_val[n][x], both(fabsf(su[k])));
+                    const float w0 = warp_max_f32(w.x), w1 = warp_max_f32(w.y);
+                    if (lane == 0) *reinterpret_cast<float2*>(&sh.red_w[quarter][k * ROWS + 8 * (n0 + n) + 2 * x]) = make_float2(w0, w1);
+                  }
+                }
+            token_sync();
+            // Weights that came between two moves are not in `met`: a factor may be larger for that, which loses nothing.
+            bool odd = false;
+            if (tid < NG * ROWS) {
+              const float kept = sh.keep_row[tid % ROWS] * sh.keep_unit[tid / ROWS];
+              const float w = fmaxf(sh.met[tid] * kept, fmaxf(fmaxf(sh.red_w[0][tid], sh.red_w[1][tid]), fmaxf(sh.red_w[2][tid], sh.red_w[3][tid])));
+              odd = !(w >= kLeast);
+              const float f = odd && w > 0.f ? pow2(min(129 - static_cast<int>(__float_as_uint(w) >> 23), 100)) : 1.f;
+              sh.met[tid] = w;
+              sh.keep[turn][0][tid] = kept * (f / sh.factor[0][tid]);
+              sh.factor[0][tid] = f;
+            }
+            __syncwarp();
+            factors = token_any(odd);
+            char* weights_at = smem + C::OFF_P + (page % C::WEIGHTS) * C::PBUF + n0 * C::PTILE + (token & 63) * 16;
+            if (factors && here)
+#pragma unroll 1
+              for (int k = 0; k < NG; ++k)
+#pragma unroll
+                for (int n = 0; n < HT; ++n)
+                  if (n < my_tiles) {
+                    uint32_t h[4];
+#pragma unroll
+                    for (int x = 0; x < 4; ++x) {
+                      const float2 v = mul2(mul2(p_val[n][x], both(su[k])), *reinterpret_cast<const float2*>(&sh.factor[k][8 * (n0 + n) + 2 * x]));
+                      h[x] = pack_half2(v.x, v.y);
+                    }
+                    *reinterpret_cast<uint4*>(weights_at + (k * NH + n) * C::PTILE) = make_uint4(h[0], h[1], h[2], h[3]);
+                  }
+          }
           token_sync();
         }
         if (tid == 0) {
@@ -829,7 +929,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             for (int x = 0; x < 4; ++x) {
               l_sum[n][x] = add2(l_sum[n][x], p_val[n][x]);
 #pragma unroll
-              for (int k = 0; k < NG; ++k) zsum[k][n][x] = fma2(p_val[n][x], both(s_tok[k] * unit[k] * z_tok[k]), zsum[k][n][x]);
+              for (int k = 0; k < NG; ++k) zsum[k][n][x] = fma2(p_val[n][x], both(z_tok[k] * unit[k]), zsum[k][n][x]);
             }
           }
       }
@@ -850,6 +950,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
         }
       if (tid < ROWS) sh.max_out[tid] = sh.max[tid];
+      if (tid < NG * ROWS) sh.factor_out[tid] = 1.f / sh.factor[0][tid];
       if (tid == 0)
 #pragma unroll
         for (int k = 0; k < NG; ++k) sh.unit_out[k] = unit[k];
