@@ -59,7 +59,7 @@ constexpr int kMinPages = 2;
 constexpr float kSlack = 1024.f, kScaleTop = 8.f, kScaleSlack = 32.f;
 constexpr float kLeast = 2.f;       // the least of a row's largest P s unit that needs no factor of the row's own
 constexpr float kZeroShare = 9.094947017729282e-13f;  // 2^-40: a scale below this share of its value's size counts as that much
-constexpr float kNoMax = -1e30f, kNoUnit = 1.329227995784916e36f;  // references not yet set: the first token passes them
+constexpr float kNoMax = -3.402823466e38f, kNoUnit = 1.329227995784916e36f;  // references not yet set: the first token passes them
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
 template <int D, int DR, int NH>
