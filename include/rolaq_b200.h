@@ -409,6 +409,7 @@ int rolaq_int4_decode(const uint16_t* q, int64_t q_stride_b, int64_t q_stride_t,
  * of the others, those of the largest score, as many as the budget leaves (equal scores: the lower
  * index).  score = max over the heads of the sum over both parts of
  *   2^(e_q + e_page) (sum q8 center + sum |q8| radius),  q8 = round_half_even(q / 2^e_q) in -127..127,
+ * e_q the least exponent (>= -100) with max |q| <= 127 * 2^e_q over the part's columns and all heads,
  * an upper bound, up to q's rounding, of any token's q k^T; the sums are whole numbers, so the choice
  * does not depend on their order; an element of q that is no finite number counts as 0.  sel_table[b] holds the chosen pages in the request's order, then
  * -1; sel_lens[b] = (chosen - 1) * 64 + tokens of the last page (0 for an empty request).

@@ -13,6 +13,7 @@
 // pages and the search are chains of dependent steps.
 #include <algorithm>
 #include <atomic>
+#include <type_traits>
 
 #include "int4.cuh"
 #include "kernels.cuh"
@@ -169,29 +170,42 @@ __global__ void __launch_bounds__(kThreads) select_kernel(const SelectArgs a, co
 
   // ---- the query in 8 bits, in operand order ----
   const uint16_t* q = a.q + b * a.q_sb;
-  float top[2] = {0.f, 0.f};
-  for (int i = tid; i < a.heads * (W / 8); i += kThreads) {
-    const int col = 8 * (i % (W / 8));
-    const uint4 w = *reinterpret_cast<const uint4*>(q + (i / (W / 8)) * a.q_sh + col);
-    const uint32_t v[4] = {w.x, w.y, w.z, w.w};
-    float m = 0.f;
+  // The parts' largest elements; elements that are no finite numbers are looked for only where an infinity shows.
+  float m[2];
+  auto find_tops = [&](auto finite) {
+    float top[2] = {0.f, 0.f};
+    for (int i = tid; i < a.heads * (W / 8); i += kThreads) {
+      const int col = 8 * (i % (W / 8));
+      const uint4 w = *reinterpret_cast<const uint4*>(q + (i / (W / 8)) * a.q_sh + col);
+      const uint32_t v[4] = {w.x, w.y, w.z, w.w};
+      float most = 0.f;
 #pragma unroll
-    for (int k = 0; k < 4; ++k) m = fmaxf(m, fmaxf(fabsf(bf16_lo(v[k])), fabsf(bf16_hi(v[k]))));
-    top[col >= D] = fmaxf(top[col >= D], m);
-  }
+      for (int k = 0; k < 4; ++k)
 #pragma unroll
-  for (int k = 0; k < 2; ++k) {
-    top[k] = warp_max_f32(top[k]);
-    if (lane == 0) tops[k][warp] = top[k];
-  }
-  __syncthreads();
-  int e[2];
+        for (int h = 0; h < 2; ++h) {
+          const float size = fabsf(h ? bf16_hi(v[k]) : bf16_lo(v[k]));
+          if (!finite || size < INFINITY) most = fmaxf(most, size);  // fmaxf passes a NaN over
+        }
+      top[col >= D] = fmaxf(top[col >= D], most);
+    }
 #pragma unroll
-  for (int k = 0; k < 2; ++k) {
-    float m = 0.f;
-    for (int i = 0; i < kWarps; ++i) m = fmaxf(m, tops[k][i]);
-    e[k] = unit_exponent(m);
+    for (int k = 0; k < 2; ++k) {
+      top[k] = warp_max_f32(top[k]);
+      if (lane == 0) tops[k][warp] = top[k];
+    }
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      m[k] = 0.f;
+      for (int i = 0; i < kWarps; ++i) m[k] = fmaxf(m[k], tops[k][i]);
+    }
+  };
+  find_tops(std::false_type());
+  if (!(m[0] < INFINITY && m[1] < INFINITY)) {
+    __syncthreads();
+    find_tops(std::true_type());
   }
+  const int e[2] = {unit_exponent(m[0]), unit_exponent(m[1])};
   // Operand register r of lane (g, j), step s: row g + 8 (r & 1), columns that the boxes' 16-byte pieces put there:
   // block s / 2, bytes 16 j + 8 (s & 1) + 4 (r >> 1) of it; a half block at the end (DR = 32) has 8-byte pieces.
   const int tiles = (a.heads + 15) / 16;
@@ -208,7 +222,7 @@ __global__ void __launch_bounds__(kThreads) select_kernel(const SelectArgs a, co
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
         const float t = rintf(x[k] * inv);
-        const int c = t == t ? static_cast<int>(fminf(fmaxf(t, -127.f), 127.f)) : 0;
+        const int c = fabsf(x[k]) < INFINITY ? static_cast<int>(fminf(fmaxf(t, -127.f), 127.f)) : 0;
         v |= static_cast<uint32_t>(c & 255) << (8 * k);
         u |= static_cast<uint32_t>(abs(c)) << (8 * k);
       }
