@@ -2,7 +2,9 @@
 //
 // score(page) = max over the heads of sum over both parts of 2^(e_q + e_page) (sum q8 center + sum |q8| radius).
 // The sums are whole numbers below 2^24 (127 * 127 * 512 for the centers, 127 * 128 * 512 for the radii),
-// so their order does not matter; each part is one conversion and one exact product, the two parts one addition.
+// so their order does not matter; each part is one conversion and one exact product, the two parts one addition.  Only
+// the order of a request's scores counts, so they are taken over 2^20 times the query's larger unit: with units of 2^-100
+// to 2^122 in the boxes none then overflows, and infinity is left to the pages that are kept whatever they score.
 //
 // The boxes are read once (bandwidth is the bound): a warp takes 8 pages at a time, a lane 16 bytes of a page
 // per 64 columns, which are the operands of two m16n8k32 integer products as they are - centers times q8 and radii
@@ -30,6 +32,12 @@ constexpr int kCached = 4096;   // scores that the radix search holds in shared 
 __device__ __forceinline__ uint32_t rank_key(float s) {
   const uint32_t u = __float_as_uint(s);
   return u & 0x80000000u ? ~u : u | 0x80000000u;
+}
+
+// 2^e for e <= 127, rounded to a subnormal or 0 below 2^-126.
+__device__ __forceinline__ float any_pow2(int e) {
+  const float x = pow2(max(e, -126));
+  return e >= -126 ? x : x * pow2(max(e + 126, -126));
 }
 
 __device__ __forceinline__ void mma_s8s8(int (&d)[4], const uint4& a, uint32_t b0, uint32_t b1) {
@@ -206,6 +214,8 @@ __global__ void __launch_bounds__(kThreads) select_kernel(const SelectArgs a, co
     find_tops(std::true_type());
   }
   const int e[2] = {unit_exponent(m[0]), unit_exponent(m[1])};
+  const int e_top = m[0] > 0.f ? (m[1] > 0.f ? max(e[0], e[1]) : e[0]) : e[1];  // of the parts that hold anything
+  const int rel[2] = {m[0] > 0.f ? e[0] - e_top - 20 : -20, m[1] > 0.f ? e[1] - e_top - 20 : -20};
   // Operand register r of lane (g, j), step s: row g + 8 (r & 1), columns that the boxes' 16-byte pieces put there:
   // block s / 2, bytes 16 j + 8 (s & 1) + 4 (r >> 1) of it; a half block at the end (DR = 32) has 8-byte pieces.
   const int tiles = (a.heads + 15) / 16;
@@ -243,8 +253,8 @@ __global__ void __launch_bounds__(kThreads) select_kernel(const SelectArgs a, co
 #pragma unroll
     for (int x = 0; x < 2; ++x) {
       const int from = (2 * j + x) * 4;
-      unit[x][0] = pow2(e[0]) * pow2(__shfl_sync(0xFFFFFFFFu, e_page.x, from));
-      unit[x][1] = pow2(e[1]) * pow2(__shfl_sync(0xFFFFFFFFu, e_page.y, from));
+      unit[x][0] = any_pow2(rel[0] + __shfl_sync(0xFFFFFFFFu, e_page.x, from));
+      unit[x][1] = any_pow2(rel[1] + __shfl_sync(0xFFFFFFFFu, e_page.y, from));
       there[x] = __shfl_sync(0xFFFFFFFFu, ok, from);
     }
     float best[2] = {-INFINITY, -INFINITY};

@@ -41,3 +41,53 @@ def test_elements_of_the_query_that_are_no_numbers_count_as_zero(d, dr, heads, v
     for i, n in enumerate(lens):
         kept = ref.choose(clean[i], view.boxes, table[i], n, budget, 1, 2)
         assert got[i].tolist() == [int(table[i, j]) for j in kept]
+
+
+def _boxes(pages, w, dr, seed):
+    g = torch.Generator().manual_seed(seed)
+    center = torch.randint(-127, 128, (pages, w), generator=g).to(torch.int8)
+    radius = torch.randint(0, 128, (pages, w), generator=g).to(torch.uint8)
+    return center, radius
+
+
+@pytest.mark.parametrize("d,dr", [(512, 64), (256, 32)])
+@pytest.mark.parametrize("e_page,e_q", [(120, 115), (115, 0), (-100, -95), (-100, -30), (0, 0)])
+def test_scores_of_any_size_keep_their_order(d, dr, e_page, e_q):
+    """Boxes and a query at the ends of FP32's range choose what the same ones in its middle do, the request's last
+    pages always among them."""
+    pages, heads, budget = 150, 5, 9
+    center, radius = _boxes(pages, d + dr, dr, 84)
+    spread = torch.randint(0, 3, (pages, 2), generator=torch.Generator().manual_seed(85)).int()
+    table = torch.randperm(pages, generator=torch.Generator().manual_seed(86)).int()[None]
+    q = torch.randn(1, heads, d + dr, generator=torch.Generator().manual_seed(87)).bfloat16()
+    middle = [center.cuda(), radius.cuda(), spread.cuda()]
+    kept = ref.choose(q[0], middle, table[0], pages * 64, budget, 1, 2)
+    cache = ref.random_cache(pages * 64, d, dr, seed=88)
+    far = (center.cuda(), radius.cuda(), (spread + e_page).cuda())
+    got = _select(_view(cache, far), (q.float() * 2.0**e_q).bfloat16(), table, [pages * 64], budget)
+    assert got[0].tolist() == [int(table[0, j]) for j in kept]
+
+
+@pytest.mark.parametrize("part", ["latent", "rotary"])
+def test_a_part_of_the_query_that_is_zero(part):
+    """The other part alone decides, however small it is."""
+    d, dr, pages, budget = 512, 64, 90, 6
+    center, radius = _boxes(pages, d + dr, dr, 89)
+    q = torch.randn(1, 4, d + dr, generator=torch.Generator().manual_seed(90))
+    q[..., slice(0, d) if part == "latent" else slice(d, d + dr)] = 0
+    table = torch.arange(pages).int()[None]
+    zero = torch.zeros(pages, 2, dtype=torch.int32)
+    kept = ref.choose(q[0].bfloat16(), [center, radius, zero], table[0], pages * 64, budget, 1, 2)
+    view = _view(ref.random_cache(pages * 64, d, dr, seed=91), (center.cuda(), radius.cuda(), (zero - 90).cuda()))
+    got = _select(view, (q * 2.0**-95).bfloat16(), table, [pages * 64], budget)
+    assert got[0].tolist() == kept
+
+
+def test_equal_scores_of_any_size_leave_the_last_pages_their_place():
+    d, dr, pages, budget = 256, 32, 100, 8
+    boxes = (torch.full((pages, d + dr), 127, dtype=torch.int8, device="cuda"), torch.full((pages, d + dr), 127, dtype=torch.uint8, device="cuda"),
+             torch.full((pages, 2), 121, dtype=torch.int32, device="cuda"))
+    view = _view(ref.random_cache(pages * 64, d, dr, seed=92), boxes)
+    q = torch.full((1, 3, d + dr), 3e38).bfloat16()
+    got = _select(view, q, torch.arange(pages).int()[None], [pages * 64], budget)
+    assert got[0].tolist() == [0, 1, 2, 3, 4, 5, 98, 99]
