@@ -367,7 +367,8 @@ int rolaq_int4_read(const rolaq_int4_cache* cache, const void* slots, int slots_
  * max(|lo|, |hi|) <= 127 units over the part's columns (1 where all are 0), center =
  * round_half_even((lo + hi) / 2 / unit), radius = ceil(max(hi / unit - center, center - lo / unit)):
  * center -+ radius holds every token's value.  A page outside the pool or a count outside 1..64 is
- * skipped, ROLAQ_DEV_BAD_PAGE.  A NaN value is passed over; a column that holds an infinity has no box.
+ * skipped, ROLAQ_DEV_BAD_PAGE.  A NaN value is passed over; a column that holds an infinity, or nothing but NaN, has
+ * no box (0 -+ 0) and no part in the unit.
  */
 int rolaq_int4_update_boxes(const rolaq_int4_cache* cache, const int32_t* pages, const int32_t* counts, int64_t n,
                             int32_t* err, cudaStream_t stream);

@@ -325,6 +325,8 @@ __global__ void __launch_bounds__(256, 4) boxes_kernel(rolaq_int4_cache cache, c
     } else {
       continue;
     }
+    // no number among the tokens, or an infinity: no box (0 -+ 0), no part in the unit
+    if (!(fabsf(lo[k]) < INFINITY && fabsf(hi[k]) < INFINITY)) lo[k] = hi[k] = 0.f;
     top[col >= D] = fmaxf(top[col >= D], fmaxf(fabsf(lo[k]), fabsf(hi[k])));
   }
 #pragma unroll
