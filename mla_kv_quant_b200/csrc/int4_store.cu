@@ -348,8 +348,9 @@ __global__ void __launch_bounds__(256, 4) boxes_kernel(rolaq_int4_cache cache, c
     const int col = tid + 256 * k;
     if (col >= W) continue;
     const float inv = pow2(-e[col >= D]);
-    const float center = rintf(__fmul_rn(__fmul_rn(__fadd_rn(lo[k], hi[k]), 0.5f), inv));
-    const float radius = ceilf(fmaxf(__fsub_rn(__fmul_rn(hi[k], inv), center), __fsub_rn(center, __fmul_rn(lo[k], inv))));
+    const float a = __fmul_rn(lo[k], inv), b = __fmul_rn(hi[k], inv);  // in units, at most 127: their sum cannot overflow
+    const float center = rintf(__fmul_rn(__fadd_rn(a, b), 0.5f));
+    const float radius = ceilf(fmaxf(__fsub_rn(b, center), __fsub_rn(center, a)));
     cache.box_center[page * W + col] = static_cast<int8_t>(static_cast<int>(fminf(fmaxf(center, -127.f), 127.f)));
     cache.box_radius[page * W + col] = static_cast<uint8_t>(static_cast<int>(fminf(fmaxf(radius, 0.f), 255.f)));
   }

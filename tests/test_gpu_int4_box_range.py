@@ -57,3 +57,21 @@ def test_a_nan_among_numbers_is_passed_over():
     center = torch.round((lo + hi) * 0.5 * unit)
     assert torch.equal(view.boxes[0][0].cpu(), center.to(torch.int8))
     assert torch.equal(view.boxes[1][0].cpu(), torch.ceil(torch.maximum(hi * unit - center, center - lo * unit)).to(torch.uint8))
+
+
+@pytest.mark.parametrize("d,dr", [(512, 64), (256, 32)])
+@pytest.mark.parametrize("sign", [1, -1])
+def test_values_whose_sum_leaves_the_range(d, dr, sign):
+    """Values of about 3e38, all of one sign: the box holds them."""
+    g = torch.Generator().manual_seed(10)
+    codes = torch.randint(0, 256, (64, d // 2), generator=g).to(torch.uint8) | 0x88
+    params = torch.zeros(64, d // 128, 2)
+    params[..., 0] = sign * 2e37
+    rope = (sign * (2.5e38 + 0.5e38 * torch.rand(64, dr, generator=g))).bfloat16()
+    cache = [codes.cuda(), params.cuda(), rope.cuda()]
+    _, lo, hi = _boxes(cache, [0], [64])
+    v = torch.cat([ref.values32(ref.unpack(codes), params), rope.float()], 1).double()
+    assert torch.isfinite(v).all()
+    slack = 2.0**-18 * 2.0**122  # the bounds' own rounding
+    assert (v >= lo - slack).all() and (v <= hi + slack).all()
+    assert ((hi - lo) <= v.amax(0) - v.amin(0) + 2 * 2.0**122).all()
