@@ -1037,8 +1037,9 @@ __global__ void __launch_bounds__(kMergeThreads) merge_kernel(const DecodeArgs a
 struct Shape {
   int tiles, blocks, groups;  // tiles of a CTA, CTAs for all rows, runs of pages (a CTA each and row block)
 };
+int most_tiles(int d) { return d == 512 ? 2 : 5; }
 Shape shape_of(int d, int q_len, int heads) {
-  const int tiles = (q_len * heads + 7) / 8, most = d == 512 ? 2 : 5;
+  const int tiles = (q_len * heads + 7) / 8, most = most_tiles(d);
   const int blocks = (tiles + most - 1) / most;
   return {(tiles + blocks - 1) / blocks, blocks, std::max(1, sm_count() / blocks)};
 }
@@ -1116,9 +1117,12 @@ int launch_tiles(const DecodeArgs& a, cudaStream_t s) {
 
 }  // namespace
 
+// The partials of the largest of all calls of up to this many rows: a CTA's tiles may fall as rows are added (41 rows of
+// D = 256 take two CTAs of 3 tiles, 40 one of 5), so tiles and CTAs are counted apart, each at its most.
 int64_t decode_workspace(int batch, int q_len, int heads, int d) {
-  const Shape s = shape_of(d, q_len, heads);  // groups * blocks <= sm_count() + blocks; that does not shrink as calls grow
-  return kHeaderBytes + int64_t(16) * batch + int64_t(2) * (sm_count() + s.blocks) * s.tiles * 8 * (d + 1) * 4;
+  const int tiles = (q_len * heads + 7) / 8, most = most_tiles(d), blocks = (tiles + most - 1) / most;
+  // groups * blocks <= sm_count() + blocks
+  return kHeaderBytes + int64_t(16) * batch + int64_t(2) * (sm_count() + blocks) * std::min(tiles, most) * 8 * (d + 1) * 4;
 }
 
 int launch_decode(const DecodeArgs& a, cudaStream_t s) {
