@@ -74,7 +74,8 @@ class Int4View:
 
 class Workspace:
     """Device scratch of ``decode`` / ``select_pages`` / ``sparse_decode`` calls of up to this size, and the selection's
-    page table ``sel_table`` int32 ``[batch, budget]`` and lengths ``sel_lens``.  One per stream."""
+    page table ``sel_table`` int32 ``[batch, budget]`` and lengths ``sel_lens`` (a smaller ``sparse_decode`` leaves its
+    choice in ``sel_table[:B, :budget]`` and ``sel_lens[:B]``).  One per stream."""
 
     def __init__(self, view: Int4View, batch: int, q_len: int, heads: int, max_pages: int, budget: int = 0):
         n = _lib.load().rolaq_int4_workspace_bytes(batch, q_len, heads, view.latent_dim, max_pages)
@@ -239,7 +240,8 @@ def select_pages(q: torch.Tensor, view: Int4View, page_table: torch.Tensor, seq_
                  sel_table: torch.Tensor, sel_lens: torch.Tensor, ws: Workspace, keep_first: int = 1,
                  keep_last: int = 2, err: torch.Tensor | None = None) -> None:
     """The ``budget`` pages that each single-token query ``q`` (``[B, H, D + Dr]`` or ``[B, 1, H, D + Dr]``) attends to,
-    as a page table: the first ``keep_first``, the last ``keep_last``, and those whose boxes score highest."""
+    as a page table (``sel_table``, rows at any stride): the first ``keep_first``, the last ``keep_last``, and those whose
+    boxes score highest."""
     if view.boxes is None:
         raise ValueError("the cache has no page boxes")
     if q.dim() not in (3, 4) or q.dim() == 4 and q.shape[1] != 1:
@@ -247,24 +249,29 @@ def select_pages(q: torch.Tensor, view: Int4View, page_table: torch.Tensor, seq_
     shape = q.shape
     b, h = shape[0], shape[-2]
     pt_stride, max_pages = _requests(shape, q, view, page_table, seq_lens)
-    if sel_table.dtype != _I32 or sel_table.shape != (b, budget) or not sel_table.is_contiguous():
-        raise ValueError("sel_table must be contiguous int32 [B, budget]")
+    if sel_table.dtype != _I32 or sel_table.shape != (b, budget) or (budget > 1 and sel_table.stride(1) != 1):
+        raise ValueError("sel_table must be int32 [B, budget] with contiguous rows")
     if sel_lens.dtype != _I32 or sel_lens.shape != (b,) or not sel_lens.is_contiguous():
         raise ValueError("sel_lens must be contiguous int32 [B]")
     _lib.call("rolaq_int4_select_pages", q.data_ptr(), q.stride(0), q.stride(-2), b, h, view._ref,
               page_table.data_ptr(), pt_stride, max_pages, seq_lens.data_ptr(), budget, keep_first,
-              keep_last, ws._ptr, ws.nbytes, sel_table.data_ptr(), budget, sel_lens.data_ptr(), _err(err),
+              keep_last, ws._ptr, ws.nbytes, sel_table.data_ptr(), sel_table.stride(0) if b > 1 else budget,
+              sel_lens.data_ptr(), _err(err),
               _stream(view.index, q, page_table, seq_lens, sel_table, sel_lens, ws.scratch, err))
 
 
 def sparse_decode(q: torch.Tensor, view: Int4View, page_table: torch.Tensor, seq_lens: torch.Tensor, sm_scale: float,
                   budget: int, out: torch.Tensor, lse: torch.Tensor | None, ws: Workspace, keep_first: int = 1,
                   keep_last: int = 2, err: torch.Tensor | None = None) -> None:
-    """``select_pages`` into the workspace's ``sel_table`` / ``sel_lens``, then ``decode`` over what it chose."""
-    if ws.sel_table.shape != (q.shape[0], budget):
-        raise ValueError(f"the workspace was made for batch and budget {tuple(ws.sel_table.shape)}, not {(q.shape[0], budget)}")
-    select_pages(q, view, page_table, seq_lens, budget, ws.sel_table, ws.sel_lens, ws, keep_first, keep_last, err)
-    decode(q, view, ws.sel_table, ws.sel_lens, sm_scale, out, lse, ws, err)
+    """``select_pages`` into the workspace's ``sel_table`` / ``sel_lens`` (their first rows and columns, where the workspace
+    was made for more), then ``decode`` over what it chose."""
+    b, table, lens = q.shape[0], ws.sel_table, ws.sel_lens
+    if table.shape != (b, budget):
+        if b > table.shape[0] or budget > table.shape[1]:
+            raise ValueError(f"the workspace was made for batch and budget {tuple(table.shape)}, not {(b, budget)}")
+        table, lens = table[:b, :budget], lens[:b]
+    select_pages(q, view, page_table, seq_lens, budget, table, lens, ws, keep_first, keep_last, err)
+    decode(q, view, table, lens, sm_scale, out, lse, ws, err)
 
 
 class Int4LatentPool:

@@ -33,3 +33,27 @@ def test_attention_in_a_larger_calls_workspace(d, dr, made, used):
     again, lse2 = torch.empty_like(out), torch.empty_like(lse)
     int4.decode(q, view, table, sl, cases.SM, again, lse2, fit)
     assert torch.equal(out, again) and torch.equal(lse, lse2)
+
+
+@pytest.mark.parametrize("batch,budget", [(4, 5), (2, 9), (1, 9), (3, 4), (4, 9)])
+def test_chosen_pages_in_a_larger_calls_workspace(batch, budget):
+    lens = [4000, 130, 0, 2777]
+    view, table, sl, q, out, lse = _case(lens, 512, 64, 16)
+    table, sl, q, out, lse = (x[:batch] for x in (table, sl, q, out, lse))
+    ws = int4.Workspace(view, 4, 1, 16, table.shape[1], budget=9)
+    fit = int4.Workspace(view, batch, 1, 16, table.shape[1], budget=budget)
+    int4.sparse_decode(q, view, table, sl, cases.SM, budget, out, lse, ws)
+    again, lse2 = torch.empty_like(out), torch.empty_like(lse)
+    int4.sparse_decode(q, view, table, sl, cases.SM, budget, again, lse2, fit)
+    assert torch.equal(ws.sel_table[:batch, :budget], fit.sel_table) and torch.equal(ws.sel_lens[:batch], fit.sel_lens)
+    assert torch.equal(out, again) and torch.equal(lse, lse2)
+
+
+def test_larger_selections_than_the_workspaces_are_refused():
+    view, table, sl, q, out, lse = _case([300, 300], 512, 64, 16)
+    ws = int4.Workspace(view, 1, 1, 16, table.shape[1], budget=4)
+    for n, budget in ((2, 4), (1, 5)):
+        with pytest.raises(ValueError, match="batch and budget"):
+            int4.sparse_decode(q[:n], view, table[:n], sl[:n], cases.SM, budget, out[:n], lse[:n], ws)
+    with pytest.raises(ValueError, match="sel_table"):
+        int4.select_pages(q[:1], view, table[:1], sl[:1], 4, torch.zeros(4, 2, dtype=torch.int32, device="cuda").t()[:1], ws.sel_lens, ws)
