@@ -205,7 +205,7 @@ def _requests(shape, q, view, page_table, seq_lens) -> tuple[int, int]:
         raise ValueError("page_table must be [B, max_pages] with contiguous rows")
     if seq_lens.shape != (b,) or not seq_lens.is_contiguous():
         raise ValueError("seq_lens must be contiguous [B]")
-    return page_table.stride(0), table[1]
+    return page_table.stride(0) if b > 1 else table[1], table[1]  # one row has no stride
 
 
 def decode(q: torch.Tensor, view: Int4View, page_table: torch.Tensor, seq_lens: torch.Tensor, sm_scale: float,

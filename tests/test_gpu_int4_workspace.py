@@ -57,3 +57,14 @@ def test_larger_selections_than_the_workspaces_are_refused():
             int4.sparse_decode(q[:n], view, table[:n], sl[:n], cases.SM, budget, out[:n], lse[:n], ws)
     with pytest.raises(ValueError, match="sel_table"):
         int4.select_pages(q[:1], view, table[:1], sl[:1], 4, torch.zeros(4, 2, dtype=torch.int32, device="cuda").t()[:1], ws.sel_lens, ws)
+
+
+def test_a_table_of_one_row_with_any_row_stride():
+    view, table, sl, q, out, lse = _case([700], 512, 64, 16)
+    ws = int4.Workspace(view, 1, 1, 16, table.shape[1], budget=4)
+    int4.decode(q, view, table, sl, cases.SM, out, lse, ws)
+    again, lse2 = torch.empty_like(out), torch.empty_like(lse)
+    column = table[0].clone()[:, None].t()  # [1, pages], a row stride of 1
+    int4.decode(q, view, column, sl, cases.SM, again, lse2, ws)
+    assert torch.equal(out, again) and torch.equal(lse, lse2)
+    int4.sparse_decode(q, view, column, sl, cases.SM, 4, again, lse2, ws)
