@@ -5,7 +5,8 @@
 //   sum_t P_t v_t = sum_t (P_t s_gt) c_gt - sum_t (P_t s_gt) z_gt
 // so both contractions run on the raw codes, which become operands by ANDs:
 //   - scores: the E4M3 patterns 0..15 are c 2^-9 exactly.  tcgen05.mma of 128 tokens (codes in TMEM) by the query rows
-//     in two E4M3 terms each (hi + lo: exact for BF16 within 2^10 of the row's largest element, 2^-18 of it below),
+//     in two E4M3 terms each (hi + lo: with the row's largest element in [2^7, 2^8) and steps of 2^-9 at the lower end, BF16
+//     within 2^9 of that element is exact, what lies below is off by 2^-17 of it),
 //     one FP32 sum a group; the rotary part BF16 by BF16.  Asynchronous: no warp's issue slots go into it.
 //   - sums: the FP16 patterns 0..255 are that many 2^-24 exactly.  mma.sync m16n8k16 with the codes as rows (c of an
 //     even element, and c + 16 c' of it and the next: c' comes out at the end) and P s in FP16 as columns.
