@@ -91,3 +91,38 @@ def test_equal_scores_of_any_size_leave_the_last_pages_their_place():
     q = torch.full((1, 3, d + dr), 3e38).bfloat16()
     got = _select(view, q, torch.arange(pages).int()[None], [pages * 64], budget)
     assert got[0].tolist() == [0, 1, 2, 3, 4, 5, 98, 99]
+
+
+@pytest.mark.parametrize("d,dr,heads", [(512, 64, 16), (256, 32, 40)])
+def test_scores_from_the_boxes_bound_the_logits_and_the_best_token_is_found(d, dr, heads):
+    """The score that the rule forms of a box and the 8-bit query is no less than any token's logit but for that rounding;
+    a page whose token outweighs all others' scores by itself is chosen."""
+    lens, budget = [4000], 6
+    table, pages = cases.pool_for(lens, 93)
+    g = torch.Generator().manual_seed(94)
+    q = torch.randn(1, heads, d + dr, generator=g).bfloat16()
+    rows, pe = torch.randn(4000, d, generator=g), torch.randn(4000, dr, generator=g)
+    best = 64 * 23 + 17
+    rows[best], pe[best] = 40 * q[0, 1, :d].float(), 40 * q[0, 1, d:].float()
+    cache = cases.stored([rows], [pe], table, lens, pages)
+    view = _view(cache)
+    center, radius, exps = (x.cpu().double() for x in view.boxes)
+    qd = q[0].double()
+    v = torch.cat([ref.values32(ref.unpack(cache[0].cpu()), cache[1].cpu()), cache[2].cpu().float()], 1).double()
+    scores = []
+    for j in range(-(-4000 // 64)):
+        page = int(table[0, j])
+        score = slack = 0
+        for k, part in enumerate((slice(0, d), slice(d, d + dr))):
+            unit = 2.0 ** ref.exponent(float(qd[:, part].abs().max()))
+            q8 = torch.round(qd[:, part] / unit)
+            size = 2.0 ** exps[page, k]
+            score = score + unit * size * (q8 @ center[page, part] + q8.abs() @ radius[page, part])
+            slack = slack + 0.5 * unit * size * (center[page, part].abs() + radius[page, part]).sum() + 2.0**-18 * size * qd[:, part].abs().sum(1)
+        logit = (qd @ v[page * 64 : page * 64 + 64].T).amax(1)
+        assert (logit <= score + slack).all()
+        scores.append(float(score.max()))
+    others = [s for j, s in enumerate(scores) if j != best // 64]
+    assert scores[best // 64] > max(others)
+    got = _select(view, q, table, lens, budget)
+    assert int(table[0, best // 64]) in got[0].tolist()

@@ -68,3 +68,29 @@ def test_a_table_of_one_row_with_any_row_stride():
     int4.decode(q, view, column, sl, cases.SM, again, lse2, ws)
     assert torch.equal(out, again) and torch.equal(lse, lse2)
     int4.sparse_decode(q, view, column, sl, cases.SM, 4, again, lse2, ws)
+
+
+def test_the_calls_allocate_nothing():
+    lens = [900, 77]
+    view, table, sl, q, out, lse = _case(lens, 512, 64, 16)
+    ws = int4.Workspace(view, 4, 1, 16, table.shape[1], budget=8)
+    rows, pe = torch.randn(5, 512, device="cuda"), torch.randn(5, 64, device="cuda").bfloat16()
+    slots, pages = torch.arange(5, device="cuda"), torch.zeros(1, dtype=torch.int32, device="cuda")
+    counts, lo, hi = torch.full((1,), 5, dtype=torch.int32, device="cuda"), torch.empty(1, 576, device="cuda"), torch.empty(1, 576, device="cuda")
+    err = torch.zeros(1, dtype=torch.int32, device="cuda")
+
+    def calls():
+        int4.write(view, rows, pe, slots, err)
+        int4.read(view, slots, rows, pe, err)
+        int4.update_boxes(view, pages, counts, err)
+        int4.read_boxes(view, pages, lo, hi, err)
+        int4.decode(q, view, table, sl, cases.SM, out, lse, ws, err)
+        int4.sparse_decode(q, view, table, sl, cases.SM, 5, out, lse, ws, err=err)
+
+    calls()
+    torch.cuda.synchronize()
+    before = torch.cuda.memory_stats()["allocation.all.allocated"]
+    calls()
+    torch.cuda.synchronize()
+    assert torch.cuda.memory_stats()["allocation.all.allocated"] == before
+    assert err.item() == 0
