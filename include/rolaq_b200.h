@@ -343,7 +343,8 @@ typedef struct rolaq_int4_cache {
  * Quantise rows as they are written: per 128 elements lo / hi = min / max, scale = (hi - lo) / 15
  * (1 where |hi - lo| <= 1e-8), code = clamp(round_half_even((x - lo) / scale), 0, 15), zero =
  * -lo / scale, every operation one IEEE FP32 rounding; k_pe is copied.  Row i goes to slots[i]
- * (outside [0, num_slots): skipped, ROLAQ_DEV_BAD_SLOT).  Rows that share a slot leave any one of them.
+ * (outside [0, num_slots): skipped, ROLAQ_DEV_BAD_SLOT).  Rows that share a slot may leave parts of
+ * different ones there (a slot that nothing reads, for padding); all other slots are as if they were not.
  * A group that holds a NaN or an infinity, or whose hi - lo overflows, gets params that read back as NaN.
  *   c    bf16 or f32 (c_is_f32) [n, D], row stride ld_c;  k_pe bf16 [n, Dr], row stride ld_pe
  *   (both 16-byte aligned, strides multiples of 8 elements);  slots int32 or int64 [n]

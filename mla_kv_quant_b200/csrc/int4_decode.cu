@@ -6,8 +6,8 @@
 // so both contractions run on the raw codes, which become operands by ANDs:
 //   - scores: the E4M3 patterns 0..15 are c 2^-9 exactly.  tcgen05.mma of 128 tokens (codes in TMEM) by the query rows
 //     in two E4M3 terms each (hi + lo: with the row's largest element in [2^7, 2^8) and steps of 2^-9 at the lower end, BF16
-//     within 2^9 of that element is exact, what lies below is off by 2^-17 of it),
-//     one FP32 sum a group; the rotary part BF16 by BF16.  Asynchronous: no warp's issue slots go into it.
+//     within 2^9 of that element is exact, what lies below is off by up to 2^-17 of it), one FP32 sum a group; the rotary
+//     part BF16 by BF16.  Asynchronous: no warp's issue slots go into it.
 //   - sums: the FP16 patterns 0..255 are that many 2^-24 exactly.  mma.sync m16n8k16 with the codes as rows (c of an
 //     even element, and c + 16 c' of it and the next: c' comes out at the end) and P s in FP16 as columns.
 // All sums are FP32, and so is the zeros' share.
@@ -16,8 +16,8 @@
 // a group's unit follows the largest scale, which is enough while each row gives weight to tokens of about that scale.
 // Where the references move, and the scales do not already say that each row has met a P s unit of 2 in each group, the
 // rows' largest are taken too, and a row that has not met that much in a group (its tokens' scales are far below
-// others') gets a power of two of its own there; while one is in use, each tile goes that way.  Equal elements are stored with scale 1 and codes 0: they add nothing but
-// their zero's share, and their scale is not taken for a size.
+// others') gets a power of two of its own there; while one is in use, each tile goes that way.  Equal elements are stored
+// with scale 1 and codes 0: they add nothing but their zero's share, and their scale is not taken for a size.
 //
 // A CTA holds NH tiles of 8 query rows (query tokens x heads; up to two for D = 512, five for D = 256) and walks the
 // pages of one or more requests, two (a tile of 128 tokens) at a time:

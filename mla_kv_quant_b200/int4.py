@@ -134,7 +134,8 @@ def _err(t: torch.Tensor | None):
 
 def write(view: Int4View, c: torch.Tensor, k_pe: torch.Tensor, slots: torch.Tensor,
           err: torch.Tensor | None = None) -> None:
-    """Quantise the rows ``c`` (bf16 or f32 ``[n, D]``) into ``slots`` and copy ``k_pe`` (bf16 ``[n, Dr]``) beside them."""
+    """Quantise the rows ``c`` (bf16 or f32 ``[n, D]``) into ``slots`` and copy ``k_pe`` (bf16 ``[n, Dr]``) beside them.
+    A slot that several rows share holds parts of any of them: only one that nothing reads (padding) may be shared."""
     is64 = _slots(slots)
     n = slots.shape[0]
     if c.dtype != _BF16 and c.dtype != _F32:
