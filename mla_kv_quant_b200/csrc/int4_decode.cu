@@ -619,15 +619,14 @@ __global__ void __launch_bounds__(kThreads, 1)
             odd = fmaf(bf16_lo(v[k]), 0.f, fmaf(bf16_hi(v[k]), 0.f, odd));  // NaN where an element is no finite number
           }
         }
-        {  // the rotary part (0 in the lanes that have none of it): its products alone could be all -inf, a row that sees nothing
-          uint32_t odd_pe = 0;
-          for (const uint32_t v : {pe.x, pe.y, pe.z, pe.w}) asm("fma.rn.bf16x2 %0, %1, %2, %0;" : "+r"(odd_pe) : "r"(v), "r"(0u));
-          odd += bf16_lo(odd_pe) + bf16_hi(odd_pe);
-        }
+        // The rotary part (0 in the lanes that have none of it): its products alone could be all -inf, a row that sees nothing.
+        uint32_t odd_pe = 0;
+        for (const uint32_t v : {pe.x, pe.y, pe.z, pe.w}) asm("fma.rn.bf16x2 %0, %1, %2, %0;" : "+r"(odd_pe) : "r"(v), "r"(0u));
+        const bool no_row = __any_sync(0xFFFFFFFFu, (odd_pe & 0x7FFF7FFFu) != 0);
         top = warp_max_f32(odd != 0.f ? INFINITY : top);
         // 2^k with top 2^k in [2^7, 2^8)
         const float up = top > 0.f ? pow2(min(max(7 - (static_cast<int>(__float_as_uint(top) >> 23) - 127), -120), 100)) : 1.f;
-        if (lane == 0) sh.row_scale[r] = top == INFINITY ? __int_as_float(0x7FC00000) : (qk_scale * 512.f) / up;
+        if (lane == 0) sh.row_scale[r] = top == INFINITY || no_row ? __int_as_float(0x7FC00000) : (qk_scale * 512.f) / up;
 #pragma unroll
         for (int i = 0; i < D / 256; ++i) {
           const uint32_t v[4] = {w[i].x, w[i].y, w[i].z, w[i].w};
