@@ -30,11 +30,12 @@
 // The roles meet in mbarriers only.  The pages of all requests are dealt to the CTAs in one equal run each (a run may
 // begin or end inside a request); what is cut is joined by merge_kernel by log-sum-exp.
 //
-// Measured, 16 heads of 512 + 64, 64 requests of about 16K tokens (417 MB): 135 us, 3.1 TB/s, 47% of a copy's rate.  What
+// Measured, 16 heads of 512 + 64, 64 requests of about 16K tokens (417 MB): 137 to 142 us, 3.0 TB/s, 45 to 47% of a copy's
+// rate (290 while a row of each request has a factor of its own, 340 with a row of zeros among small latents in each tile).  What
 // bounds it is the schedulers: a tile costs each of them about 2000 instructions and 128 mma.sync, and an mma.sync holds
 // back all else for 8 cycles (HMMA + n logic + m FP32 instructions measured 8 + 0.9 n + 1.2 m cycles), 2900 of the 3900
-// cycles a tile takes; memory alone would take 2050.  With the scores on mma.sync too it was 160 us.  Slower, in the same
-// setting: four warps more that only bring codes (179), the adding warps bringing them (166), sharing that (152); one
+// cycles a tile takes; memory alone would take 2050.  With the scores on mma.sync too it was 160 us.  Slower, where this
+// took 135: four warps more that only bring codes (179), the adding warps bringing them (166), sharing that (152); one
 // thread of a divergent branch issuing (167: 2000 cycles for 20 products, against 300 by an elected lane of a warp whose
 // operands are the same in all lanes).
 #include <algorithm>
@@ -52,12 +53,12 @@ namespace {
 // block of 640 is launched with, the others hand some to the token warps.
 constexpr int kTokenWarps = 8, kAddWarps = 8;
 constexpr int kTokens = kTokenWarps * 32, kAdders = kAddWarps * 32, kThreads = kTokens + kAdders + 128;
-constexpr int kAhead = 4;         // pages ahead of their loads that they are called to L2 (24: 143 us against 134)
+constexpr int kAhead = 4;         // pages ahead of their loads that they are called to L2 (24: 157 us against 144, single calls)
 // The least run of pages worth a CTA of its own (a tile), unless the requests are shorter: 31 of 20 tokens, 4 query tokens of
-// 40 heads of 256: 22 us, 33 with two requests a CTA.
+// 40 heads of 256, are 10 us faster with a request a CTA than with two (40 us against 50, single calls).
 constexpr int kMinPages = 2;
-// Scales are brought into [2^2, 2^3); weights and scales may pass their references until P s is 2^15.
-constexpr float kSlack = 1024.f, kScaleTop = 8.f, kScaleSlack = 32.f;
+// Scales are brought into [2^3, 2^4); weights and scales may pass their references until P s is 2^15.
+constexpr float kSlack = 1024.f, kScaleTop = 16.f, kScaleSlack = 32.f;
 constexpr float kLeast = 2.f;       // the least of a row's largest P s unit that needs no factor of the row's own
 constexpr float kZeroShare = 9.094947017729282e-13f;  // 2^-40: a scale below this share of its value's size counts as that much
 constexpr float kNoMax = -3.402823466e38f, kNoUnit = 1.329227995784916e36f;  // references not yet set: the first token passes them
@@ -835,7 +836,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             const float s = fmaxf(fmaxf(sh.red_s[0][k], sh.red_s[1][k]), fmaxf(sh.red_s[2][k], sh.red_s[3][k]));
             keep_unit[k] = 1.f;
             if (s * unit[k] > kScaleTop) {  // bring the largest scale into [kScaleTop / 2, kScaleTop)
-              const float u = pow2(min(max(129 - static_cast<int>(__float_as_uint(s) >> 23), -126), 100));
+              const float u = pow2(min(max(130 - static_cast<int>(__float_as_uint(s) >> 23), -126), 100));
               keep_unit[k] = u / unit[k];
               unit[k] = u;
             }
@@ -847,7 +848,8 @@ __global__ void __launch_bounds__(kThreads, 1)
             const float m = fmaxf(fmaxf(sh.red_m[0][tid], sh.red_m[1][tid]), fmaxf(sh.red_m[2][tid], sh.red_m[3][tid]));
             sh.keep_row[tid] = ex2_approx(old - fmaxf(old, m));
             sh.max[tid] = fmaxf(old, m);
-            if (m < old)  // else the row's largest weight, 1, is in this tile
+            // Else the row's largest weight, 1, is in this tile; or it has seen nothing yet, and its first token moves again.
+            if (m < old && old > kNoMax)
 #pragma unroll
               for (int k = 0; k < NG; ++k) doubt |= !(sh.met[k * ROWS + tid] * keep_unit[k] >= kLeast);
           }
@@ -886,7 +888,8 @@ __global__ void __launch_bounds__(kThreads, 1)
                   for (int x = 0; x < 4; ++x) {
                     const float2 w = mul2(p_val[n][x], both(fabsf(su[k])));
                     const float w0 = warp_max_f32(w.x), w1 = warp_max_f32(w.y);
-                    if (lane == 0) *reinterpret_cast<float2*>(&sh.red_w[quarter][k * ROWS + 8 * (n0 + n) + 2 * x]) = make_float2(w0, w1);
+                    float* at_row = &sh.red_w[quarter][k * ROWS + 8 * (n0 + n) + 2 * x];
+                    if (lane == 0) *reinterpret_cast<float2*>(at_row) = make_float2(w0, w1);
                   }
                 }
             token_sync();
@@ -894,9 +897,10 @@ __global__ void __launch_bounds__(kThreads, 1)
             bool odd = false;
             if (tid < NG * ROWS) {
               const float kept = sh.keep_row[tid % ROWS] * sh.keep_unit[tid / ROWS];
-              const float w = fmaxf(sh.met[tid] * kept, fmaxf(fmaxf(sh.red_w[0][tid], sh.red_w[1][tid]), fmaxf(sh.red_w[2][tid], sh.red_w[3][tid])));
-              odd = !(w >= kLeast);
-              const float f = odd && w > 0.f ? pow2(min(129 - static_cast<int>(__float_as_uint(w) >> 23), 100)) : 1.f;
+              const float here_w = fmaxf(fmaxf(sh.red_w[0][tid], sh.red_w[1][tid]), fmaxf(sh.red_w[2][tid], sh.red_w[3][tid]));
+              const float w = fmaxf(sh.met[tid] * kept, here_w);
+              odd = !(w >= kLeast) && sh.max[tid % ROWS] > kNoMax;  // of a row that has seen something
+              const float f = odd && w > 0.f ? pow2(min(130 - static_cast<int>(__float_as_uint(w) >> 23), 100)) : 1.f;
               sh.met[tid] = w;
               sh.keep[turn][0][tid] = kept * (f / sh.factor[0][tid]);
               sh.factor[0][tid] = f;
@@ -913,7 +917,8 @@ __global__ void __launch_bounds__(kThreads, 1)
                     uint32_t h[4];
 #pragma unroll
                     for (int x = 0; x < 4; ++x) {
-                      const float2 v = mul2(mul2(p_val[n][x], both(su[k])), *reinterpret_cast<const float2*>(&sh.factor[k][8 * (n0 + n) + 2 * x]));
+                      const float2 f = *reinterpret_cast<const float2*>(&sh.factor[k][8 * (n0 + n) + 2 * x]);
+                      const float2 v = mul2(mul2(p_val[n][x], both(su[k])), f);
                       h[x] = pack_half2(v.x, v.y);
                     }
                     *reinterpret_cast<uint4*>(weights_at + (k * NH + n) * C::PTILE) = make_uint4(h[0], h[1], h[2], h[3]);
@@ -1033,7 +1038,7 @@ __global__ void __launch_bounds__(kMergeThreads) merge_kernel(const DecodeArgs a
 
 // A CTA's tiles of 8 query rows: as few CTAs as hold them all, evenly filled.  A page is read once for each, so five
 // tiles (40 rows) in one CTA beat three in each of two even though its registers spill a little: 128 requests of 8K,
-// 40 heads of 256 + 32: 185 us against 238.
+// 40 heads of 256 + 32: 190 us against 241, single calls.
 struct Shape {
   int tiles, blocks, groups;  // tiles of a CTA, CTAs for all rows, runs of pages (a CTA each and row block)
 };
@@ -1091,7 +1096,7 @@ int launch(const DecodeArgs& a, const Shape& shape, cudaStream_t s) {
   cfg.numAttrs = 1;
   if (cudaLaunchKernelEx(&cfg, decode_kernel<D, DR, NH>, codes, rope, a, part, groups, blocks) != cudaSuccess) return ROLAQ_ECUDA;
 
-  // Few requests are cut into many partials: all warps of a CTA share 128 columns of a row then (one request of 128K: 37 us
+  // Few requests are cut into many partials: all warps of a CTA share 128 columns of a row then (one request of 128K: 42 us
   // in all); with less than 8 partials a request a warp each is enough and needs no join.
   const bool wide = groups >= 8 * a.batch;
   const int tasks = a.q_len * a.heads * (D / 128), per_cta = wide ? 1 : kMergeWarps;
