@@ -368,8 +368,9 @@ int rolaq_int4_read(const rolaq_int4_cache* cache, const void* slots, int slots_
  * max(|lo|, |hi|) <= 127 units over the part's columns (1 where all are 0), center =
  * round_half_even((lo + hi) / 2 / unit), radius = ceil(max(hi / unit - center, center - lo / unit)):
  * center -+ radius holds every token's value, but for the FP32 rounding of these differences (2^-18
- * units).  A page outside the pool or a count outside 1..64 is skipped, ROLAQ_DEV_BAD_PAGE.  A NaN value is passed over; a column that holds an infinity, or nothing but NaN, has
- * no box (0 -+ 0) and no part in the unit.
+ * units).  A page outside the pool or a count outside 1..64 is skipped, ROLAQ_DEV_BAD_PAGE.  A NaN value
+ * is passed over; a column that holds an infinity, or nothing but NaN, has no box (0 -+ 0) and no part in
+ * the unit.
  */
 int rolaq_int4_update_boxes(const rolaq_int4_cache* cache, const int32_t* pages, const int32_t* counts, int64_t n,
                             int32_t* err, cudaStream_t stream);
@@ -414,7 +415,8 @@ int rolaq_int4_decode(const uint16_t* q, int64_t q_stride_b, int64_t q_stride_t,
  * e_q the least exponent (>= -100) with max |q| <= 127 * 2^e_q over the part's columns and all heads,
  * an upper bound, up to q's rounding, of any token's q k^T; the sums are whole numbers, so the choice
  * does not depend on their order; an element of q that is no finite number counts as 0.  sel_table[b]
- * holds the chosen pages in the request's order, then -1; sel_lens[b] = (chosen - 1) * 64 + tokens of the last page (0 for an empty request).
+ * holds the chosen pages in the request's order, then -1; sel_lens[b] = (chosen - 1) * 64 + tokens of the
+ * last page (0 for an empty request).
  *   q  bf16 [B, H, D + Dr], strides in elements;  sel_table int32 [B, budget] (row stride sel_stride)
  *   budget >= keep_first + keep_last, keep_last >= 1
  */

@@ -11,7 +11,7 @@
 // times |q8| into the same sums - with the 16 heads of a tile as rows; q8 lies in shared memory in operand order.
 // A request's pages are shared by a few CTAs; the one that scores last keeps the pages: the budget-th largest
 // score by an 8-bit radix search, then, in the pages' order, all above it and the first of its equals.
-// Measured: 64 requests of 256 pages, 16 heads (19 MB of boxes) 18 us, of which memory needs 3: a CTA's one pass over its
+// Measured: 64 requests of 256 pages, 16 heads (19 MB of boxes) 17 us, of which memory needs 3: a CTA's one pass over its
 // pages and the search are chains of dependent steps.
 #include <algorithm>
 #include <atomic>

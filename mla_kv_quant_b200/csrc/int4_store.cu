@@ -50,8 +50,8 @@ __device__ __forceinline__ float max3_nan(float a, float b, float c) {
 // product a y, which is within 1.5 units, within one, the second to the quotient.  All is far from the ends of the range:
 // 6e-10 < scale < 3e37.  That is without branches, where a check of the product for nearness to a half and a division then
 // met the many exact halves of BF16 rows (62 us against 55).
-// Measured: 131072 rows of 512 + 64 in BF16 (206 MB) 55 us, 3.7 TB/s, bound by instructions (61% of the
-// issue slots) and their latency at 32 warps; 76 with a thread's elements side by side and k_pe among the groups.
+// Measured: 131072 rows of 512 + 64 in BF16 (206 MB) 54 us, 3.8 TB/s, in FP32 (340 MB) 61 us, 5.6
+// TB/s; in BF16 bound by instructions (61% of the issue slots) and their latency at 32 warps; 76 with a thread's elements side by side and k_pe among the groups.
 template <typename T, int NG>
 __global__ void __launch_bounds__(256, 4) write_kernel(const T* __restrict__ c, int64_t ld_c,
                                                        const uint16_t* __restrict__ k_pe, int64_t ld_pe, const void* slots,
@@ -138,7 +138,7 @@ __device__ __forceinline__ void store8(uint16_t* p, const float (&v)[8]) {
 
 // Eight threads per unit, a unit being a group of a row or its k_pe, and two rows a thread, `apart` rows from each other, so that
 // twice as much is under way: a thread reads the words of 8 elements at 8 part and at 64 + 8 part of its group, so
-// that a warp's stores are whole lines.  Bound by memory: the rows above back in BF16 43 us, 4.8 TB/s.
+// that a warp's stores are whole lines.  Bound by memory: the rows above back in BF16 41 us, 5.0 TB/s, in FP32 67 us, 5.1 TB/s.
 template <typename T, int NG>
 __global__ void __launch_bounds__(256) read_kernel(rolaq_int4_cache cache, const void* slots, int slots64, int64_t n,
                                                    int64_t apart, T* __restrict__ out, int64_t ld_out,
@@ -237,7 +237,7 @@ __device__ __forceinline__ void widen(const uint32_t (&w)[2], const float2 (&p)[
 
 // One CTA per page: a thread takes a word (8 columns) of every (512 * 8 / W)-th token, the CTA joins them through
 // shared memory.  The operations on an element bound it (the logic pipe, which the minima and maxima need, is 58% full),
-// not memory: 2048 whole pages of 512 + 64 (57 MB) 31 us, 1.8 TB/s; 37 with addresses for pages that may end early, and
+// not memory: 2048 whole pages of 512 + 64 (57 MB) 30 us, 1.9 TB/s; 37 with addresses for pages that may end early, and
 // with a token a step and the rotary part in FP32.
 template <int D, int DR>
 __global__ void __launch_bounds__(256, 4) boxes_kernel(rolaq_int4_cache cache, const int32_t* __restrict__ pages,
