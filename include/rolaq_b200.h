@@ -394,9 +394,10 @@ int64_t rolaq_int4_workspace_bytes(int32_t batch, int32_t q_len, int32_t heads, 
  * a page outside the pool take no weight (ROLAQ_DEV_BAD_PAGE); a length above 64 max_pages is cut
  * (ROLAQ_DEV_BAD_REQ); what a page holds past a request's length is never used.
  * A query's latent part is taken in two E4M3 terms under a power of two of the row: exactly where an element
- * is within 2^9 of the row's largest, else to 2^-17 of that; all sums are FP32; a weight times its group's scale is held
- * in FP16 for the value product, to 11 bits or to 2^-26 of the largest such product that the row has met in the group,
- * whatever other tokens and rows hold.  A query row that holds a NaN or an infinity gets NaN, and only that row.
+ * is within 2^9 of the row's largest, else to 2^-17 of that (to 2^-110 in a row whose largest is below
+ * 2^-93); all sums are FP32; a weight times its group's scale is held in FP16 for the value product, to 11
+ * bits or to 2^-26 of the largest such product that the row has met in the group, whatever other tokens
+ * and rows hold.  A query row that holds a NaN or an infinity gets NaN, and only that row.
  *   q    bf16 [B, q_len, H, D + Dr], strides in elements (multiples of 8), 16-byte aligned
  *   out  bf16 [B, q_len, H, D], likewise;  lse f32 [B, q_len, H] contiguous (natural log; NULL: not wanted)
  */

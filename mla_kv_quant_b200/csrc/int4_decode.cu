@@ -625,7 +625,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         for (const uint32_t v : {pe.x, pe.y, pe.z, pe.w}) asm("fma.rn.bf16x2 %0, %1, %2, %0;" : "+r"(odd_pe) : "r"(v), "r"(0u));
         const bool no_row = __any_sync(0xFFFFFFFFu, (odd_pe & 0x7FFF7FFFu) != 0);
         top = warp_max_f32(odd != 0.f ? INFINITY : top);
-        // 2^k with top 2^k in [2^7, 2^8)
+        // 2^k with top 2^k in [2^7, 2^8), at most 2^100: scores of smaller rows stay normal numbers in row_scale
         const float up = top > 0.f ? pow2(min(max(7 - (static_cast<int>(__float_as_uint(top) >> 23) - 127), -120), 100)) : 1.f;
         if (lane == 0) sh.row_scale[r] = top == INFINITY || no_row ? __int_as_float(0x7FC00000) : (qk_scale * 512.f) / up;
 #pragma unroll
